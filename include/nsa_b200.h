@@ -438,6 +438,122 @@ int nsa_select_blocks_cached(const void* Qb, const void* Kb, int32_t* idx, int B
                              int force_first, int force_local, int shared_per_group, int dtype,
                              nsa_stream_t stream);
 
+/* ---------------------------------------------------------------- the layer around the attention
+ * What a decoder layer computes before, between and after its attention calls (the reference leaves these to plain
+ * torch modules, nsa/model/llama_dense.py:19-134): norm, rotary embedding, projections, gated feed-forward block.
+ * Rows are dense; pointers may have any alignment (16-byte aligned rows take the fast kernels).  Workspaces are
+ * device memory, 256-byte aligned, contents free before and after. */
+#define NSA_ACT_NONE 0
+#define NSA_ACT_SILU 1
+#define NSA_ACT_GELU_TANH 2 /* 0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */
+#define NSA_ACT_RELU 3
+
+/* Root-mean-square norm behind the residual's addition, rows of `hidden` elements:
+ *   h = round(x + residual) in the residual's type (h = x where residual is NULL),
+ *   y = h / sqrt(mean(h^2) + eps) * weight.
+ * x: bf16, fp16 or fp32; residual and h: x's type or fp32; weight: x's type or fp32; y: x's type, or NSA_FP8_* with one
+ * fp32 scale per row (scale = max(max|y|, 1e-12) / fmt_max, q = round(y / scale); a row that holds NaN gets a NaN
+ * scale).  rstd [rows] (NULL: not wanted) is kept for the backward.  All arithmetic fp32, sums in a fixed order. */
+typedef struct nsa_norm_args {
+  const void *x, *residual, *weight;
+  void *y, *h;
+  float *scale, *rstd;
+  int64_t rows;
+  int32_t hidden;
+  int32_t x_dtype, res_dtype, w_dtype, y_dtype;
+  float eps;
+} nsa_norm_args;
+int nsa_rms_norm(const nsa_norm_args* args, nsa_stream_t stream);
+
+/* Gradients of nsa_rms_norm (16-bit or fp32 y): dy (x's type), dh (h's type, NULL: none) -> dx (x's type), the same values as
+ * dres in the residual's type where that differs (NULL: not wanted), dweight (NULL: not wanted).  h: the normed
+ * stream (x itself without a residual; res_dtype is then x's).  ws: nsa_rms_norm_bwd_ws_bytes(rows, hidden) bytes.
+ * Repeats bit for bit. */
+typedef struct nsa_norm_bwd_args {
+  const void *dy, *dh, *h, *weight;
+  const float* rstd;
+  void *dx, *dres, *dweight, *ws;
+  int64_t ws_bytes, rows;
+  int32_t hidden;
+  int32_t x_dtype, res_dtype, w_dtype;
+} nsa_norm_bwd_args;
+int64_t nsa_rms_norm_bwd_ws_bytes(int64_t rows, int hidden);
+int nsa_rms_norm_bwd(const nsa_norm_bwd_args* args, nsa_stream_t stream);
+
+/* x [rows, n] -> fp8 values and one fp32 scale per row, by the rule of nsa_rms_norm's fp8 result: the weights of
+ * nsa_linear with fp8 operands. */
+int nsa_quantize_rows_fp8(const void* x, void* q, float* scale, int64_t rows, int n, int x_dtype, int fmt, nsa_stream_t stream);
+
+/* Rotary embedding whose D/2 frequencies are dealt out to n_axes (1..8) position axes: frequency j turns by
+ * positions[axis(j), b, t] * inv_freq[j], axis a owning sections[a] consecutive frequencies (they add up to D/2).
+ * Forward: q [B,T,H,D], k and v [B,T,Hkv,D] with any batch and token pitch (elements; heads D apart) -> rotated q and k,
+ * unrotated v as [B,heads,T,D] in y_dtype (bf16 / fp16).  backward != 0: q, k, v are gradients [B,heads,T,D] in y_dtype and
+ * the outputs are dense [B,T,heads,D] gradients in x_dtype (the pitches are then unused).
+ * positions [n_axes,B,T] int32 or int64 (pos64); inv_freq [D/2] fp64.  D even, at most 1024.  Angles are reduced in fp64. */
+typedef struct nsa_rope_axes_args {
+  const void *q, *k, *v;
+  void *q_out, *k_out, *v_out;
+  const void* positions;
+  const double* inv_freq;
+  int64_t q_batch, q_token, k_batch, k_token, v_batch, v_token;
+  int32_t B, T, H, Hkv, D;
+  int32_t n_axes, sections[8];
+  int32_t pos64, x_dtype, y_dtype, backward;
+} nsa_rope_axes_args;
+int nsa_rope_axes(const nsa_rope_axes_args* args, nsa_stream_t stream);
+
+/* y = act(x w^T + bias) + residual:  x [M,K], w [N,K], bias [N], residual and y [M,N].
+ * x and w: both bf16 or both fp16 (bias, residual and y share the type); or both e4m3 or both e5m2 with x_scale [M] and w_scale
+ * [N] (y, bias and residual in y_dtype).  bias, residual NULL: none.  z (NULL: not wanted; 16-bit operands): act's
+ * argument, kept for the backward.  Sums, bias, activation and residual in fp32, one rounding.
+ * ws: nsa_linear_ws_bytes(&args) bytes (the pointers may still be NULL when it is asked; negative: bad arguments). */
+typedef struct nsa_linear_args {
+  const void *x, *w, *bias, *residual;
+  const float *x_scale, *w_scale;
+  void *y, *z, *ws;
+  int64_t ws_bytes;
+  int32_t M, N, K;
+  int32_t dtype, y_dtype, act;
+} nsa_linear_args;
+int64_t nsa_linear_ws_bytes(const nsa_linear_args* args);
+int nsa_linear(const nsa_linear_args* args, nsa_stream_t stream);
+
+/* Gradients of nsa_linear (16-bit operands): dx [M,K], dw [N,K], dbias [N], each NULL if not wanted; residual's is dy. z may be
+ * NULL where act is none.  Repeats bit for bit. */
+typedef struct nsa_linear_bwd_args {
+  const void *dy, *x, *w, *z;
+  void *dx, *dw, *dbias, *ws;
+  int64_t ws_bytes;
+  int32_t M, N, K;
+  int32_t dtype, act;
+} nsa_linear_bwd_args;
+int64_t nsa_linear_bwd_ws_bytes(const nsa_linear_bwd_args* args);
+int nsa_linear_bwd(const nsa_linear_bwd_args* args, nsa_stream_t stream);
+
+/* Gated feed-forward block:  y = (act(x wg^T) * (x wu^T)) wd^T + residual,  x, residual, y [M,N], wg and wu [F,N], wd [N,F], all of
+ * one 16-bit type.  The gated product is held in that type between the two matrix products.  g, u [M,F] (both NULL: not
+ * wanted): the two products, kept for the backward.  ws as for nsa_linear. */
+typedef struct nsa_gated_mlp_args {
+  const void *x, *wg, *wu, *wd, *residual;
+  void *y, *g, *u, *ws;
+  int64_t ws_bytes;
+  int32_t M, N, F;
+  int32_t dtype, act;
+} nsa_gated_mlp_args;
+int64_t nsa_gated_mlp_ws_bytes(const nsa_gated_mlp_args* args);
+int nsa_gated_mlp(const nsa_gated_mlp_args* args, nsa_stream_t stream);
+
+/* Its gradients: dx [M,N], dwg and dwu [F,N], dwd [N,F], each NULL if not wanted; residual's is dy.  Repeats bit for bit. */
+typedef struct nsa_gated_mlp_bwd_args {
+  const void *dy, *x, *wg, *wu, *wd, *g, *u;
+  void *dx, *dwg, *dwu, *dwd, *ws;
+  int64_t ws_bytes;
+  int32_t M, N, F;
+  int32_t dtype, act;
+} nsa_gated_mlp_bwd_args;
+int64_t nsa_gated_mlp_bwd_ws_bytes(const nsa_gated_mlp_bwd_args* args);
+int nsa_gated_mlp_bwd(const nsa_gated_mlp_bwd_args* args, nsa_stream_t stream);
+
 /* Strided copy between host and device on `stream`: `rows` rows of `row_bytes` bytes, row r at
  * dst + r*dst_pitch / src + r*src_pitch; to_device = 1 host->device, 0 device->host.  Asynchronous when
  * the host side is pinned.  Lets the host-tensor entry point move the [heads, chunk, D] slab of one

@@ -19,6 +19,7 @@ ABI_VERSION = 7      # nsa_abi_version() of the library these struct mirrors and
 BF16, FP16, FP8_E4M3, FP8_E5M2, FP32 = 0, 1, 2, 3, 4
 BRANCH_COMPRESSED, BRANCH_SELECTED, BRANCH_SLIDING = 1, 2, 4
 GATE_SIGMOID, GATE_SOFTMAX = 0, 1
+ACTIVATIONS = {None: 0, "silu": 1, "gelu_tanh": 2, "relu": 3}
 ENGINE_AUTO, ENGINE_GENERIC, ENGINE_TCGEN05 = 0, 1, 2
 IO_OUT_BTHD, IO_GATES_BTHD = 1, 2
 
@@ -100,6 +101,72 @@ class DecodeArgs(C.Structure):
     ]
 
 
+class NormArgs(C.Structure):
+    """Mirror of `struct nsa_norm_args`."""
+    _fields_ = [
+        ("x", C.c_void_p), ("residual", C.c_void_p), ("weight", C.c_void_p), ("y", C.c_void_p), ("h", C.c_void_p),
+        ("scale", C.c_void_p), ("rstd", C.c_void_p), ("rows", C.c_int64), ("hidden", C.c_int32),
+        ("x_dtype", C.c_int32), ("res_dtype", C.c_int32), ("w_dtype", C.c_int32), ("y_dtype", C.c_int32), ("eps", C.c_float),
+    ]
+
+
+class NormBwdArgs(C.Structure):
+    """Mirror of `struct nsa_norm_bwd_args`."""
+    _fields_ = [
+        ("dy", C.c_void_p), ("dh", C.c_void_p), ("h", C.c_void_p), ("weight", C.c_void_p), ("rstd", C.c_void_p),
+        ("dx", C.c_void_p), ("dres", C.c_void_p), ("dweight", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_int64),
+        ("rows", C.c_int64), ("hidden", C.c_int32), ("x_dtype", C.c_int32), ("res_dtype", C.c_int32), ("w_dtype", C.c_int32),
+    ]
+
+
+class RopeAxesArgs(C.Structure):
+    """Mirror of `struct nsa_rope_axes_args`."""
+    _fields_ = [
+        ("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("q_out", C.c_void_p), ("k_out", C.c_void_p), ("v_out", C.c_void_p),
+        ("positions", C.c_void_p), ("inv_freq", C.c_void_p),
+        ("q_batch", C.c_int64), ("q_token", C.c_int64), ("k_batch", C.c_int64), ("k_token", C.c_int64), ("v_batch", C.c_int64), ("v_token", C.c_int64),
+        ("B", C.c_int32), ("T", C.c_int32), ("H", C.c_int32), ("Hkv", C.c_int32), ("D", C.c_int32),
+        ("n_axes", C.c_int32), ("sections", C.c_int32 * 8),
+        ("pos64", C.c_int32), ("x_dtype", C.c_int32), ("y_dtype", C.c_int32), ("backward", C.c_int32),
+    ]
+
+
+class LinearArgs(C.Structure):
+    """Mirror of `struct nsa_linear_args`."""
+    _fields_ = [
+        ("x", C.c_void_p), ("w", C.c_void_p), ("bias", C.c_void_p), ("residual", C.c_void_p), ("x_scale", C.c_void_p), ("w_scale", C.c_void_p),
+        ("y", C.c_void_p), ("z", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_int64),
+        ("M", C.c_int32), ("N", C.c_int32), ("K", C.c_int32), ("dtype", C.c_int32), ("y_dtype", C.c_int32), ("act", C.c_int32),
+    ]
+
+
+class LinearBwdArgs(C.Structure):
+    """Mirror of `struct nsa_linear_bwd_args`."""
+    _fields_ = [
+        ("dy", C.c_void_p), ("x", C.c_void_p), ("w", C.c_void_p), ("z", C.c_void_p), ("dx", C.c_void_p), ("dw", C.c_void_p), ("dbias", C.c_void_p),
+        ("ws", C.c_void_p), ("ws_bytes", C.c_int64),
+        ("M", C.c_int32), ("N", C.c_int32), ("K", C.c_int32), ("dtype", C.c_int32), ("act", C.c_int32),
+    ]
+
+
+class GatedMlpArgs(C.Structure):
+    """Mirror of `struct nsa_gated_mlp_args`."""
+    _fields_ = [
+        ("x", C.c_void_p), ("wg", C.c_void_p), ("wu", C.c_void_p), ("wd", C.c_void_p), ("residual", C.c_void_p),
+        ("y", C.c_void_p), ("g", C.c_void_p), ("u", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_int64),
+        ("M", C.c_int32), ("N", C.c_int32), ("F", C.c_int32), ("dtype", C.c_int32), ("act", C.c_int32),
+    ]
+
+
+class GatedMlpBwdArgs(C.Structure):
+    """Mirror of `struct nsa_gated_mlp_bwd_args`."""
+    _fields_ = [
+        ("dy", C.c_void_p), ("x", C.c_void_p), ("wg", C.c_void_p), ("wu", C.c_void_p), ("wd", C.c_void_p), ("g", C.c_void_p), ("u", C.c_void_p),
+        ("dx", C.c_void_p), ("dwg", C.c_void_p), ("dwu", C.c_void_p), ("dwd", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_int64),
+        ("M", C.c_int32), ("N", C.c_int32), ("F", C.c_int32), ("dtype", C.c_int32), ("act", C.c_int32),
+    ]
+
+
 _vp, _i, _f, _i64 = C.c_void_p, C.c_int, C.c_float, C.c_int64
 
 PROTOTYPES = {
@@ -139,6 +206,19 @@ PROTOTYPES = {
     "nsa_cache_append": (_i, [_vp] * 7 + [_i] * 12 + [_vp]),
     "nsa_cache_append_dev": (_i, [_vp] * 7 + [_i] * 4 + [_vp] + [_i] * 7 + [_vp]),
     "nsa_select_blocks_cached": (_i, [_vp, _vp, _vp, _i, _i, _i, _i, _i, _i, _i, _i, _i, _vp, _f, _i, _i, _i, _i, _vp]),
+    "nsa_rms_norm": (_i, [C.POINTER(NormArgs), _vp]),
+    "nsa_rms_norm_bwd_ws_bytes": (_i64, [_i64, _i]),
+    "nsa_rms_norm_bwd": (_i, [C.POINTER(NormBwdArgs), _vp]),
+    "nsa_quantize_rows_fp8": (_i, [_vp, _vp, _vp, _i64, _i, _i, _i, _vp]),
+    "nsa_rope_axes": (_i, [C.POINTER(RopeAxesArgs), _vp]),
+    "nsa_linear_ws_bytes": (_i64, [C.POINTER(LinearArgs)]),
+    "nsa_linear": (_i, [C.POINTER(LinearArgs), _vp]),
+    "nsa_linear_bwd_ws_bytes": (_i64, [C.POINTER(LinearBwdArgs)]),
+    "nsa_linear_bwd": (_i, [C.POINTER(LinearBwdArgs), _vp]),
+    "nsa_gated_mlp_ws_bytes": (_i64, [C.POINTER(GatedMlpArgs)]),
+    "nsa_gated_mlp": (_i, [C.POINTER(GatedMlpArgs), _vp]),
+    "nsa_gated_mlp_bwd_ws_bytes": (_i64, [C.POINTER(GatedMlpBwdArgs)]),
+    "nsa_gated_mlp_bwd": (_i, [C.POINTER(GatedMlpBwdArgs), _vp]),
     "nsa_memcpy_2d": (_i, [_vp, C.c_size_t, _vp, C.c_size_t, C.c_size_t, C.c_size_t, _i, _vp]),
 }
 

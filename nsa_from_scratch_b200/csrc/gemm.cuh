@@ -1,0 +1,165 @@
+// What the matrix-product kernels of the layer share: the problem they are given, the activations, and the epilogue that
+// turns fp32 sums into results, eight consecutive columns of a row at a time.
+//
+//   out[m,n] = epilogue( sum_k A[m,k] * B[n,k] )
+//
+// A and B are 16-bit (fp32 sums) or fp8 (e4m3 / e5m2, fp32 sums); each is stored with the contraction k along its rows
+// ("k-major", [rows][k]) or down its columns ("mn-major", [k][rows]): x W^T, dy W and dy^T x are the same kernel.
+// A contraction may come in two segments (A0 B0^T + A1 B1^T: the gradient that reaches x through gate and up).
+#pragma once
+#include "common.cuh"
+
+namespace nsa {
+
+enum { ACT_NONE = 0, ACT_SILU = 1, ACT_GELU_TANH = 2, ACT_RELU = 3 };
+enum {
+  EPI_LINEAR = 0,   // v = acc * xs[m] * ws[n] + bias[n]; z = v (optional); y = act(v) + residual
+  EPI_GLU = 1,      // two products g, u of the same A: y = act(g) * u; g and u themselves are optional results
+  EPI_GLU_BWD = 2   // acc = dh: y = dg = dh * u * act'(g), o1 = du = dh * act(g), o2 = h = act(g) * u, from stored g and u
+};
+
+// p = act(z), d = act'(z).  exp overflows to infinity for large -z and the quotient is then 0, as it should be.
+__device__ __forceinline__ float sigmoid_f(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+__device__ __forceinline__ float tanh_f(float z) { return 1.f - __fdividef(2.f, 1.f + __expf(2.f * z)); }
+constexpr float kGeluC = 0.7978845608028654f;   // sqrt(2 / pi)
+constexpr float kGeluA = 0.044715f;             // the cubic's coefficient in gelu's tanh form
+
+__device__ __forceinline__ float act_f(float z, int act) {
+  if (act == ACT_SILU) return z * sigmoid_f(z);
+  if (act == ACT_GELU_TANH) return 0.5f * z * (1.f + tanh_f(kGeluC * (z + kGeluA * z * z * z)));
+  // a comparison that NaN fails keeps NaN
+  if (act == ACT_RELU) return z < 0.f ? 0.f : z;
+  return z;
+}
+__device__ __forceinline__ void act_both(float z, int act, float& p, float& d) {
+  if (act == ACT_SILU) {
+    const float s = sigmoid_f(z);
+    p = z * s;
+    d = s == 1.f ? 1.f : fmaf(p, 1.f - s, s);          // a stored z that overflowed fp16 to infinity: slope 1, not inf * 0
+  } else if (act == ACT_GELU_TANH) {
+    const float t = tanh_f(kGeluC * (z + kGeluA * z * z * z));
+    p = 0.5f * z * (1.f + t);
+    const float q = 1.f - t * t;
+    d = 0.5f * (1.f + t) + (q == 0.f ? 0.f : 0.5f * z * q * kGeluC * (1.f + 3.f * kGeluA * z * z));
+  } else if (act == ACT_RELU) {
+    p = z < 0.f ? 0.f : z;
+    d = z > 0.f ? 1.f : 0.f;
+  } else {
+    p = z;
+    d = 1.f;
+  }
+}
+
+struct Epi {
+  int mode, act;
+  int M, N;                      // results are [M][N], dense
+  int vec;                       // 1: N % 8 == 0 and every 16-bit pointer below is 16-byte aligned
+  const void *bias, *residual;   // EPI_LINEAR; out type; NULL: none
+  const float *xs, *ws;          // EPI_LINEAR: scales per row and per column of the sums; NULL: none
+  const void *i0, *i1;           // EPI_GLU_BWD: stored g and u
+  void *y, *o1, *o2;             // LINEAR: y, z (NULL: not wanted), -;  GLU: h, g, u (NULL: not wanted);  GLU_BWD: dg, du, h
+};
+
+struct GemmProblem {
+  const void *A[2], *B[2];       // EPI_GLU: B[0], B[1] are the two weights (one segment)
+  int segments;                  // 1 or 2
+  int a_mn, b_mn;                // 1: stored [K][M] / [K][N]
+  int M, N, K;                   // K: contraction length of each segment
+  long long lda, ldb;            // elements between stored rows
+  int dtype;                     // NSA_BF16, NSA_FP16, or an fp8 type of both operands
+  int out_dtype;                 // NSA_BF16 or NSA_FP16
+  Epi e;
+};
+
+template <typename T>
+__device__ __forceinline__ void load8(const void* p, long long i, int n, int vec, float (&v)[8]) {
+  const T* q = reinterpret_cast<const T*>(p) + i;
+  if (vec) {
+    const uint4 a = *reinterpret_cast<const uint4*>(q);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { const float2 f = Elem<T>::unpack(w[e]); v[2 * e] = f.x; v[2 * e + 1] = f.y; }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < n ? Elem<T>::to_f(q[e]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(void* p, long long i, int n, int vec, const float (&v)[8]) {
+  T* q = reinterpret_cast<T*>(p) + i;
+  if (vec) {
+    *reinterpret_cast<uint4*>(q) = make_uint4(Elem<T>::pack(v[0], v[1]), Elem<T>::pack(v[2], v[3]), Elem<T>::pack(v[4], v[5]), Elem<T>::pack(v[6], v[7]));
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (e < n) q[e] = Elem<T>::from_f(v[e]);
+  }
+}
+
+// Columns col..col+7 (those below N) of row `row`: a = fp32 sums, b = the second product's (EPI_GLU).  Everything is
+// formed in fp32 and rounded once where it is stored.
+template <typename T, int MODE>
+__device__ __forceinline__ void epilogue8(const Epi& e, long long row, int col, float (&a)[8], const float (&b)[8]) {
+  const int n = e.N - col;
+  if (row >= e.M || n <= 0) return;
+  const long long at = row * e.N + col;
+  if constexpr (MODE == EPI_LINEAR) {
+    if (e.xs != nullptr) {
+      const float s = e.xs[row];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] *= i < n ? s * e.ws[col + i] : 0.f;
+    }
+    if (e.bias != nullptr) {
+      float c[8];
+      load8<T>(e.bias, col, n, e.vec, c);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] += c[i];
+    }
+    if (e.o1 != nullptr) store8<T>(e.o1, at, n, e.vec, a);
+    if (e.act != ACT_NONE) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] = act_f(a[i], e.act);
+    }
+    if (e.residual != nullptr) {
+      float c[8];
+      load8<T>(e.residual, at, n, e.vec, c);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] += c[i];
+    }
+    store8<T>(e.y, at, n, e.vec, a);
+  } else if constexpr (MODE == EPI_GLU) {
+    if (e.o1 != nullptr) { store8<T>(e.o1, at, n, e.vec, a); store8<T>(e.o2, at, n, e.vec, b); }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = act_f(a[i], e.act) * b[i];
+    store8<T>(e.y, at, n, e.vec, a);
+  } else {
+    float g[8], u[8], du[8], h[8];
+    load8<T>(e.i0, at, n, e.vec, g);
+    load8<T>(e.i1, at, n, e.vec, u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float p, d;
+      act_both(g[i], e.act, p, d);
+      du[i] = a[i] * p;
+      h[i] = p * u[i];
+      a[i] = a[i] * u[i] * d;
+    }
+    store8<T>(e.y, at, n, e.vec, a);
+    store8<T>(e.o1, at, n, e.vec, du);
+    store8<T>(e.o2, at, n, e.vec, h);
+  }
+}
+
+static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+static inline int sm_count() {
+  int dev = 0, sms = 148;
+  cudaGetDevice(&dev);
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  return sms;
+}
+
+int gemm_generic(const GemmProblem& p, cudaStream_t st);
+int column_sum(const float* part, void* out, int parts, int N, int dt, cudaStream_t st);   // norm.cu
+
+}  // namespace nsa

@@ -84,6 +84,21 @@ def _need_cuda(*ts: Tensor) -> None:
             raise RuntimeError("nsa_from_scratch_b200 kernels need CUDA tensors (there is no CPU path)")
 
 
+def _same_device(x: Tensor, **others: Optional[Tensor]) -> None:
+    """Every operand lies where `x` does."""
+    for name, t in others.items():
+        if t is not None and t.device != x.device:
+            _need_cuda(t)
+            raise ValueError(f"{name} is on {t.device}, the first operand on {x.device}")
+
+
+def activation_code(name: Optional[str]) -> int:
+    try:
+        return L.ACTIVATIONS[name]
+    except KeyError:
+        raise ValueError(f"unknown activation: {name}") from None
+
+
 def softmax_scale(D: int, scale: Optional[float]) -> float:
     return float(scale) if scale is not None else 1.0 / math.sqrt(D)
 

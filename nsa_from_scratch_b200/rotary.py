@@ -1,0 +1,94 @@
+"""Rotary embedding with several position axes (time, height and width of image and video tokens), from the projections'
+token-major tensors to the attention's head-major ones: `rope_to_heads` of q, k and v in one launch, with the angles
+formed from integer positions instead of read from tables, and with gradients.
+
+Frequency j of D/2 turns by positions[axis(j), b, t] * inv_freq[j]; axis a owns sections[a] consecutive frequencies.
+One axis is the ordinary rotary embedding (nsa/model/llama_dense.py:19-37) at arbitrary positions."""
+from __future__ import annotations
+
+import ctypes as C
+from typing import Sequence, Tuple
+
+import torch
+from torch import Tensor
+
+from . import _lib as L
+from . import ops
+
+
+def rope_frequencies(head_dim: int, base: float = 10000.0, device="cuda") -> Tensor:
+    """inv_freq [D/2] fp64: base ** (-2 j / D), the frequencies of `rope_cache`.  Scale or replace them freely."""
+    if head_dim <= 0 or head_dim % 2:
+        raise ValueError(f"rope_frequencies: head_dim {head_dim} must be even")
+    return float(base) ** (-torch.arange(0, head_dim, 2, device=device, dtype=torch.float64) / head_dim)
+
+
+def _pitched(t: Tensor, name: str) -> Tensor:
+    """Heads and columns dense; the batch and token pitch may be anything (slices of a packed projection)."""
+    D = t.shape[-1]
+    if (t.stride(3) == 1 or D == 1) and (t.stride(2) == D or t.shape[2] == 1):
+        return t
+    return ops._dense(t, name)
+
+
+def _launch(q, k, v, positions, inv_freq, sections, x_dtype, y_dtype, backward):
+    B, H, Hkv, D = q.shape[0], q.shape[1 if backward else 2], k.shape[1 if backward else 2], q.shape[3]
+    T = q.shape[2 if backward else 1]
+    shape = (lambda h: (B, T, h, D)) if backward else (lambda h: (B, h, T, D))
+    out = [torch.empty(shape(h), device=q.device, dtype=x_dtype if backward else y_dtype) for h in (H, Hkv, Hkv)]
+    a = L.RopeAxesArgs(q.data_ptr(), k.data_ptr(), v.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), out[2].data_ptr(),
+                       positions.data_ptr(), inv_freq.data_ptr(), q.stride(0), q.stride(1), k.stride(0), k.stride(1), v.stride(0), v.stride(1),
+                       B, T, H, Hkv, D, len(sections), (C.c_int32 * 8)(*sections), int(positions.dtype == torch.int64),
+                       L.dtype_code(x_dtype), L.dtype_code(y_dtype), int(backward))
+    with L.on_device(q):
+        L.check(L.load().nsa_rope_axes(C.byref(a), L.stream_ptr()), "nsa_rope_axes")
+    return tuple(out)
+
+
+class _RopeAxesFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, positions, inv_freq, sections, dtype):
+        ctx.save_for_backward(positions, inv_freq)
+        ctx.sections, ctx.x_dtype, ctx.dtype = sections, q.dtype, dtype
+        return _launch(q, k, v, positions, inv_freq, sections, q.dtype, dtype, False)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq, dk, dv):
+        positions, inv_freq = ctx.saved_tensors
+        grads = _launch(dq.contiguous(), dk.contiguous(), dv.contiguous(), positions, inv_freq, ctx.sections, ctx.x_dtype, ctx.dtype, True)
+        return (*grads, None, None, None, None)
+
+
+def rope_axes_to_heads(q: Tensor, k: Tensor, v: Tensor, positions: Tensor, inv_freq: Tensor, sections: Sequence[int], *,
+                       dtype: torch.dtype = torch.bfloat16) -> Tuple[Tensor, Tensor, Tensor]:
+    """q [B,T,H,D], k and v [B,T,Hkv,D] as the projections leave them (one dtype: fp32, bf16 or fp16; slices of a packed
+    projection are read where they lie), positions [axes,B,T] int32 or int64, inv_freq [D/2] (fp64; fp32 is converted),
+    sections: frequencies of each axis, D/2 in all.  Returns q and k rotated, v as it is, [B,heads,T,D] in `dtype` (bf16 or
+    fp16): fp32 inside, one rounding.  Differentiable wrt q, k and v."""
+    ops._need_cuda(q, k, v, positions, inv_freq)
+    ops._same_device(q, k=k, v=v, positions=positions, inv_freq=inv_freq)
+    if q.dim() != 4:
+        raise ValueError(f"rope_axes_to_heads: q must be [B,T,H,D], got {tuple(q.shape)}")
+    B, T, H, D = q.shape
+    if k.dim() != 4 or k.shape[:2] != (B, T) or k.shape[3] != D or v.shape != k.shape:
+        raise ValueError(f"rope_axes_to_heads: k/v shapes {tuple(k.shape)}/{tuple(v.shape)} do not match q {tuple(q.shape)}")
+    if k.dtype != q.dtype or v.dtype != q.dtype or q.dtype not in (torch.float32, torch.bfloat16, torch.float16):
+        raise TypeError("rope_axes_to_heads: q, k and v must share a dtype (fp32, bf16 or fp16)")
+    if dtype not in ops._16:
+        raise TypeError(f"rope_axes_to_heads: the result is bf16 or fp16, not {dtype}")
+    sections = tuple(int(s) for s in sections)
+    if D % 2 or not 1 <= len(sections) <= 8 or min(sections) < 0 or sum(sections) != D // 2:
+        raise ValueError(f"rope_axes_to_heads: 1 to 8 sections that add up to D/2 = {D / 2:g} are needed, got {sections}")
+    if positions.shape != (len(sections), B, T) or positions.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"rope_axes_to_heads: positions must be [{len(sections)},{B},{T}] int32 or int64, got {tuple(positions.shape)} {positions.dtype}")
+    if inv_freq.shape != (D // 2,) or inv_freq.dtype not in (torch.float64, torch.float32):
+        raise ValueError(f"rope_axes_to_heads: inv_freq must be [{D // 2}] fp64 or fp32, got {tuple(inv_freq.shape)} {inv_freq.dtype}")
+    q, k, v = _pitched(q, "q"), _pitched(k, "k"), _pitched(v, "v")
+    positions, inv_freq = ops._dense(positions, "positions"), inv_freq.detach().to(torch.float64).contiguous()
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return _RopeAxesFn.apply(q, k, v, positions, inv_freq, sections, dtype)
+    return _launch(q, k, v, positions, inv_freq, sections, q.dtype, dtype, False)
+
+
+__all__ = ["rope_axes_to_heads", "rope_frequencies"]

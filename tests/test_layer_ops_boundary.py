@@ -1,0 +1,98 @@
+"""No-GPU checks of the layer's operators: struct mirrors, and refusals before anything touches a device."""
+import ctypes as C
+import os
+
+import pytest
+import torch
+
+import nsa_from_scratch_b200 as nsa
+from nsa_from_scratch_b200 import _lib as L
+from test_cpu_boundary import _struct_fields
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+ARG, UNSUPPORTED = -1, -2
+
+
+@pytest.mark.parametrize("mirror,name", [
+    (L.NormArgs, "nsa_norm_args"), (L.NormBwdArgs, "nsa_norm_bwd_args"), (L.RopeAxesArgs, "nsa_rope_axes_args"), (L.LinearArgs, "nsa_linear_args"),
+    (L.LinearBwdArgs, "nsa_linear_bwd_args"), (L.GatedMlpArgs, "nsa_gated_mlp_args"), (L.GatedMlpBwdArgs, "nsa_gated_mlp_bwd_args")])
+def test_struct_mirrors(mirror, name):
+    header = open(os.path.join(ROOT, "include", "nsa_b200.h")).read()
+    assert [f[0] for f in mirror._fields_] == [f.split("[")[0] for f in _struct_fields(header, name)]
+
+
+def refused(rc, code, text):
+    assert rc == code and text.encode() in L.load().nsa_last_error(), (rc, L.load().nsa_last_error())
+
+
+def test_c_entry_points_refuse():
+    lib = L.load()
+    for fn in ("nsa_rms_norm", "nsa_rms_norm_bwd", "nsa_rope_axes", "nsa_linear", "nsa_linear_bwd", "nsa_gated_mlp", "nsa_gated_mlp_bwd"):
+        refused(getattr(lib, fn)(None, None), ARG, "NULL argument block")
+    for fn in ("nsa_linear_ws_bytes", "nsa_linear_bwd_ws_bytes", "nsa_gated_mlp_ws_bytes", "nsa_gated_mlp_bwd_ws_bytes"):
+        refused(getattr(lib, fn)(None), ARG, "NULL argument block")
+    n = L.NormArgs(rows=2, hidden=8, x_dtype=0, res_dtype=0, w_dtype=0, y_dtype=0, eps=1e-6)
+    refused(lib.nsa_rms_norm(C.byref(n), None), ARG, "NULL pointer")
+    n.w_dtype = 1
+    refused(lib.nsa_rms_norm(C.byref(n), None), UNSUPPORTED, "weight dtype")
+    n.w_dtype, n.hidden = 0, 0
+    refused(lib.nsa_rms_norm(C.byref(n), None), ARG, "bad sizes")
+    n.hidden, n.residual = 8, 16
+    refused(lib.nsa_rms_norm(C.byref(n), None), ARG, "both be given")
+    n.residual, n.y_dtype = None, 4
+    refused(lib.nsa_rms_norm(C.byref(n), None), UNSUPPORTED, "result dtype")
+    n.y_dtype, n.eps = 0, float("nan")
+    refused(lib.nsa_rms_norm(C.byref(n), None), ARG, "eps")
+    n.eps, n.rows = 1e-6, 0
+    assert lib.nsa_rms_norm(C.byref(n), None) == 0                                  # nothing to do
+    refused(lib.nsa_quantize_rows_fp8(1, 1, 1, 2, 8, 0, 1, None), ARG, "format")
+    refused(lib.nsa_quantize_rows_fp8(1, None, 1, 2, 8, 0, 2, None), ARG, "NULL")
+    r = L.RopeAxesArgs(B=1, T=4, H=2, Hkv=1, D=64, n_axes=2, sections=(C.c_int32 * 8)(16, 16), x_dtype=0, y_dtype=0)
+    refused(lib.nsa_rope_axes(C.byref(r), None), ARG, "NULL pointer")
+    r.sections = (C.c_int32 * 8)(16, 15)
+    refused(lib.nsa_rope_axes(C.byref(r), None), ARG, "add up to 31")
+    r.n_axes = 9
+    refused(lib.nsa_rope_axes(C.byref(r), None), ARG, "9 axes")
+    r.D = 63
+    refused(lib.nsa_rope_axes(C.byref(r), None), UNSUPPORTED, "even")
+    a = L.LinearArgs(M=4, N=8, K=8, dtype=0, y_dtype=0, act=0)
+    refused(lib.nsa_linear(C.byref(a), None), ARG, "NULL pointer")
+    a.act = 4
+    refused(lib.nsa_linear(C.byref(a), None), ARG, "activation")
+    refused(lib.nsa_linear_ws_bytes(C.byref(a)), ARG, "activation")
+    a.act, a.y_dtype = 0, 1
+    refused(lib.nsa_linear(C.byref(a), None), UNSUPPORTED, "result dtype")
+    a.y_dtype, a.dtype = 0, 4
+    refused(lib.nsa_linear(C.byref(a), None), UNSUPPORTED, "operand dtype")
+    a.dtype, a.x, a.w, a.y = 2, 16, 16, 16
+    refused(lib.nsa_linear(C.byref(a), None), ARG, "scales")
+    a.dtype, a.K = 0, 0
+    refused(lib.nsa_linear(C.byref(a), None), ARG, "bad sizes")
+    b = L.LinearBwdArgs(dy=16, x=16, w=16, M=4, N=8, K=8, dtype=0, act=1, ws=16)
+    refused(lib.nsa_linear_bwd(C.byref(b), None), ARG, "NULL pointer")              # no z beside an activation
+    b.z = 16
+    refused(lib.nsa_linear_bwd(C.byref(b), None), ARG, "workspace")
+    m = L.GatedMlpArgs(x=16, wg=16, wu=16, wd=16, y=16, ws=16, M=4, N=8, F=16, dtype=0, act=1)
+    refused(lib.nsa_gated_mlp(C.byref(m), None), ARG, "workspace")
+    m.g = 16
+    refused(lib.nsa_gated_mlp(C.byref(m), None), ARG, "both g and u")
+    m.dtype = 4
+    refused(lib.nsa_gated_mlp(C.byref(m), None), UNSUPPORTED, "dtype")
+
+
+def test_no_cpu_path():
+    x, w = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(8, 8, dtype=torch.bfloat16)
+    for call in (lambda: nsa.rms_norm(x, w[0]), lambda: nsa.rms_norm_fp8(x, w[0]), lambda: nsa.quantize_rows_to_fp8(x), lambda: nsa.linear(x, w),
+                 lambda: nsa.gated_mlp(x, w, w, w)):
+        with pytest.raises(RuntimeError, match="CUDA"):
+            call()
+    with pytest.raises(RuntimeError, match="CUDA"):
+        q = torch.zeros(1, 2, 1, 8)
+        nsa.rope_axes_to_heads(q, q, q, torch.zeros(1, 1, 2, dtype=torch.int64), torch.zeros(4), (4,))
+
+
+def test_rope_frequencies():
+    f = nsa.rope_frequencies(64, 10000.0, device="cpu")
+    assert f.dtype == torch.float64 and f.shape == (32,) and float(f[0]) == 1.0 and abs(float(f[16]) - 0.01) < 1e-15
+    with pytest.raises(ValueError):
+        nsa.rope_frequencies(7)
