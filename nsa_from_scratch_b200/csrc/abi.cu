@@ -51,6 +51,8 @@ bool cmp_scores_tc5_supports(int, int, int, int, int, int);
 int cmp_block_scores_tc5(const void*, const void*, const float*, float*, float*, int, int, int, int, int, int, int, int, int, int, int, int,
                          int, float, int, int, int, int, cudaStream_t);
 int cs5_take_status(int*);
+int gemm_take_status(int*);
+int gemm_set_status(int);
 int rope_to_heads(const void*, void*, const void*, const void*, int, int, int, int, int, int, int, cudaStream_t);
 
 static bool is16(int dt) { return dt == NSA_BF16 || dt == NSA_FP16; }
@@ -208,13 +210,17 @@ int nsa_device_status(nsa_stream_t stream) {
   int v4 = 0;
   if ((rc = bst_take_status(&v4)) != NSA_OK) return rc;
   if (v == 0 && v4 != 0) v = 300 + v4;
+  int v5 = 0;
+  if ((rc = gemm_take_status(&v5)) != NSA_OK) return rc;
+  if (v == 0 && v5 != 0) v = 400 + v5;
   if (v != 0) return fail(NSA_ERR_DEVICE, "a kernel gave up waiting on barrier %d (bounded wait expired)", v - 1);
   return NSA_OK;
 }
 
 int nsa_debug_set_device_status(int kernel_family, int value) {
-  NSA_REQUIRE(kernel_family == 0 || kernel_family == 2 || kernel_family == 3, NSA_ERR_ARG,
-              "debug status: kernel family %d (0 = forward, 2 = selected backward, 3 = whole forward's backward)", kernel_family);
+  NSA_REQUIRE(kernel_family == 0 || kernel_family == 2 || kernel_family == 3 || kernel_family == 4, NSA_ERR_ARG,
+              "debug status: kernel family %d (0 = forward, 2 = selected backward, 3 = whole forward's backward, 4 = the layer's matrix products)", kernel_family);
+  if (kernel_family == 4) return gemm_set_status(value);
   return kernel_family == 0 ? tc5_set_status(value) : (kernel_family == 2 ? bw5_set_status(value) : bst_set_status(value));
 }
 

@@ -52,14 +52,17 @@ __device__ __forceinline__ void act_both(float z, int act, float& p, float& d) {
 
 struct Epi {
   int mode, act;
-  int M, N;                      // results are [M][N], dense
-  int vec;                       // 1: N % 8 == 0 and every 16-bit pointer below is 16-byte aligned
+  int M, N;                      // results are [M][N]
+  long long ldy;                 // elements between rows of y (EPI_GLU_BWD: of o1 and o2 too); everything else is dense
+  int vec;                       // 1: N % 8 == 0 and every 16-bit pointer to a dense matrix is 16-byte aligned
+  int vecy;                      // 1: ldy % 8 == 0 and y (o1, o2) aligned; columns N..ldy-1 of a padded row may be written
   const void *bias, *residual;   // EPI_LINEAR; out type; NULL: none
   const float *xs, *ws;          // EPI_LINEAR: scales per row and per column of the sums; NULL: none
   const void *i0, *i1;           // EPI_GLU_BWD: stored g and u
   void *y, *o1, *o2;             // LINEAR: y, z (NULL: not wanted), -;  GLU: h, g, u (NULL: not wanted);  GLU_BWD: dg, du, h
 };
 
+// One product; rows of A and B start on 16-byte boundaries.
 struct GemmProblem {
   const void *A[2], *B[2];       // EPI_GLU: B[0], B[1] are the two weights (one segment)
   int segments;                  // 1 or 2
@@ -102,7 +105,7 @@ template <typename T, int MODE>
 __device__ __forceinline__ void epilogue8(const Epi& e, long long row, int col, float (&a)[8], const float (&b)[8]) {
   const int n = e.N - col;
   if (row >= e.M || n <= 0) return;
-  const long long at = row * e.N + col;
+  const long long at = row * e.N + col, ay = row * e.ldy + col;
   if constexpr (MODE == EPI_LINEAR) {
     if (e.xs != nullptr) {
       const float s = e.xs[row];
@@ -126,12 +129,12 @@ __device__ __forceinline__ void epilogue8(const Epi& e, long long row, int col, 
 #pragma unroll
       for (int i = 0; i < 8; ++i) a[i] += c[i];
     }
-    store8<T>(e.y, at, n, e.vec, a);
+    store8<T>(e.y, ay, n, e.vecy, a);
   } else if constexpr (MODE == EPI_GLU) {
     if (e.o1 != nullptr) { store8<T>(e.o1, at, n, e.vec, a); store8<T>(e.o2, at, n, e.vec, b); }
 #pragma unroll
     for (int i = 0; i < 8; ++i) a[i] = act_f(a[i], e.act) * b[i];
-    store8<T>(e.y, at, n, e.vec, a);
+    store8<T>(e.y, ay, n, e.vecy, a);
   } else {
     float g[8], u[8], du[8], h[8];
     load8<T>(e.i0, at, n, e.vec, g);
@@ -144,9 +147,9 @@ __device__ __forceinline__ void epilogue8(const Epi& e, long long row, int col, 
       h[i] = p * u[i];
       a[i] = a[i] * u[i] * d;
     }
-    store8<T>(e.y, at, n, e.vec, a);
-    store8<T>(e.o1, at, n, e.vec, du);
-    store8<T>(e.o2, at, n, e.vec, h);
+    store8<T>(e.y, ay, n, e.vecy, a);
+    store8<T>(e.o1, ay, n, e.vecy, du);
+    store8<T>(e.o2, ay, n, e.vecy, h);
   }
 }
 
@@ -159,7 +162,8 @@ static inline int sm_count() {
   return sms;
 }
 
-int gemm_generic(const GemmProblem& p, cudaStream_t st);
+long long gemm_tc5_ws_bytes(const GemmProblem& p);                       // gemm_tc5.cu
+int gemm_tc5(const GemmProblem& p, void* ws, cudaStream_t st);
 int column_sum(const float* part, void* out, int parts, int N, int dt, cudaStream_t st);   // norm.cu
 
 }  // namespace nsa

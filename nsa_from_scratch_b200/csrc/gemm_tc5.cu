@@ -1,0 +1,520 @@
+// Matrix product on the 5th-generation tensor cores; operand rows start on 16-byte boundaries (linear.cu pads others).
+//
+// Persistent and warp-specialised: warp 0 brings operand tiles with TMA (128-byte swizzle, zeros outside), warp 1 issues
+// tcgen05.mma, warps 4-11 take the finished sums from TMEM through shared memory to the epilogue.  The sums are double
+// buffered in TMEM, so a tile's epilogue runs under the next tile's products.
+//
+//   CG = 2: a pair of CTAs computes 256 x 256 results; each brings 128 rows of A and half of B's 256 rows, and the pair's
+//           tensor cores read both halves.  Per CTA and 64-deep step that is 32 KB from L2 for 256 x 128 x 64 products a
+//           CTA; one CTA alone on 128 x 256 would need 48 KB, more than L2 delivers at the tensor cores' pace.
+//   CG = 1: one CTA computes 128 x 128 results: problems with few tiles.
+//
+// EPI_GLU computes both products in one tile: the B rows of a tile are BN/2 rows of each weight, so that g and u of a
+// column stand BN/2 columns apart in the same TMEM lane.
+//
+// Every wait is bounded; a wait that gives up raises the CTA's abort flag and the device status word, and the CTA still
+// frees its TMEM.
+#include "gemm.cuh"
+#include "tc5_ptx.cuh"
+
+#include <cudaTypedefs.h>
+
+namespace nsa {
+
+using namespace tc5;
+
+__device__ int g_gemm_status;
+
+// ---------------------------------------------------------------- CTA pairs
+__device__ __forceinline__ uint32_t cluster_rank() { uint32_t r; asm volatile("mov.u32 %0, %%cluster_ctarank;\n" : "=r"(r)); return r; }
+__device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
+  uint32_t r;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;\n" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
+}
+__device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_addr) : "memory");
+}
+// `bar` is a shared::cluster address: with CG = 2 the pair's first CTA counts the bytes of both
+template <int CG>
+__device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
+  if constexpr (CG == 2)
+    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
+  else
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];\n"
+                 ::"r"(dst), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
+}
+template <int CG> __device__ __forceinline__ void tm_alloc(uint32_t smem_dst, uint32_t ncols) {
+  if constexpr (CG == 2) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_dst), "r"(ncols) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;\n" ::: "memory");
+  } else {
+    tmem_alloc(smem_dst, ncols);
+    tmem_relinquish();
+  }
+}
+template <int CG> __device__ __forceinline__ void tm_dealloc(uint32_t taddr, uint32_t ncols) {
+  if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(taddr), "r"(ncols) : "memory");
+  else tmem_dealloc(taddr, ncols);
+}
+// one arrival on `bar` (of both CTAs of a pair) when every product issued so far is done
+template <int CG> __device__ __forceinline__ void commit(uint32_t bar) {
+  if constexpr (CG == 2)
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(bar), "h"((uint16_t)3) : "memory");
+  else tc_commit(bar);
+}
+template <int CG, bool F8>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+#define NSA_MMA(G, K)                                                                                                        \
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::" G ".kind::" K " [%0], %1, %2, %3, p;\n\t}\n" \
+               ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory")
+  if constexpr (CG == 2) { if constexpr (F8) NSA_MMA("2", "f8f6f4"); else NSA_MMA("2", "f16"); }
+  else { if constexpr (F8) NSA_MMA("1", "f8f6f4"); else NSA_MMA("1", "f16"); }
+#undef NSA_MMA
+}
+
+// ---------------------------------------------------------------- kernel
+struct GemmTcParams {
+  CUtensorMap tmA[2], tmB[2];
+  Epi e;
+  float* part;              // PARTIAL: [splits][products][M][N] fp32
+  int M, N;
+  int tiles_m, tiles_n;
+  int ksteps, segments;     // 128-byte steps of one segment
+  int splits, per_split;    // the steps of all segments, dealt out to `splits` tiles
+};
+
+constexpr int EPI_PARTIAL = 3, EPI_PARTIAL2 = 4;       // raw sums of one product / of a gated pair, for the joining kernel
+
+template <int CG, int BN> struct TcShape {
+  static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / CG * 128;
+  static constexpr int STAGES = 196608 / (A_BYTES + B_BYTES) > 6 ? 6 : 196608 / (A_BYTES + B_BYTES);
+  static constexpr int SMEM = STAGES * (A_BYTES + B_BYTES) + 8 * 4096 + 1024;
+};
+
+// F: 0 fp16, 1 bf16, 2 e4m3, 3 e5m2;  T: result type
+template <int F, typename T, bool A_MN, bool B_MN, int MODE, int CG, int BN>
+__global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant__ GemmTcParams p) {
+  using S = TcShape<CG, BN>;
+  constexpr bool F8 = F >= 2;
+  constexpr int KE = F8 ? 128 : 64;                                  // elements of a 128-byte step
+  constexpr bool PAIR = MODE == EPI_GLU || MODE == EPI_PARTIAL2;     // two products a tile
+  constexpr int NW = PAIR ? BN / 2 : BN;                             // result columns of a tile
+  constexpr int BROWS = BN / CG;                                     // B rows that this CTA brings
+  constexpr uint32_t IDESC = idesc_f16(F8 ? F - 2 : F, 128 * CG, BN, A_MN, B_MN);
+  static_assert(!F8 || (!A_MN && !B_MN), "fp8 operands are k-major");
+
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  const uint32_t s_tiles = smem_u32(smem);
+  float* stage_f = reinterpret_cast<float*>(smem + S::STAGES * (S::A_BYTES + S::B_BYTES));
+  __shared__ __align__(8) uint64_t full[S::STAGES], empty[S::STAGES], tfull[2], tempty[2];
+  __shared__ uint32_t tmem_s;
+  __shared__ int abort_flag;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t rank = CG == 2 ? cluster_rank() : 0;
+  const int unit = blockIdx.x / CG, units = gridDim.x / CG;
+  const int tiles = p.tiles_m * p.tiles_n * p.splits;
+  const int all_steps = p.ksteps * p.segments;
+
+  if (tid == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < S::STAGES; ++i) { mbar_init(smem_u32(&full[i]), 1); mbar_init(smem_u32(&empty[i]), 1); }
+    for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&tfull[i]), 1); mbar_init(smem_u32(&tempty[i]), 8 * CG); }
+    fence_barrier_init();
+  }
+  if (warp == 2) tm_alloc<CG>(smem_u32(&tmem_s), 2 * BN);
+  tc_fence_before();
+  __syncthreads();
+  if constexpr (CG == 2) cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = tmem_s;
+  int fail_id = 0;
+
+  // tile t: which split of the contraction, which rows and columns (8 tile rows walk the columns together: their B tiles meet in L2)
+  auto place = [&](int t, int& m0, int& n0, int& k0, int& k1, int& split) {
+    const int mn = p.tiles_m * p.tiles_n;
+    split = t / mn;
+    t -= split * mn;
+    const int group = 8 * p.tiles_n, g = t / group, first = g * 8, rows = min(8, p.tiles_m - first);
+    t -= g * group;
+    m0 = (first + t % rows) * 128 * CG;
+    n0 = t / rows * NW;
+    k0 = split * p.per_split;
+    k1 = min(all_steps, k0 + p.per_split);
+  };
+
+  if (warp == 0) {
+    // =============================== TMA producer ===============================
+    const bool leader = elect_one();
+    if (leader) {
+      for (int i = 0; i < p.segments; ++i) { tma_prefetch_desc(&p.tmA[i]); tma_prefetch_desc(&p.tmB[i]); }
+      if constexpr (PAIR) tma_prefetch_desc(&p.tmB[1]);
+    }
+    __syncwarp();
+    int it = 0;
+    bool ok = true;
+    for (int t = unit; t < tiles && ok; t += units) {
+      int m0, n0, k0, k1, split;
+      place(t, m0, n0, k0, k1, split);
+      for (int k = k0; k < k1; ++k, ++it) {
+        const int s = it % S::STAGES, ph = (it / S::STAGES) & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[s]), ph ^ 1, &abort_flag));
+        if (!ok) { fail_id = 1; break; }
+        if (leader) {
+          uint32_t bar = smem_u32(&full[s]);
+          if (rank == 0) mbar_expect_tx(bar, CG * (S::A_BYTES + S::B_BYTES));
+          if constexpr (CG == 2) bar = map_to_rank(bar, 0);
+          const int seg = k >= p.ksteps, kc = (k - seg * p.ksteps) * KE;
+          const uint32_t da = s_tiles + s * (S::A_BYTES + S::B_BYTES), db = da + S::A_BYTES;
+          const int ma = m0 + (int)rank * 128;
+          if constexpr (A_MN) {
+            tma_load_2d<CG>(da, &p.tmA[seg], bar, ma, kc);
+            tma_load_2d<CG>(da + 8192, &p.tmA[seg], bar, ma + 64, kc);
+          } else {
+            tma_load_2d<CG>(da, &p.tmA[seg], bar, kc, ma);
+          }
+          if constexpr (PAIR) {
+            if constexpr (CG == 2) tma_load_2d<CG>(db, &p.tmB[rank], bar, kc, n0);
+            else { tma_load_2d<CG>(db, &p.tmB[0], bar, kc, n0); tma_load_2d<CG>(db + S::B_BYTES / 2, &p.tmB[1], bar, kc, n0); }
+          } else if constexpr (B_MN) {
+#pragma unroll
+            for (int c = 0; c < BROWS / 64; ++c) tma_load_2d<CG>(db + c * 8192, &p.tmB[seg], bar, n0 + (int)rank * BROWS + c * 64, kc);
+          } else {
+            tma_load_2d<CG>(db, &p.tmB[seg], bar, kc, n0 + (int)rank * BROWS);
+          }
+        }
+        __syncwarp();
+      }
+    }
+  } else if (warp == 1) {
+    // =============================== MMA issuer (the pair's first CTA) ===============================
+    if (rank == 0) {
+      const bool leader = elect_one();
+      int it = 0, n = 0;
+      bool ok = true;
+      for (int t = unit; t < tiles && ok; t += units, ++n) {
+        int m0, n0, k0, k1, split;
+        place(t, m0, n0, k0, k1, split);
+        const int buf = n & 1;
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&tempty[buf]), ((n >> 1) & 1) ^ 1, &abort_flag));
+        if (!ok) { fail_id = 2; break; }
+        tc_fence_after();
+        const uint32_t acc = tmem + buf * BN;
+        for (int k = k0; k < k1; ++k, ++it) {
+          const int s = it % S::STAGES, ph = (it / S::STAGES) & 1;
+          ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[s]), ph, &abort_flag));
+          if (!ok) { fail_id = 3; break; }
+          tc_fence_after();
+          if (leader) {
+            const uint32_t da = s_tiles + s * (S::A_BYTES + S::B_BYTES);
+            const uint64_t a = smem_desc_sw128(da, A_MN ? 8192 : 16, 1024), b = smem_desc_sw128(da + S::A_BYTES, B_MN ? 8192 : 16, 1024);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) mma<CG, F8>(acc, a + i * (A_MN ? 128 : 2), b + i * (B_MN ? 128 : 2), IDESC, (k > k0 || i > 0) ? 1u : 0u);
+            commit<CG>(smem_u32(&empty[s]));
+          }
+          __syncwarp();
+        }
+        if (!ok) break;
+        if (leader) commit<CG>(smem_u32(&tfull[buf]));
+        __syncwarp();
+      }
+    }
+  } else if (warp >= 4) {
+    // =============================== epilogue ===============================
+    // A warp owns 32 TMEM lanes (rows) and half of the columns.  32 x 32 sums pass through its 4 KB of shared memory, 16-byte
+    // pieces swizzled by row: written by row (a lane's 32 columns), read as 8 columns of 4 lanes to a row, so that
+    // global memory sees runs of 64 bytes.
+    const int quarter = warp & 3, half = (warp - 4) >> 2;
+    float* st = stage_f + (warp - 4) * 1024;
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    int n = 0;
+    bool ok = true;
+    for (int t = unit; t < tiles && ok; t += units, ++n) {
+      int m0, n0, k0, k1, split;
+      place(t, m0, n0, k0, k1, split);
+      const int buf = n & 1;
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&tfull[buf]), (n >> 1) & 1, &abort_flag));
+      if (!ok) { fail_id = 4; break; }
+      tc_fence_after();
+      const long long row0 = m0 + (int)rank * 128 + quarter * 32;
+      constexpr int STEP = PAIR ? 16 : 32;                               // result columns a step
+      constexpr int STEPS = NW / 2 / STEP;
+#pragma unroll 1
+      for (int c = 0; c < STEPS; ++c) {
+        const int col = half * (NW / 2) + c * STEP;
+        uint32_t v[32];
+        if constexpr (PAIR) {
+          uint32_t g[16], u[16];
+          tmem_ld16(tmem + lanes + buf * BN + col, g);
+          tmem_ld16(tmem + lanes + buf * BN + NW + col, u);
+          tc_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 16; ++i) { v[i] = g[i]; v[16 + i] = u[i]; }
+        } else {
+          tmem_ld32(tmem + lanes + buf * BN + col, v);
+          tc_wait_ld();
+        }
+        if (c == STEPS - 1) {                                            // everything is in registers: the buffer may be filled again
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (CG == 2) arrive_remote(map_to_rank(smem_u32(&tempty[buf]), 0));
+            else mbar_arrive(smem_u32(&tempty[buf]));
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          *reinterpret_cast<uint4*>(st + lane * 32 + ((i ^ (lane & 7)) << 2)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        __syncwarp();
+        auto get8 = [&](int r, int piece, float (&x)[8]) {
+          const float4 lo = *reinterpret_cast<const float4*>(st + r * 32 + ((piece ^ (r & 7)) << 2));
+          const float4 hi = *reinterpret_cast<const float4*>(st + r * 32 + (((piece + 1) ^ (r & 7)) << 2));
+          x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w; x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
+        };
+        auto put_raw = [&](long long row, int cc, int product, const float (&x)[8]) {
+          if (row >= p.M) return;
+          float* dst = p.part + (((long long)split * (PAIR ? 2 : 1) + product) * p.M + row) * p.N + cc;
+          if (p.N % 4 == 0 && cc + 8 <= p.N) {
+            reinterpret_cast<float4*>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
+            reinterpret_cast<float4*>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              if (cc + i < p.N) dst[i] = x[i];
+          }
+        };
+        if constexpr (PAIR) {
+#pragma unroll
+          for (int q = 0; q < 2; ++q) {
+            const int r = q * 16 + (lane >> 1), cc = n0 + col + (lane & 1) * 8;
+            float a[8], b[8];
+            get8(r, (lane & 1) * 2, a);
+            get8(r, 4 + (lane & 1) * 2, b);
+            if constexpr (MODE == EPI_PARTIAL2) { put_raw(row0 + r, cc, 0, a); put_raw(row0 + r, cc, 1, b); }
+            else epilogue8<T, EPI_GLU>(p.e, row0 + r, cc, a, b);
+          }
+        } else {
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int r = q * 8 + (lane >> 2), cc = n0 + col + (lane & 3) * 8;
+            float a[8];
+            get8(r, (lane & 3) * 2, a);
+            if constexpr (MODE == EPI_PARTIAL) put_raw(row0 + r, cc, 0, a);
+            else epilogue8<T, MODE>(p.e, row0 + r, cc, a, a);
+          }
+        }
+        __syncwarp();
+      }
+    }
+  }
+
+  if (fail_id != 0) atomicCAS(&g_gemm_status, 0, fail_id);
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (abort_flag) __nanosleep(1000000);                                  // copies still under way land long before this
+  if constexpr (CG == 2) cluster_sync();                                 // no CTA of a pair leaves while the other may signal it
+  if (warp == 2) { tc_fence_after(); tm_dealloc<CG>(tmem, 2 * BN); }
+}
+
+// Joins the partial sums of a split contraction, in split order, and runs the epilogue: 8 columns a thread.
+template <typename T, int MODE>
+__global__ void __launch_bounds__(256) gemm_join_kernel(const float* __restrict__ part, const Epi e, int splits) {
+  constexpr int PR = MODE == EPI_GLU ? 2 : 1;
+  const int groups = (e.N + 7) / 8;
+  const long long total = (long long)e.M * groups;
+  const long long mn = (long long)e.M * e.N;
+  grid_dep_wait();
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const long long row = i / groups;
+    const int col = (int)(i % groups) * 8;
+    float a[PR][8] = {};
+    for (int s = 0; s < splits; ++s) {
+#pragma unroll
+      for (int q = 0; q < PR; ++q) {
+        const float* src = part + (s * PR + q) * mn + row * e.N + col;
+        if (e.N % 8 == 0) {
+          const float4 lo = reinterpret_cast<const float4*>(src)[0], hi = reinterpret_cast<const float4*>(src)[1];
+          a[q][0] += lo.x; a[q][1] += lo.y; a[q][2] += lo.z; a[q][3] += lo.w;
+          a[q][4] += hi.x; a[q][5] += hi.y; a[q][6] += hi.z; a[q][7] += hi.w;
+        } else {
+#pragma unroll
+          for (int c = 0; c < 8; ++c)
+            if (col + c < e.N) a[q][c] += src[c];
+        }
+      }
+    }
+    epilogue8<T, MODE>(e, row, col, a[0], a[PR - 1]);
+  }
+}
+
+// ---------------------------------------------------------------- host side
+static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
+  static const PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    cudaDriverEntryPointQueryResult q;
+    void* ptr = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) ptr = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
+  }();
+  return fn;
+}
+
+// [rows][cols] matrix with `ld` elements between rows; boxes of 128 bytes x `box_rows`, 128-byte swizzle, zeros outside
+static int map_2d(CUtensorMap* m, const void* ptr, long long rows, long long cols, long long ld, int box_rows, int dtype) {
+  auto enc = tensor_map_encoder();
+  NSA_REQUIRE(enc != nullptr, NSA_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  const int size = dtype == NSA_BF16 || dtype == NSA_FP16 ? 2 : 1;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld * size};
+  cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows};
+  cuuint32_t es[2] = {1, 1};
+  const CUtensorMapDataType dt = dtype == NSA_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : dtype == NSA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
+  auto encode = [&] { return enc(m, dt, 2, const_cast<void*>(ptr), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE); };
+  CUresult r = encode();
+  if (r == CUDA_ERROR_INVALID_CONTEXT) {     // a thread that has not used the runtime yet (autograd's): bind the device's context to it
+    int dev = 0;
+    NSA_CUDA_OK(cudaGetDevice(&dev));
+    NSA_CUDA_OK(cudaSetDevice(dev));
+    r = encode();
+  }
+  NSA_REQUIRE(r == CUDA_SUCCESS, NSA_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d", (int)r);
+  return NSA_OK;
+}
+
+static int esize(int dtype) { return dtype == NSA_BF16 || dtype == NSA_FP16 ? 2 : 1; }
+
+// Which kernel and how many ways the contraction is split.
+struct TcPlan { int cg, bn, tiles_m, tiles_n, ksteps, splits, per_split; };
+static TcPlan tc_plan(const GemmProblem& p) {
+  TcPlan t;
+  const int sms = sm_count();
+  const int pair = p.e.mode == EPI_GLU ? 2 : 1;
+  auto tiles = [&](int cg, int bn, int& tm, int& tn) {
+    tm = (p.M + 128 * cg - 1) / (128 * cg);
+    tn = (p.N + bn / pair - 1) / (bn / pair);
+    return (long long)tm * tn;
+  };
+  t.cg = 2; t.bn = 256;
+  const long long big = tiles(2, 256, t.tiles_m, t.tiles_n);
+  if (big < sms / 2) { t.cg = 1; t.bn = 128; tiles(1, 128, t.tiles_m, t.tiles_n); }
+  t.ksteps = (p.K * esize(p.dtype) + 127) / 128;
+  const int steps = t.ksteps * p.segments;
+  const long long n = (long long)t.tiles_m * t.tiles_n, units = sms / t.cg;
+  t.splits = 1;
+  if (n * 2 <= units && steps >= 8) {
+    long long s = units / n;
+    if (s > steps / 4) s = steps / 4;
+    if (s > 16) s = 16;
+    t.splits = (int)(s < 1 ? 1 : s);
+  }
+  t.per_split = (steps + t.splits - 1) / t.splits;
+  t.splits = (steps + t.per_split - 1) / t.per_split;
+  return t;
+}
+
+long long gemm_tc5_ws_bytes(const GemmProblem& p) {
+  const TcPlan t = tc_plan(p);
+  return t.splits == 1 ? 0 : (long long)t.splits * (p.e.mode == EPI_GLU ? 2 : 1) * p.M * p.N * 4;
+}
+
+template <int F, typename T, bool A_MN, bool B_MN, int MODE, int CG, int BN>
+static int tc_launch(const GemmTcParams& g, long long tiles, cudaStream_t st) {
+  using S = TcShape<CG, BN>;
+  auto fn = gemm_tc5_kernel<F, T, A_MN, B_MN, MODE, CG, BN>;
+  NSA_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+  const long long units = sm_count() / CG;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)((tiles < units ? tiles : units) * CG));
+  cfg.blockDim = dim3(384);
+  cfg.dynamicSmemBytes = S::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = CG; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = CG == 2 ? 1 : 0;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, g);
+  if (e != cudaSuccess) return fail(NSA_ERR_CUDA, "gemm_tc5 launch failed: %s", cudaGetErrorString(e));
+  return NSA_OK;
+}
+
+template <int F, typename T, bool A_MN, bool B_MN, int MODE>
+static int tc_shape(const GemmTcParams& g, const TcPlan& t, cudaStream_t st) {
+  const long long tiles = (long long)t.tiles_m * t.tiles_n * t.splits;
+  if (t.cg == 2) return tc_launch<F, T, A_MN, B_MN, MODE, 2, 256>(g, tiles, st);
+  return tc_launch<F, T, A_MN, B_MN, MODE, 1, 128>(g, tiles, st);
+}
+
+template <int F, typename T>
+static int tc_mode(const GemmTcParams& g, const TcPlan& t, const GemmProblem& p, cudaStream_t st) {
+  const bool split = t.splits > 1;
+  if constexpr (F >= 2) {
+    return split ? tc_shape<F, T, false, false, EPI_PARTIAL>(g, t, st) : tc_shape<F, T, false, false, EPI_LINEAR>(g, t, st);
+  } else {
+    if (p.e.mode == EPI_GLU) return split ? tc_shape<F, T, false, false, EPI_PARTIAL2>(g, t, st) : tc_shape<F, T, false, false, EPI_GLU>(g, t, st);
+    if (p.e.mode == EPI_GLU_BWD) return split ? tc_shape<F, T, false, true, EPI_PARTIAL>(g, t, st) : tc_shape<F, T, false, true, EPI_GLU_BWD>(g, t, st);
+    if (p.a_mn) return split ? tc_shape<F, T, true, true, EPI_PARTIAL>(g, t, st) : tc_shape<F, T, true, true, EPI_LINEAR>(g, t, st);
+    if (p.b_mn) return split ? tc_shape<F, T, false, true, EPI_PARTIAL>(g, t, st) : tc_shape<F, T, false, true, EPI_LINEAR>(g, t, st);
+    return split ? tc_shape<F, T, false, false, EPI_PARTIAL>(g, t, st) : tc_shape<F, T, false, false, EPI_LINEAR>(g, t, st);
+  }
+}
+
+template <typename T>
+static int join(const float* part, const GemmProblem& p, int splits, cudaStream_t st) {
+  const long long want = ((long long)p.M * ((p.N + 7) / 8) + 255) / 256, cap = 8LL * sm_count();
+  const dim3 grid((unsigned)(want < cap ? want : cap));
+  if (p.e.mode == EPI_GLU) return launch_pdl("gemm_join", gemm_join_kernel<T, EPI_GLU>, grid, 256, 0, st, part, p.e, splits);
+  if (p.e.mode == EPI_GLU_BWD) return launch_pdl("gemm_join", gemm_join_kernel<T, EPI_GLU_BWD>, grid, 256, 0, st, part, p.e, splits);
+  return launch_pdl("gemm_join", gemm_join_kernel<T, EPI_LINEAR>, grid, 256, 0, st, part, p.e, splits);
+}
+
+int gemm_tc5(const GemmProblem& p, void* ws, cudaStream_t st) {
+  const TcPlan t = tc_plan(p);
+  NSA_REQUIRE((long long)t.tiles_m * t.tiles_n * t.splits < 2147483647LL, NSA_ERR_ARG, "matrix product: %d x %d results are too many tiles", p.M, p.N);
+  GemmTcParams g;
+  int rc;
+  const int ke = 128 / esize(p.dtype);
+  const int pair = p.e.mode == EPI_GLU;
+  const int brows = pair ? t.bn / 2 : t.bn / t.cg;                     // rows of a box of B
+  for (int i = 0; i < p.segments; ++i) {
+    rc = p.a_mn ? map_2d(&g.tmA[i], p.A[i], p.K, p.M, p.lda, ke, p.dtype) : map_2d(&g.tmA[i], p.A[i], p.M, p.K, p.lda, 128, p.dtype);
+    if (rc != NSA_OK) return rc;
+    rc = p.b_mn ? map_2d(&g.tmB[i], p.B[i], p.K, p.N, p.ldb, ke, p.dtype) : map_2d(&g.tmB[i], p.B[i], p.N, p.K, p.ldb, brows, p.dtype);
+    if (rc != NSA_OK) return rc;
+  }
+  if (pair && (rc = map_2d(&g.tmB[1], p.B[1], p.N, p.K, p.ldb, brows, p.dtype)) != NSA_OK) return rc;
+  g.e = p.e;
+  g.part = reinterpret_cast<float*>(ws);
+  g.M = p.M; g.N = p.N;
+  g.tiles_m = t.tiles_m; g.tiles_n = t.tiles_n;
+  g.ksteps = t.ksteps; g.segments = p.segments;
+  g.splits = t.splits; g.per_split = t.per_split;
+  const bool bf = p.out_dtype == NSA_BF16;
+  if (p.dtype == NSA_BF16) rc = tc_mode<1, __nv_bfloat16>(g, t, p, st);
+  else if (p.dtype == NSA_FP16) rc = tc_mode<0, __half>(g, t, p, st);
+  else if (p.dtype == NSA_FP8_E4M3) rc = bf ? tc_mode<2, __nv_bfloat16>(g, t, p, st) : tc_mode<2, __half>(g, t, p, st);
+  else rc = bf ? tc_mode<3, __nv_bfloat16>(g, t, p, st) : tc_mode<3, __half>(g, t, p, st);
+  if (rc != NSA_OK || t.splits == 1) return rc;
+  return bf ? join<__nv_bfloat16>(g.part, p, t.splits, st) : join<__half>(g.part, p, t.splits, st);
+}
+
+int gemm_take_status(int* status) {
+  int v = 0, zero = 0;
+  NSA_CUDA_OK(cudaMemcpyFromSymbol(&v, g_gemm_status, sizeof(int)));
+  if (v != 0) NSA_CUDA_OK(cudaMemcpyToSymbol(g_gemm_status, &zero, sizeof(int)));
+  *status = v;
+  return NSA_OK;
+}
+int gemm_set_status(int v) {
+  NSA_CUDA_OK(cudaMemcpyToSymbol(g_gemm_status, &v, sizeof(int)));
+  return NSA_OK;
+}
+
+}  // namespace nsa

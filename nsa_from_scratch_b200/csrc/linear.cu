@@ -8,7 +8,7 @@ namespace nsa {
 // block row).  A thread owns 8 columns and walks the rows of its block row; bound by HBM.
 template <typename T>
 __global__ void __launch_bounds__(128) act_bwd_kernel(const void* __restrict__ dy, const void* __restrict__ z, void* __restrict__ dz,
-                                                      float* __restrict__ part, int M, int N, int rows, int act, int vec) {
+                                                      float* __restrict__ part, int M, int N, long long lddz, int rows, int act, int vec, int vecz) {
   const int c = (blockIdx.x * 128 + threadIdx.x) * 8, n = N - c;
   if (n <= 0) return;
   const int r0 = blockIdx.y * rows, r1 = min(M, r0 + rows);
@@ -26,7 +26,7 @@ __global__ void __launch_bounds__(128) act_bwd_kernel(const void* __restrict__ d
         act_both(v[i], act, p, s);
         d[i] *= s;
       }
-      store8<T>(dz, at, n, vec, d);
+      store8<T>(dz, (long long)r * lddz + c, n, vecz, d);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) sum[i] += d[i];
@@ -49,54 +49,119 @@ static ActBwdPlan act_bwd_plan(int M, int N) {
   return p;
 }
 
-static int act_bwd(const void* dy, const void* z, void* dz, float* part, int M, int N, int act, int dtype, cudaStream_t st) {
+static int act_bwd(const void* dy, const void* z, void* dz, long long lddz, float* part, int M, int N, int act, int dtype, cudaStream_t st) {
   const ActBwdPlan p = act_bwd_plan(M, N);
-  const int vec = N % 8 == 0 && aligned16(dy) && aligned16(z) && aligned16(dz);
+  const int vec = N % 8 == 0 && aligned16(dy) && aligned16(z), vecz = lddz % 8 == 0;
   const dim3 grid(p.strips, p.groups);
-  if (dtype == NSA_BF16) act_bwd_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(dy, z, dz, part, M, N, p.rows, act, vec);
-  else act_bwd_kernel<__half><<<grid, 128, 0, st>>>(dy, z, dz, part, M, N, p.rows, act, vec);
+  if (dtype == NSA_BF16) act_bwd_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(dy, z, dz, part, M, N, lddz, p.rows, act, vec, vecz);
+  else act_bwd_kernel<__half><<<grid, 128, 0, st>>>(dy, z, dz, part, M, N, lddz, p.rows, act, vec, vecz);
   return launch_status("act_bwd");
 }
 
 // ---------------------------------------------------------------- workspaces
-// Hands out 256-byte aligned pieces; with base 0 it only counts.
+// The workspace of a call: 256-byte aligned pieces, then one scratch area that its matrix products use in turn.  Each call
+// goes through its steps twice, dry (counting, nothing is launched) and in earnest.
 struct Arena {
-  unsigned char* base;
-  long long at = 0;
+  unsigned char* base;               // NULL: dry
+  long long scratch_at;              // where the scratch starts (from the dry pass)
+  cudaStream_t st;
+  long long at = 0, scratch = 0;
+  bool dry() const { return base == nullptr; }
   void* take(long long bytes) {
-    void* p = base == nullptr ? nullptr : base + at;
+    void* p = dry() ? nullptr : base + at;
     at += (bytes + 255) / 256 * 256;
     return p;
   }
+  long long bytes() const { return at + scratch; }
 };
 
-static int gemm(const GemmProblem& p, cudaStream_t st) {
-  if (p.M == 0 || p.N == 0) return NSA_OK;
-  return gemm_generic(p, st);
+template <typename Args>
+static long long ws_bytes(const Args& a, int (*steps)(const Args&, Arena&)) {
+  Arena w{nullptr, 0, nullptr};
+  const int rc = steps(a, w);
+  return rc != NSA_OK ? rc : w.bytes();
 }
-
-static GemmProblem problem(const void* A, int a_mn, long long lda, const void* B, int b_mn, long long ldb, int M, int N, int K, int dtype) {
-  GemmProblem p = {};
-  p.A[0] = A; p.B[0] = B;
-  p.segments = 1;
-  p.a_mn = a_mn; p.b_mn = b_mn;
-  p.M = M; p.N = N; p.K = K;
-  p.lda = lda; p.ldb = ldb;
-  p.dtype = p.out_dtype = dtype;
-  p.e.M = M; p.e.N = N;
-  return p;
-}
-// EPI_LINEAR without anything around the sums
-static int product(GemmProblem p, void* out, cudaStream_t st) {
-  if (out == nullptr) return NSA_OK;
-  p.e.mode = EPI_LINEAR;
-  p.e.y = out;
-  p.e.vec = p.N % 8 == 0 && aligned16(out);
-  return gemm(p, st);
+template <typename Args>
+static int run_steps(const char* what, const Args& a, int (*steps)(const Args&, Arena&), cudaStream_t st) {
+  Arena count{nullptr, 0, st};
+  int rc = steps(a, count);
+  if (rc != NSA_OK) return rc;
+  const long long need = count.bytes();
+  NSA_REQUIRE(a.ws_bytes >= need && (a.ws != nullptr || need == 0), NSA_ERR_ARG, "%s: workspace of %lld bytes, %lld needed", what, (long long)a.ws_bytes, need);
+  static unsigned char none[16];     // stands for a workspace of no bytes
+  Arena w{a.ws != nullptr ? reinterpret_cast<unsigned char*>(a.ws) : none, count.at, st};
+  return steps(a, w);
 }
 
 static bool is16(int dt) { return dt == NSA_BF16 || dt == NSA_FP16; }
 static bool is8(int dt) { return dt == NSA_FP8_E4M3 || dt == NSA_FP8_E5M2; }
+static int elem(int dt) { return is16(dt) ? 2 : 1; }
+static long long padded(long long cols, int dt) { const int per = 16 / elem(dt); return (cols + per - 1) / per * per; }
+
+// dst [rows][ldd] = src [rows][cols], zeros behind: 16 bytes a thread
+template <typename E>
+__global__ void __launch_bounds__(256) pad_rows_kernel(const E* __restrict__ src, E* __restrict__ dst, long long rows, int cols, int ldd) {
+  constexpr int PER = 16 / sizeof(E);
+  const int groups = ldd / PER;
+  const long long total = rows * groups;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
+    const long long r = i / groups;
+    const int c = (int)(i % groups) * PER;
+    __align__(16) E v[PER];
+#pragma unroll
+    for (int e = 0; e < PER; ++e) v[e] = c + e < cols ? src[r * cols + c + e] : E(0);
+    *reinterpret_cast<uint4*>(dst + r * ldd + c) = *reinterpret_cast<const uint4*>(v);
+  }
+}
+
+// An operand whose rows start on 16-byte boundaries: the caller's own, or a padded copy.
+struct Mat { const void* p; long long ld; };
+static int operand(Arena& w, const void* p, long long rows, int cols, int dtype, Mat* m) {
+  const long long ld = padded(cols, dtype);
+  *m = Mat{p, cols};
+  if (ld == cols && aligned16(p)) return NSA_OK;
+  void* q = w.take(rows * ld * elem(dtype));
+  *m = Mat{q, ld};
+  if (w.dry()) return NSA_OK;
+  const long long want = (rows * (ld * elem(dtype) / 16) + 255) / 256, cap = 16LL * sm_count();
+  const int grid = (int)(want < cap ? want : cap);
+  if (is16(dtype)) pad_rows_kernel<<<grid, 256, 0, w.st>>>((const uint16_t*)p, (uint16_t*)q, rows, cols, (int)ld);
+  else pad_rows_kernel<<<grid, 256, 0, w.st>>>((const uint8_t*)p, (uint8_t*)q, rows, cols, (int)ld);
+  return launch_status("pad_rows");
+}
+
+static int gemm(Arena& w, const GemmProblem& p) {
+  if (!w.dry()) return gemm_tc5(p, w.base + w.scratch_at, w.st);
+  const long long need = gemm_tc5_ws_bytes(p);
+  if (need > w.scratch) w.scratch = need;
+  return NSA_OK;
+}
+
+static GemmProblem problem(Mat A, int a_mn, Mat B, int b_mn, int M, int N, int K, int dtype) {
+  GemmProblem p = {};
+  p.A[0] = A.p; p.B[0] = B.p;
+  p.segments = 1;
+  p.a_mn = a_mn; p.b_mn = b_mn;
+  p.M = M; p.N = N; p.K = K;
+  p.lda = A.ld; p.ldb = B.ld;
+  p.dtype = p.out_dtype = dtype;
+  p.e.M = M; p.e.N = N; p.e.ldy = N;
+  return p;
+}
+// EPI_LINEAR without anything around the sums
+static int product(Arena& w, GemmProblem p, void* out) {
+  if (out == nullptr) return NSA_OK;
+  p.e.mode = EPI_LINEAR;
+  p.e.y = out;
+  p.e.vec = p.e.vecy = p.N % 8 == 0 && aligned16(out);
+  return gemm(w, p);
+}
+
+static int zero(void* p, long long bytes, cudaStream_t st) {
+  if (p != nullptr) NSA_CUDA_OK(cudaMemsetAsync(p, 0, (size_t)bytes, st));
+  return NSA_OK;
+}
+#define NSA_TRY(expr) do { const int rc__ = (expr); if (rc__ != NSA_OK) return rc__; } while (0)
 
 // ---------------------------------------------------------------- linear
 static int check_linear(const nsa_linear_args& a) {
@@ -107,28 +172,28 @@ static int check_linear(const nsa_linear_args& a) {
   return NSA_OK;
 }
 
-int linear(const nsa_linear_args& a, cudaStream_t st) {
-  int rc = check_linear(a);
-  if (rc != NSA_OK) return rc;
-  if (a.M == 0) return NSA_OK;
-  NSA_REQUIRE(a.x && a.w && a.y, NSA_ERR_ARG, "linear: NULL pointer");
-  NSA_REQUIRE(is8(a.dtype) == (a.x_scale != nullptr) && is8(a.dtype) == (a.w_scale != nullptr), NSA_ERR_ARG, "linear: fp8 operands, and only they, have scales");
-  NSA_REQUIRE(a.z == nullptr || is16(a.dtype), NSA_ERR_UNSUPPORTED, "linear: fp8 operands keep nothing for a backward");
-  GemmProblem p = problem(a.x, 0, a.K, a.w, 0, a.K, a.M, a.N, a.K, a.dtype);
+static int linear_steps(const nsa_linear_args& a, Arena& w) {
+  Mat x, wt;
+  NSA_TRY(operand(w, a.x, a.M, a.K, a.dtype, &x));
+  NSA_TRY(operand(w, a.w, a.N, a.K, a.dtype, &wt));
+  GemmProblem p = problem(x, 0, wt, 0, a.M, a.N, a.K, a.dtype);
   p.out_dtype = a.y_dtype;
   p.e.mode = EPI_LINEAR;
   p.e.act = a.act;
   p.e.bias = a.bias; p.e.residual = a.residual; p.e.xs = a.x_scale; p.e.ws = a.w_scale;
   p.e.y = a.y; p.e.o1 = a.z;
-  p.e.vec = a.N % 8 == 0 && aligned16(a.bias) && aligned16(a.residual) && aligned16(a.y) && aligned16(a.z);
-  return gemm(p, st);
+  p.e.vec = a.N % 8 == 0 && aligned16(a.bias) && aligned16(a.residual) && aligned16(a.z);
+  p.e.vecy = a.N % 8 == 0 && aligned16(a.y);
+  return gemm(w, p);
 }
 
-static long long linear_bwd_ws(const nsa_linear_bwd_args& a, unsigned char* base, void** dz, float** part) {
-  Arena w{base};
-  *dz = a.act != NSA_ACT_NONE ? w.take((long long)a.M * a.N * 2) : nullptr;
-  *part = reinterpret_cast<float*>(w.take((long long)act_bwd_plan(a.M, a.N).groups * a.N * 4));
-  return w.at;
+int linear(const nsa_linear_args& a, cudaStream_t st) {
+  NSA_TRY(check_linear(a));
+  if (a.M == 0) return NSA_OK;
+  NSA_REQUIRE(a.x && a.w && a.y, NSA_ERR_ARG, "linear: NULL pointer");
+  NSA_REQUIRE(is8(a.dtype) == (a.x_scale != nullptr) && is8(a.dtype) == (a.w_scale != nullptr), NSA_ERR_ARG, "linear: fp8 operands, and only they, have scales");
+  NSA_REQUIRE(a.z == nullptr || is16(a.dtype), NSA_ERR_UNSUPPORTED, "linear: fp8 operands keep nothing for a backward");
+  return run_steps("linear", a, linear_steps, st);
 }
 
 static int check_linear_bwd(const nsa_linear_bwd_args& a) {
@@ -138,31 +203,39 @@ static int check_linear_bwd(const nsa_linear_bwd_args& a) {
   return NSA_OK;
 }
 
-static int zero(void* p, long long bytes, cudaStream_t st) {
-  if (p != nullptr) NSA_CUDA_OK(cudaMemsetAsync(p, 0, (size_t)bytes, st));
+static int linear_bwd_steps(const nsa_linear_bwd_args& a, Arena& w) {
+  const bool run = !w.dry();
+  Mat g, x, wt;
+  float* part = reinterpret_cast<float*>(w.take((long long)act_bwd_plan(a.M, a.N).groups * a.N * 4));
+  if (a.act != NSA_ACT_NONE) {
+    const long long ld = padded(a.N, a.dtype);
+    void* dz = w.take((long long)a.M * ld * 2);
+    g = Mat{dz, ld};
+    if (run) NSA_TRY(act_bwd(a.dy, a.z, dz, ld, a.dbias ? part : nullptr, a.M, a.N, a.act, a.dtype, w.st));
+  } else {
+    if (run && a.dbias) NSA_TRY(act_bwd(a.dy, nullptr, nullptr, 0, part, a.M, a.N, a.act, a.dtype, w.st));
+    if (a.dx || a.dw || !run) NSA_TRY(operand(w, a.dy, a.M, a.N, a.dtype, &g));
+  }
+  if (run && a.dbias) NSA_TRY(column_sum(part, a.dbias, act_bwd_plan(a.M, a.N).groups, a.N, a.dtype, w.st));
+  if (a.dx || !run) {
+    NSA_TRY(operand(w, a.w, a.N, a.K, a.dtype, &wt));
+    NSA_TRY(product(w, problem(g, 0, wt, 1, a.M, a.K, a.N, a.dtype), run ? a.dx : &w));
+  }
+  if (a.dw || !run) {
+    NSA_TRY(operand(w, a.x, a.M, a.K, a.dtype, &x));
+    NSA_TRY(product(w, problem(g, 1, x, 1, a.N, a.K, a.M, a.dtype), run ? a.dw : &w));
+  }
   return NSA_OK;
 }
 
 int linear_bwd(const nsa_linear_bwd_args& a, cudaStream_t st) {
-  int rc = check_linear_bwd(a);
-  if (rc != NSA_OK) return rc;
+  NSA_TRY(check_linear_bwd(a));
   if (a.M == 0) {                                             // sums over no rows
-    if ((rc = zero(a.dw, (long long)a.N * a.K * 2, st)) != NSA_OK) return rc;
+    NSA_TRY(zero(a.dw, (long long)a.N * a.K * 2, st));
     return zero(a.dbias, (long long)a.N * 2, st);
   }
-  NSA_REQUIRE(a.dy && a.x && a.w && a.ws && (a.z || a.act == NSA_ACT_NONE), NSA_ERR_ARG, "linear backward: NULL pointer");
-  void* dz;
-  float* part;
-  const long long need = linear_bwd_ws(a, reinterpret_cast<unsigned char*>(a.ws), &dz, &part);
-  NSA_REQUIRE(a.ws_bytes >= need, NSA_ERR_ARG, "linear backward: workspace of %lld bytes, %lld needed", (long long)a.ws_bytes, need);
-  const void* g = a.dy;
-  if (a.act != NSA_ACT_NONE || a.dbias != nullptr) {
-    if ((rc = act_bwd(a.dy, a.z, dz, a.dbias ? part : nullptr, a.M, a.N, a.act, a.dtype, st)) != NSA_OK) return rc;
-    if (a.act != NSA_ACT_NONE) g = dz;
-    if (a.dbias != nullptr && (rc = column_sum(part, a.dbias, act_bwd_plan(a.M, a.N).groups, a.N, a.dtype, st)) != NSA_OK) return rc;
-  }
-  if ((rc = product(problem(g, 0, a.N, a.w, 1, a.K, a.M, a.K, a.N, a.dtype), a.dx, st)) != NSA_OK) return rc;
-  return product(problem(g, 1, a.N, a.x, 1, a.K, a.N, a.K, a.M, a.dtype), a.dw, st);
+  NSA_REQUIRE(a.dy && a.x && a.w && (a.z || a.act == NSA_ACT_NONE), NSA_ERR_ARG, "linear backward: NULL pointer");
+  return run_steps("linear backward", a, linear_bwd_steps, st);
 }
 
 // ---------------------------------------------------------------- gated feed-forward block
@@ -172,70 +245,82 @@ static int check_mlp(int M, int N, int F, int dtype, int act) {
   NSA_REQUIRE(act >= NSA_ACT_NONE && act <= NSA_ACT_RELU, NSA_ERR_ARG, "gated_mlp: activation %d", act);
   return NSA_OK;
 }
-static long long mlp_ws(const nsa_gated_mlp_args& a, unsigned char* base, void** h) {
-  Arena w{base};
-  *h = w.take((long long)a.M * a.F * 2);
-  return w.at;
-}
 
-int gated_mlp(const nsa_gated_mlp_args& a, cudaStream_t st) {
-  int rc = check_mlp(a.M, a.N, a.F, a.dtype, a.act);
-  if (rc != NSA_OK) return rc;
-  if (a.M == 0) return NSA_OK;
-  NSA_REQUIRE(a.x && a.wg && a.wu && a.wd && a.y && a.ws, NSA_ERR_ARG, "gated_mlp: NULL pointer");
-  NSA_REQUIRE((a.g == nullptr) == (a.u == nullptr), NSA_ERR_ARG, "gated_mlp: give both g and u or neither");
-  void* h;
-  const long long need = mlp_ws(a, reinterpret_cast<unsigned char*>(a.ws), &h);
-  NSA_REQUIRE(a.ws_bytes >= need, NSA_ERR_ARG, "gated_mlp: workspace of %lld bytes, %lld needed", (long long)a.ws_bytes, need);
-  GemmProblem p = problem(a.x, 0, a.N, a.wg, 0, a.N, a.M, a.F, a.N, a.dtype);
-  p.B[1] = a.wu;
+static int mlp_steps(const nsa_gated_mlp_args& a, Arena& w) {
+  const long long ldh = padded(a.F, a.dtype);
+  void* h = w.take((long long)a.M * ldh * 2);
+  Mat x, wg, wu, wd;
+  NSA_TRY(operand(w, a.x, a.M, a.N, a.dtype, &x));
+  NSA_TRY(operand(w, a.wg, a.F, a.N, a.dtype, &wg));
+  NSA_TRY(operand(w, a.wu, a.F, a.N, a.dtype, &wu));
+  GemmProblem p = problem(x, 0, wg, 0, a.M, a.F, a.N, a.dtype);
+  p.B[1] = wu.p;
   p.e.mode = EPI_GLU;
   p.e.act = a.act;
-  p.e.y = h; p.e.o1 = a.g; p.e.o2 = a.u;
-  p.e.vec = a.F % 8 == 0 && aligned16(h) && aligned16(a.g) && aligned16(a.u);
-  if ((rc = gemm(p, st)) != NSA_OK) return rc;
-  GemmProblem d = problem(h, 0, a.F, a.wd, 0, a.F, a.M, a.N, a.F, a.dtype);
+  p.e.y = h; p.e.ldy = ldh; p.e.vecy = 1;
+  p.e.o1 = a.g; p.e.o2 = a.u;
+  p.e.vec = a.F % 8 == 0 && aligned16(a.g) && aligned16(a.u);
+  NSA_TRY(gemm(w, p));
+  NSA_TRY(operand(w, a.wd, a.N, a.F, a.dtype, &wd));
+  GemmProblem d = problem(Mat{h, ldh}, 0, wd, 0, a.M, a.N, a.F, a.dtype);
   d.e.mode = EPI_LINEAR;
   d.e.residual = a.residual;
   d.e.y = a.y;
-  d.e.vec = a.N % 8 == 0 && aligned16(a.residual) && aligned16(a.y);
-  return gemm(d, st);
+  d.e.vec = a.N % 8 == 0 && aligned16(a.residual);
+  d.e.vecy = a.N % 8 == 0 && aligned16(a.y);
+  return gemm(w, d);
 }
 
-static long long mlp_bwd_ws(const nsa_gated_mlp_bwd_args& a, unsigned char* base, void** dg, void** du, void** h) {
-  Arena w{base};
-  *dg = w.take((long long)a.M * a.F * 2);
-  *du = w.take((long long)a.M * a.F * 2);
-  *h = w.take((long long)a.M * a.F * 2);
-  return w.at;
+int gated_mlp(const nsa_gated_mlp_args& a, cudaStream_t st) {
+  NSA_TRY(check_mlp(a.M, a.N, a.F, a.dtype, a.act));
+  if (a.M == 0) return NSA_OK;
+  NSA_REQUIRE(a.x && a.wg && a.wu && a.wd && a.y, NSA_ERR_ARG, "gated_mlp: NULL pointer");
+  NSA_REQUIRE((a.g == nullptr) == (a.u == nullptr), NSA_ERR_ARG, "gated_mlp: give both g and u or neither");
+  return run_steps("gated_mlp", a, mlp_steps, st);
 }
 
-int gated_mlp_bwd(const nsa_gated_mlp_bwd_args& a, cudaStream_t st) {
-  int rc = check_mlp(a.M, a.N, a.F, a.dtype, a.act);
-  if (rc != NSA_OK) return rc;
-  if (a.M == 0) {
-    const long long bytes = (long long)a.N * a.F * 2;
-    if ((rc = zero(a.dwg, bytes, st)) != NSA_OK || (rc = zero(a.dwu, bytes, st)) != NSA_OK) return rc;
-    return zero(a.dwd, bytes, st);
-  }
-  NSA_REQUIRE(a.dy && a.x && a.wg && a.wu && a.wd && a.g && a.u && a.ws, NSA_ERR_ARG, "gated_mlp backward: NULL pointer");
-  void *dg, *du, *h;
-  const long long need = mlp_bwd_ws(a, reinterpret_cast<unsigned char*>(a.ws), &dg, &du, &h);
-  NSA_REQUIRE(a.ws_bytes >= need, NSA_ERR_ARG, "gated_mlp backward: workspace of %lld bytes, %lld needed", (long long)a.ws_bytes, need);
-  GemmProblem p = problem(a.dy, 0, a.N, a.wd, 1, a.F, a.M, a.F, a.N, a.dtype);             // dh = dy wd
+static int mlp_bwd_steps(const nsa_gated_mlp_bwd_args& a, Arena& w) {
+  const bool run = !w.dry();
+  const long long ldh = padded(a.F, a.dtype);
+  void *dg = w.take((long long)a.M * ldh * 2), *du = w.take((long long)a.M * ldh * 2), *h = w.take((long long)a.M * ldh * 2);
+  Mat dy, x, wg, wu, wd;
+  NSA_TRY(operand(w, a.dy, a.M, a.N, a.dtype, &dy));
+  NSA_TRY(operand(w, a.wd, a.N, a.F, a.dtype, &wd));
+  GemmProblem p = problem(dy, 0, wd, 1, a.M, a.F, a.N, a.dtype);                            // dh = dy wd
   p.e.mode = EPI_GLU_BWD;
   p.e.act = a.act;
   p.e.i0 = a.g; p.e.i1 = a.u;
-  p.e.y = dg; p.e.o1 = du; p.e.o2 = h;
   p.e.vec = a.F % 8 == 0 && aligned16(a.g) && aligned16(a.u);
-  if ((rc = gemm(p, st)) != NSA_OK) return rc;
-  GemmProblem x = problem(dg, 0, a.F, a.wg, 1, a.N, a.M, a.N, a.F, a.dtype);               // dx = dg wg + du wu
-  x.A[1] = du; x.B[1] = a.wu;
-  x.segments = 2;
-  if ((rc = product(x, a.dx, st)) != NSA_OK) return rc;
-  if ((rc = product(problem(dg, 1, a.F, a.x, 1, a.N, a.F, a.N, a.M, a.dtype), a.dwg, st)) != NSA_OK) return rc;
-  if ((rc = product(problem(du, 1, a.F, a.x, 1, a.N, a.F, a.N, a.M, a.dtype), a.dwu, st)) != NSA_OK) return rc;
-  return product(problem(a.dy, 1, a.N, h, 1, a.F, a.N, a.F, a.M, a.dtype), a.dwd, st);
+  p.e.y = dg; p.e.o1 = du; p.e.o2 = h;
+  p.e.ldy = ldh; p.e.vecy = 1;
+  NSA_TRY(gemm(w, p));
+  if (a.dx || !run) {                                                                       // dx = dg wg + du wu
+    NSA_TRY(operand(w, a.wg, a.F, a.N, a.dtype, &wg));
+    NSA_TRY(operand(w, a.wu, a.F, a.N, a.dtype, &wu));
+    GemmProblem q = problem(Mat{dg, ldh}, 0, wg, 1, a.M, a.N, a.F, a.dtype);
+    q.A[1] = du; q.B[1] = wu.p;
+    q.segments = 2;
+    NSA_TRY(product(w, q, run ? a.dx : &w));
+  }
+  if (a.dwg || a.dwu || !run) {
+    NSA_TRY(operand(w, a.x, a.M, a.N, a.dtype, &x));
+    NSA_TRY(product(w, problem(Mat{dg, ldh}, 1, x, 1, a.F, a.N, a.M, a.dtype), run ? a.dwg : &w));
+    NSA_TRY(product(w, problem(Mat{du, ldh}, 1, x, 1, a.F, a.N, a.M, a.dtype), run ? a.dwu : &w));
+  }
+  if (a.dwd || !run) NSA_TRY(product(w, problem(dy, 1, Mat{h, ldh}, 1, a.N, a.F, a.M, a.dtype), run ? a.dwd : &w));
+  return NSA_OK;
+}
+
+int gated_mlp_bwd(const nsa_gated_mlp_bwd_args& a, cudaStream_t st) {
+  NSA_TRY(check_mlp(a.M, a.N, a.F, a.dtype, a.act));
+  if (a.M == 0) {
+    const long long bytes = (long long)a.N * a.F * 2;
+    NSA_TRY(zero(a.dwg, bytes, st));
+    NSA_TRY(zero(a.dwu, bytes, st));
+    return zero(a.dwd, bytes, st);
+  }
+  NSA_REQUIRE(a.dy && a.x && a.wg && a.wu && a.wd && a.g && a.u, NSA_ERR_ARG, "gated_mlp backward: NULL pointer");
+  return run_steps("gated_mlp backward", a, mlp_bwd_steps, st);
 }
 
 int rms_norm(const nsa_norm_args&, cudaStream_t);
@@ -317,7 +402,7 @@ int nsa_rope_axes(const nsa_rope_axes_args* a, nsa_stream_t stream) {
 int64_t nsa_linear_ws_bytes(const nsa_linear_args* a) {
   NSA_REQUIRE(a, NSA_ERR_ARG, "linear: NULL argument block");
   const int rc = check_linear(*a);
-  return rc != NSA_OK ? rc : 0;
+  return rc != NSA_OK ? rc : a->M == 0 ? 0 : ws_bytes(*a, linear_steps);
 }
 int nsa_linear(const nsa_linear_args* a, nsa_stream_t stream) {
   NSA_REQUIRE(a, NSA_ERR_ARG, "linear: NULL argument block");
@@ -326,9 +411,7 @@ int nsa_linear(const nsa_linear_args* a, nsa_stream_t stream) {
 int64_t nsa_linear_bwd_ws_bytes(const nsa_linear_bwd_args* a) {
   NSA_REQUIRE(a, NSA_ERR_ARG, "linear backward: NULL argument block");
   const int rc = check_linear_bwd(*a);
-  void* dz;
-  float* part;
-  return rc != NSA_OK ? rc : linear_bwd_ws(*a, nullptr, &dz, &part);
+  return rc != NSA_OK ? rc : a->M == 0 ? 0 : ws_bytes(*a, linear_bwd_steps);
 }
 int nsa_linear_bwd(const nsa_linear_bwd_args* a, nsa_stream_t stream) {
   NSA_REQUIRE(a, NSA_ERR_ARG, "linear backward: NULL argument block");
@@ -337,8 +420,7 @@ int nsa_linear_bwd(const nsa_linear_bwd_args* a, nsa_stream_t stream) {
 int64_t nsa_gated_mlp_ws_bytes(const nsa_gated_mlp_args* a) {
   NSA_REQUIRE(a, NSA_ERR_ARG, "gated_mlp: NULL argument block");
   const int rc = check_mlp(a->M, a->N, a->F, a->dtype, a->act);
-  void* h;
-  return rc != NSA_OK ? rc : mlp_ws(*a, nullptr, &h);
+  return rc != NSA_OK ? rc : a->M == 0 ? 0 : ws_bytes(*a, mlp_steps);
 }
 int nsa_gated_mlp(const nsa_gated_mlp_args* a, nsa_stream_t stream) {
   NSA_REQUIRE(a, NSA_ERR_ARG, "gated_mlp: NULL argument block");
@@ -347,8 +429,7 @@ int nsa_gated_mlp(const nsa_gated_mlp_args* a, nsa_stream_t stream) {
 int64_t nsa_gated_mlp_bwd_ws_bytes(const nsa_gated_mlp_bwd_args* a) {
   NSA_REQUIRE(a, NSA_ERR_ARG, "gated_mlp backward: NULL argument block");
   const int rc = check_mlp(a->M, a->N, a->F, a->dtype, a->act);
-  void *dg, *du, *h;
-  return rc != NSA_OK ? rc : mlp_bwd_ws(*a, nullptr, &dg, &du, &h);
+  return rc != NSA_OK ? rc : a->M == 0 ? 0 : ws_bytes(*a, mlp_bwd_steps);
 }
 int nsa_gated_mlp_bwd(const nsa_gated_mlp_bwd_args* a, nsa_stream_t stream) {
   NSA_REQUIRE(a, NSA_ERR_ARG, "gated_mlp backward: NULL argument block");
