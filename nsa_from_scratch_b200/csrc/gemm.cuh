@@ -155,13 +155,7 @@ __device__ __forceinline__ void epilogue8(const Epi& e, long long row, int col, 
 
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
-static inline int sm_count() {
-  int dev = 0, sms = 148;
-  cudaGetDevice(&dev);
-  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-  return sms;
-}
-
+int sm_count();                                                            // of the current device (linear.cu)
 long long gemm_tc5_ws_bytes(const GemmProblem& p);                       // gemm_tc5.cu
 int gemm_tc5(const GemmProblem& p, void* ws, cudaStream_t st);
 int column_sum(const float* part, void* out, int parts, int N, int dt, cudaStream_t st);   // norm.cu

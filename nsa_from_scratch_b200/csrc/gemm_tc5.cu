@@ -428,7 +428,13 @@ template <int F, typename T, bool A_MN, bool B_MN, int MODE, int CG, int BN>
 static int tc_launch(const GemmTcParams& g, long long tiles, cudaStream_t st) {
   using S = TcShape<CG, BN>;
   auto fn = gemm_tc5_kernel<F, T, A_MN, B_MN, MODE, CG, BN>;
-  NSA_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+  static bool prepared[64];                   // per device: the attribute outlasts the call, and setting it twice is harmless
+  int dev = 0;
+  NSA_CUDA_OK(cudaGetDevice(&dev));
+  if (dev >= 64 || !prepared[dev]) {
+    NSA_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
+    if (dev < 64) prepared[dev] = true;
+  }
   const long long units = sm_count() / CG;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)((tiles < units ? tiles : units) * CG));

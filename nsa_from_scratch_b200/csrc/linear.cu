@@ -3,6 +3,17 @@
 
 namespace nsa {
 
+int sm_count() {
+  static int known[64];              // 0: not asked yet; every thread finds the same number
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && known[dev] > 0) return known[dev];
+  int sms = 148;
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  if (dev >= 0 && dev < 64) known[dev] = sms;
+  return sms;
+}
+
 // ---------------------------------------------------------------- gradient through the activation, bias gradient
 // dz = dy * act'(z) (ACT: an activation stands between) and the column sums of dz (part: a row of partial sums per
 // block row).  A thread owns 8 columns and walks the rows of its block row; bound by HBM.
@@ -13,23 +24,31 @@ __global__ void __launch_bounds__(128) act_bwd_kernel(const void* __restrict__ d
   if (n <= 0) return;
   const int r0 = blockIdx.y * rows, r1 = min(M, r0 + rows);
   float sum[8] = {};
-  for (int r = r0; r < r1; ++r) {
-    const long long at = (long long)r * N + c;
-    float d[8];
-    load8<T>(dy, at, n, vec, d);
-    if (act != ACT_NONE) {
-      float v[8];
-      load8<T>(z, at, n, vec, v);
+  constexpr int U = 4;                                        // rows under way at a time
+  for (int r = r0; r < r1; r += U) {
+    float d[U][8], v[U][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        float p, s;
-        act_both(v[i], act, p, s);
-        d[i] *= s;
-      }
-      store8<T>(dz, (long long)r * lddz + c, n, vecz, d);
+    for (int q = 0; q < U; ++q) {
+      if (r + q >= r1) break;
+      const long long at = (long long)(r + q) * N + c;
+      load8<T>(dy, at, n, vec, d[q]);
+      if (act != ACT_NONE) load8<T>(z, at, n, vec, v[q]);
     }
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum[i] += d[i];
+    for (int q = 0; q < U; ++q) {
+      if (r + q >= r1) break;
+      if (act != ACT_NONE) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          float p, s;
+          act_both(v[q][i], act, p, s);
+          d[q][i] *= s;
+        }
+        store8<T>(dz, (long long)(r + q) * lddz + c, n, vecz, d[q]);
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum[i] += d[q][i];
+    }
   }
   if (part != nullptr) {
 #pragma unroll
@@ -42,7 +61,7 @@ struct ActBwdPlan { int strips, groups, rows; };
 static ActBwdPlan act_bwd_plan(int M, int N) {
   ActBwdPlan p;
   p.strips = (N + 1023) / 1024;
-  const int want = (4 * sm_count() + p.strips - 1) / p.strips;                  // four blocks an SM
+  const int want = (8 * sm_count() + p.strips - 1) / p.strips;                  // eight blocks an SM
   p.rows = (M + want - 1) / want;
   if (p.rows < 1) p.rows = 1;
   p.groups = (M + p.rows - 1) / p.rows;

@@ -102,7 +102,7 @@ __device__ __forceinline__ uint32_t to_f8x4(const float* v, float inv, int fmt) 
 
 // X: type of x (and of a 16-bit or fp32 result); R: type of the residual stream; NORM 0: quantise the rows of x as they are
 template <typename X, typename R, int V, bool OUT8, bool NORM>
-__global__ void __launch_bounds__(V * 128) rms_norm_kernel(const NormParams p) {
+__global__ void __launch_bounds__(V == 1 ? 128 : 512) rms_norm_kernel(const NormParams p) {
   __shared__ float part[32];
   __shared__ uint32_t mpart[32];
   const long long row = blockIdx.x;
@@ -221,9 +221,9 @@ __global__ void __launch_bounds__(256) rms_norm_any_kernel(const NormParams p) {
 }
 
 // Threads of a row and vectors per thread: 1 vector up to 1024 columns (a short row still spreads over several warps),
-// 2 up to 4096, else 4; more than 16384 columns go to the kernel that re-reads the row.
-static int vectors_for(int N) { return N <= 1024 ? 1 : N <= 4096 ? 2 : 4; }
-static int threads_for(int N, int V) { return ((N / 8 + V - 1) / V + 31) / 32 * 32; }
+// 2 up to 8192, else 4; more than 16384 columns go to the kernel that re-reads the row.
+static int vectors_for(int N) { return N <= 1024 ? 1 : N <= 8192 ? 2 : 4; }
+static int threads_for(int N, int V) { return N < 8 ? 32 : ((N / 8 + V - 1) / V + 31) / 32 * 32; }
 
 template <typename X, typename R, bool OUT8, bool NORM>
 static int norm_launch(const NormParams& p, cudaStream_t st) {
@@ -271,9 +271,30 @@ struct NormBwdParams {
   int N, wdt;
 };
 
-// A block walks the rows b, b + grid, ...; its share of dw stays in registers and is written once.
-template <typename X, typename R, int V>
-__global__ void __launch_bounds__(V * 128) rms_norm_bwd_kernel(const NormBwdParams p) {
+// 8 elements as they are stored
+template <typename T> struct Raw {
+  uint4 v[sizeof(T) / 2];
+  __device__ __forceinline__ void load(const T* p) {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = reinterpret_cast<const uint4*>(p)[i];
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    if constexpr (sizeof(T) == 4) {
+      const float* q = reinterpret_cast<const float*>(v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = q[i];
+    } else {
+      const uint32_t* w = reinterpret_cast<const uint32_t*>(v);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) { const float2 t = Elem<T>::unpack(w[i]); f[2 * i] = t.x; f[2 * i + 1] = t.y; }
+    }
+  }
+};
+
+// A block walks the rows b, b + grid, ...; its share of dw stays in registers and is written once.  The next row is on its
+// way while this one is summed: with one or two blocks an SM, nothing else hides the loads.
+template <typename X, typename R, int V, bool DH>
+__global__ void __launch_bounds__(V == 1 ? 128 : 512) rms_norm_bwd_kernel(const NormBwdParams p) {
   __shared__ float part[2][32];
   const int vecs = p.N / 8, T = blockDim.x;
   float w[V][8], dw[V][8];
@@ -282,35 +303,54 @@ __global__ void __launch_bounds__(V * 128) rms_norm_bwd_kernel(const NormBwdPara
 #pragma unroll
     for (int i = 0; i < 8; ++i) w[v][i] = dw[v][i] = 0.f;
     const int c = threadIdx.x + v * T;
-    if (c < vecs) weight8(p.w, p.wdt, c * 8, w[v]);
+    if (V < 4 && c < vecs) weight8(p.w, p.wdt, c * 8, w[v]);
   }
   const float inv_n = 1.f / (float)p.N;
+  Raw<X> ry[V];
+  Raw<R> rh[V], rd[V];
+  float rr = 0.f;
+  auto fetch = [&](long long row) {
+    if (row >= p.rows) return;
+    rr = p.rstd[row];
+    const long long base = row * p.N;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+      const int c = threadIdx.x + v * T;
+      if (c < vecs) {
+        ry[v].load(reinterpret_cast<const X*>(p.dy) + base + c * 8);
+        rh[v].load(reinterpret_cast<const R*>(p.h) + base + c * 8);
+        if constexpr (DH) rd[v].load(reinterpret_cast<const R*>(p.dh) + base + c * 8);
+      }
+    }
+  };
+  constexpr bool AHEAD = V < 4;                             // with 4 vectors the next row and the weights do not fit the registers
+  if (AHEAD) fetch(blockIdx.x);
   int turn = 0;
   for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
+    if (!AHEAD) fetch(row);
     const long long base = row * p.N;
-    const float r = p.rstd[row];
+    const float r = rr;
     float u[V][8], n[V][8];
+    Raw<R> d[V];
     float dot = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = threadIdx.x + v * T;
       if (c < vecs) {
-        get8(reinterpret_cast<const X*>(p.dy), base + c * 8, u[v]);
-        get8(reinterpret_cast<const R*>(p.h), base + c * 8, n[v]);
-      } else {
+        ry[v].get(u[v]);
+        rh[v].get(n[v]);
+        if constexpr (DH) d[v] = rd[v];
+        if (!AHEAD) weight8(p.w, p.wdt, c * 8, w[v]);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) u[v][i] = n[v][i] = 0.f;
+        for (int i = 0; i < 8; ++i) {
+          n[v][i] *= r;
+          dw[v][i] = fmaf(u[v][i], n[v][i], dw[v][i]);
+          u[v][i] *= w[v][i];
+          dot = fmaf(u[v][i], n[v][i], dot);
+        }
       }
     }
-#pragma unroll
-    for (int v = 0; v < V; ++v)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        n[v][i] *= r;
-        dw[v][i] = fmaf(u[v][i], n[v][i], dw[v][i]);
-        u[v][i] *= w[v][i];
-        dot = fmaf(u[v][i], n[v][i], dot);
-      }
+    if (AHEAD) fetch(row + gridDim.x);
     dot = block_sum(dot, part[turn]) * inv_n;               // two sets of slots: a row's are read while the next one's are written
 #pragma unroll
     for (int v = 0; v < V; ++v) {
@@ -319,11 +359,11 @@ __global__ void __launch_bounds__(V * 128) rms_norm_bwd_kernel(const NormBwdPara
         float g[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) g[i] = r * (u[v][i] - n[v][i] * dot);
-        if (p.dh != nullptr) {
-          float d[8];
-          get8(reinterpret_cast<const R*>(p.dh), base + c * 8, d);
+        if constexpr (DH) {
+          float e[8];
+          d[v].get(e);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) g[i] += d[i];
+          for (int i = 0; i < 8; ++i) g[i] += e[i];
         }
         put8(reinterpret_cast<X*>(p.dx), base + c * 8, g);
         if (p.dres != nullptr) put8(reinterpret_cast<R*>(p.dres), base + c * 8, g);
@@ -391,34 +431,41 @@ int column_sum(const float* part, void* out, int parts, int N, int dt, cudaStrea
   return launch_status("column_sum");
 }
 
-// Blocks of the backward: enough to fill the SMs twice over, and no more, since each leaves a row of partial sums.
-static int norm_bwd_blocks(long long rows) {
-  const long long want = 2LL * sm_count();
+// Backward: 2 vectors a thread up to 8192 columns, else 4 (the weights and the sums of dw take 16 registers a vector).
+// Blocks: about 512 threads an SM, and no more, since each block leaves a row of partial sums.
+static int bwd_vectors_for(int N) { return N <= 1024 ? 1 : N <= 8192 ? 2 : 4; }
+static int norm_bwd_blocks(long long rows, int N) {
+  const int T = threads_for(N, bwd_vectors_for(N));
+  const long long want = (long long)sm_count() * (T >= 512 ? 1 : 512 / T);
   return (int)(rows < want ? rows : want);
 }
-long long rms_norm_bwd_ws_bytes(long long rows, int N) { return (long long)norm_bwd_blocks(rows) * N * 4; }
+long long rms_norm_bwd_ws_bytes(long long rows, int N) { return (long long)norm_bwd_blocks(rows, N) * N * 4; }
 
-template <typename X, typename R>
+template <typename X, typename R, bool DH>
 static int norm_bwd_launch(const NormBwdParams& p, int blocks, cudaStream_t st) {
   const bool vec = p.N % 8 == 0 && p.N <= 16384 && aligned16(p.dy) && aligned16(p.dh) && aligned16(p.h) && aligned16(p.w) && aligned16(p.dx) && aligned16(p.dres);
   if (!vec) rms_norm_bwd_any_kernel<X, R><<<blocks, 256, 0, st>>>(p);
   else {
-    const int V = vectors_for(p.N), T = threads_for(p.N, V);
-    if (V == 1) rms_norm_bwd_kernel<X, R, 1><<<blocks, T, 0, st>>>(p);
-    else if (V == 2) rms_norm_bwd_kernel<X, R, 2><<<blocks, T, 0, st>>>(p);
-    else rms_norm_bwd_kernel<X, R, 4><<<blocks, T, 0, st>>>(p);
+    const int V = bwd_vectors_for(p.N), T = threads_for(p.N, V);
+    if (V == 1) rms_norm_bwd_kernel<X, R, 1, DH><<<blocks, T, 0, st>>>(p);
+    else if (V == 2) rms_norm_bwd_kernel<X, R, 2, DH><<<blocks, T, 0, st>>>(p);
+    else rms_norm_bwd_kernel<X, R, 4, DH><<<blocks, T, 0, st>>>(p);
   }
   return launch_status("rms_norm_bwd");
 }
+template <typename X, typename R>
+static int norm_bwd_stream(const NormBwdParams& p, int blocks, cudaStream_t st) {
+  return p.dh != nullptr ? norm_bwd_launch<X, R, true>(p, blocks, st) : norm_bwd_launch<X, R, false>(p, blocks, st);
+}
 
 int rms_norm_bwd(const nsa_norm_bwd_args& a, cudaStream_t st) {
-  const int blocks = norm_bwd_blocks(a.rows);
+  const int blocks = norm_bwd_blocks(a.rows, a.hidden);
   const bool wide = a.res_dtype == NSA_FP32;
   NormBwdParams p{a.dy, a.dh, a.h, a.weight, a.rstd, a.dx, a.dres, reinterpret_cast<float*>(a.ws), a.rows, a.hidden, a.w_dtype};
   int rc;
-  if (a.x_dtype == NSA_FP32) rc = norm_bwd_launch<float, float>(p, blocks, st);
-  else if (a.x_dtype == NSA_FP16) rc = wide ? norm_bwd_launch<__half, float>(p, blocks, st) : norm_bwd_launch<__half, __half>(p, blocks, st);
-  else rc = wide ? norm_bwd_launch<__nv_bfloat16, float>(p, blocks, st) : norm_bwd_launch<__nv_bfloat16, __nv_bfloat16>(p, blocks, st);
+  if (a.x_dtype == NSA_FP32) rc = norm_bwd_stream<float, float>(p, blocks, st);
+  else if (a.x_dtype == NSA_FP16) rc = wide ? norm_bwd_stream<__half, float>(p, blocks, st) : norm_bwd_stream<__half, __half>(p, blocks, st);
+  else rc = wide ? norm_bwd_stream<__nv_bfloat16, float>(p, blocks, st) : norm_bwd_stream<__nv_bfloat16, __nv_bfloat16>(p, blocks, st);
   if (rc != NSA_OK || a.dweight == nullptr) return rc;
   return column_sum(p.part, a.dweight, blocks, a.hidden, a.w_dtype, st);
 }

@@ -14,7 +14,7 @@
 
 namespace nsa {
 
-constexpr int ROPE_TT = 4;            // tokens of a block: their rows of one head are a contiguous ROPE_TT * D run of the head-major side
+constexpr int ROPE_THREADS = 256;
 
 struct RopeParams {
   const void* x[3];
@@ -24,6 +24,7 @@ struct RopeParams {
   const double* inv_freq;
   int B, T, D, heads[3];
   int n_axes, sec_end[8], pos64, vec;
+  int tt;                             // tokens of a block: their rows of one head are a contiguous run of the head-major side
   int per_block;                      // heads of a block
 };
 
@@ -48,18 +49,19 @@ template <typename T> __device__ __forceinline__ void r_put8(T* p, const float (
   } else store8<T>(p, 0, 8, 1, v);
 }
 
-// X: type read, Y: type written; BACK: head-major to token-major with the angle reversed
-template <typename X, typename Y, bool BACK>
-__global__ void __launch_bounds__(256) rope_axes_kernel(const RopeParams p) {
-  extern __shared__ float2 cs[];                                   // [ROPE_TT][D/2] (cos, sin)
+// X: type read, Y: type written; BACK: head-major to token-major with the angle reversed; VEC: 16-byte rows.
+// VEC: a thread owns 8 columns and their 8 partners of one token, keeps the 8 (cos, sin) in registers and walks the heads.
+template <typename X, typename Y, bool BACK, bool VEC>
+__global__ void __launch_bounds__(ROPE_THREADS) rope_axes_kernel(const RopeParams p) {
+  extern __shared__ float2 cs[];                                   // [tt][D/2] (cos, sin)
   const int half = p.D / 2;
-  const int tiles = (p.T + ROPE_TT - 1) / ROPE_TT;
-  const int b = (int)(blockIdx.x / tiles), t0 = (int)(blockIdx.x % tiles) * ROPE_TT;
-  const int tn = min(ROPE_TT, p.T - t0);
+  const int tiles = (p.T + p.tt - 1) / p.tt;
+  const int b = (int)(blockIdx.x / tiles), t0 = (int)(blockIdx.x % tiles) * p.tt;
+  const int tn = min(p.tt, p.T - t0);
   const int all = p.heads[0] + p.heads[1] + p.heads[2], rotated = p.heads[0] + p.heads[1];
   const int h0 = blockIdx.y * p.per_block, h1 = min(all, h0 + p.per_block);
   if (h0 < rotated) {
-    for (int i = threadIdx.x; i < tn * half; i += 256) {
+    for (int i = threadIdx.x; i < tn * half; i += ROPE_THREADS) {
       const int t = i / half, j = i % half;
       int axis = 0;
       while (j >= p.sec_end[axis]) ++axis;                          // sec_end[n_axes - 1] == half
@@ -72,36 +74,54 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const RopeParams p) {
     }
     __syncthreads();
   }
-  const int chunks = p.vec ? p.D / 16 : half;                       // vec: 8 columns and their 8 partners a thread; else 1 and 1
-  const int per_head = tn * chunks;
-  for (int i = threadIdx.x; i < (h1 - h0) * per_head; i += 256) {
-    int h = h0 + i / per_head;
-    const int r = i % per_head, t = r / chunks, ch = r % chunks;
-    const bool turn = h < rotated;
-    const int which = h < p.heads[0] ? 0 : (turn ? 1 : 2);
+  // where head h (of q, k and v in a row) and token t start on either side
+  auto rows = [&](int h, int t, const X*& src, Y*& dst) {
+    const int which = h < p.heads[0] ? 0 : (h < rotated ? 1 : 2);
     if (which > 0) h -= p.heads[0];
     if (which > 1) h -= p.heads[1];
     const long long tok = (long long)b * p.xb[which] + (long long)(t0 + t) * p.xt[which] + (long long)h * p.D;
     const long long hm = (((long long)b * p.heads[which] + h) * p.T + t0 + t) * p.D;
-    const X* src = reinterpret_cast<const X*>(p.x[which]) + (BACK ? hm : tok);
-    Y* dst = reinterpret_cast<Y*>(p.y[which]) + (BACK ? tok : hm);
-    if (p.vec) {
+    src = reinterpret_cast<const X*>(p.x[which]) + (BACK ? hm : tok);
+    dst = reinterpret_cast<Y*>(p.y[which]) + (BACK ? tok : hm);
+  };
+  if constexpr (VEC) {
+    const int chunks = p.D / 16;
+    const int ch = threadIdx.x % chunks, rest = threadIdx.x / chunks, t = rest % p.tt;
+    const int step = ROPE_THREADS / chunks / p.tt, first = h0 + rest / p.tt;      // heads side by side
+    if (t >= tn || rest / p.tt >= step) return;
+    float2 w[8];
+    if (h0 < rotated) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) w[e] = cs[t * half + ch * 8 + e];
+    }
+#pragma unroll 2
+    for (int h = first; h < h1; h += step) {
+      const X* src;
+      Y* dst;
+      rows(h, t, src, dst);
       float lo[8], hi[8];
       r_get8(src + ch * 8, lo);
       r_get8(src + half + ch * 8, hi);
-      if (turn) {
+      if (h < rotated) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-          const float2 w = cs[t * half + ch * 8 + e];
           const float a = lo[e], c = hi[e];
-          lo[e] = fmaf(a, w.x, -c * w.y);
-          hi[e] = fmaf(c, w.x, a * w.y);
+          lo[e] = fmaf(a, w[e].x, -c * w[e].y);
+          hi[e] = fmaf(c, w[e].x, a * w[e].y);
         }
       }
       r_put8(dst + ch * 8, lo);
       r_put8(dst + half + ch * 8, hi);
-    } else {
+    }
+  } else {
+    const int per_head = tn * half;
+    for (int i = threadIdx.x; i < (h1 - h0) * per_head; i += ROPE_THREADS) {
+      const int h = h0 + i / per_head, r = i % per_head, t = r / half, ch = r % half;
+      const X* src;
+      Y* dst;
+      rows(h, t, src, dst);
       const float a = r_get(src + ch), c = r_get(src + half + ch);
+      const bool turn = h < rotated;
       const float2 w = turn ? cs[t * half + ch] : make_float2(1.f, 0.f);
       r_put(dst + ch, turn ? fmaf(a, w.x, -c * w.y) : a);
       r_put(dst + half + ch, turn ? fmaf(c, w.x, a * w.y) : c);
@@ -111,15 +131,21 @@ __global__ void __launch_bounds__(256) rope_axes_kernel(const RopeParams p) {
 
 template <typename X, typename Y, bool BACK>
 static int rope_launch(RopeParams& p, cudaStream_t st) {
-  const long long tiles = (long long)p.B * ((p.T + ROPE_TT - 1) / ROPE_TT);
+  // tokens of a block: as many as its threads cover side by side (a power of two, at most 32 and no more than there are)
+  const int side = p.vec ? ROPE_THREADS / (p.D / 16) : 4;
+  p.tt = 1;
+  while (p.tt * 2 <= side && p.tt < 32 && p.tt < p.T) p.tt *= 2;
+  const long long tiles = (long long)p.B * ((p.T + p.tt - 1) / p.tt);
   NSA_REQUIRE(tiles < 2147483647LL, NSA_ERR_ARG, "rope_axes: %d x %d tokens do not fit a grid", p.B, p.T);
   const int all = p.heads[0] + p.heads[1] + p.heads[2];
-  // few tokens: the heads are spread over blocks until every SM has two
-  long long ways = (2LL * sm_count() + tiles - 1) / tiles;
+  // few tokens: the heads are spread over blocks until every SM has several; a block's angles are formed anew in each
+  long long ways = (8LL * sm_count() + tiles - 1) / tiles;
   if (ways > all) ways = all;
   p.per_block = (int)((all + ways - 1) / ways);
   const dim3 grid((unsigned)tiles, (unsigned)((all + p.per_block - 1) / p.per_block));
-  rope_axes_kernel<X, Y, BACK><<<grid, 256, (size_t)ROPE_TT * (p.D / 2) * sizeof(float2), st>>>(p);
+  const size_t smem = (size_t)p.tt * (p.D / 2) * sizeof(float2);
+  if (p.vec) rope_axes_kernel<X, Y, BACK, true><<<grid, ROPE_THREADS, smem, st>>>(p);
+  else rope_axes_kernel<X, Y, BACK, false><<<grid, ROPE_THREADS, smem, st>>>(p);
   return launch_status("rope_axes");
 }
 

@@ -36,26 +36,46 @@ def _check(x: Tensor, weight: Tensor, residual: Optional[Tensor], what: str) -> 
             raise TypeError(f"{what}: residual must have x's dtype or fp32, got {residual.dtype} beside {x.dtype}")
 
 
-def _forward(x: Tensor, weight: Tensor, residual: Optional[Tensor], eps: float, y_dtype: torch.dtype, want_rstd: bool):
-    """(y, h or None, scale or None, rstd or None); dense operands."""
-    N = x.shape[-1]
-    rows = x.numel() // N if N else 0
-    y = torch.empty(x.shape, device=x.device, dtype=y_dtype)
-    h = None if residual is None else torch.empty_like(residual)
-    scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32) if y_dtype in ops._8 else None
-    rstd = torch.empty(rows, device=x.device, dtype=torch.float32) if want_rstd else None
-    xc = L.dtype_code(x.dtype)
-    a = L.NormArgs(x.data_ptr(), L.ptr(residual), weight.data_ptr(), y.data_ptr(), L.ptr(h), L.ptr(scale), L.ptr(rstd), rows, N, xc,
-                   xc if residual is None else L.dtype_code(residual.dtype), L.dtype_code(weight.dtype), L.dtype_code(y_dtype), eps)
+_plans = ops.Plans()
+
+
+def _plan(x: Tensor, weight: Tensor, residual: Optional[Tensor], eps: float, y_dtype: Optional[torch.dtype], what: str) -> bytes:
+    """nsa_norm_args without pointers, from checked operands; y_dtype None: x's."""
+    key = (x.shape, x.dtype, x.device, weight.shape, weight.dtype, weight.device, eps, y_dtype,
+           None if residual is None else (residual.shape, residual.dtype, residual.device))
+    plan = _plans.get(key)
+    if plan is None:
+        _check(x, weight, residual, what)
+        N, xc = x.shape[-1], L.dtype_code(x.dtype)
+        a = L.NormArgs(rows=x.numel() // N if N else 0, hidden=N, x_dtype=xc, res_dtype=xc if residual is None else L.dtype_code(residual.dtype),
+                       w_dtype=L.dtype_code(weight.dtype), y_dtype=xc if y_dtype is None else L.dtype_code(y_dtype), eps=eps)
+        plan = _plans.keep(key, bytes(a))
+    return plan
+
+
+def _forward(plan: bytes, x: Tensor, weight: Tensor, residual: Optional[Tensor], y: Tensor, scale: Optional[Tensor], want_rstd: bool):
+    """(h or None, rstd or None); dense operands."""
+    a = L.NormArgs.from_buffer_copy(plan)
+    a.x, a.weight, a.y = x.data_ptr(), weight.data_ptr(), y.data_ptr()
+    h = rstd = None
+    if residual is not None:
+        h = torch.empty_like(residual)
+        a.residual, a.h = residual.data_ptr(), h.data_ptr()
+    if scale is not None:
+        a.scale = scale.data_ptr()
+    if want_rstd:
+        rstd = x.new_empty(a.rows, dtype=torch.float32)
+        a.rstd = rstd.data_ptr()
     with L.on_device(x):
         L.check(L.load().nsa_rms_norm(C.byref(a), L.stream_ptr()), "nsa_rms_norm")
-    return y, h, scale, rstd
+    return h, rstd
 
 
 class _RmsNormFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, residual, weight, eps):
-        y, h, _, rstd = _forward(x, weight, residual, eps, x.dtype, True)
+    def forward(ctx, x, residual, weight, plan):
+        y = torch.empty_like(x)
+        h, rstd = _forward(plan, x, weight, residual, y, None, True)
         ctx.save_for_backward(x if h is None else h, weight, rstd)
         ctx.x_dtype, ctx.stream = x.dtype, residual is not None
         ctx.set_materialize_grads(False)
@@ -87,12 +107,14 @@ def rms_norm(x: Tensor, weight: Tensor, *, residual: Optional[Tensor] = None, ep
     """x [..., N] bf16, fp16 or fp32, weight [N] (x's dtype or fp32), residual like x (x's dtype or fp32).
     Returns y in x's dtype; with a residual (y, h), h = x + residual being the new stream in the residual's dtype.
     Differentiable wrt x, residual and weight."""
-    _check(x, weight, residual, "rms_norm")
+    plan = _plan(x, weight, residual, float(eps), None, "rms_norm")
     x, weight = ops._dense(x, "x"), ops._dense(weight, "weight")
-    residual = None if residual is None else ops._dense(residual, "residual")
+    if residual is not None:
+        residual = ops._dense(residual, "residual")
     if torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (residual is not None and residual.requires_grad)):
-        return _RmsNormFn.apply(x, residual, weight, float(eps))
-    y, h, _, _ = _forward(x, weight, residual, float(eps), x.dtype, False)
+        return _RmsNormFn.apply(x, residual, weight, plan)
+    y = torch.empty_like(x)
+    h, _ = _forward(plan, x, weight, residual, y, None, False)
     return y if h is None else (y, h)
 
 
@@ -102,10 +124,12 @@ def rms_norm_fp8(x: Tensor, weight: Tensor, *, residual: Optional[Tensor] = None
     per row: y ~= q * scale, scale = max(max|y|, 1e-12) / fmt_max.  Inference only."""
     if fmt not in ops._8:
         raise ValueError(f"unsupported fp8 format: {fmt}")
-    _check(x, weight, residual, "rms_norm_fp8")
+    plan = _plan(x, weight, residual, float(eps), fmt, "rms_norm_fp8")
     x, weight = ops._dense(x.detach(), "x"), ops._dense(weight.detach(), "weight")
-    residual = None if residual is None else ops._dense(residual.detach(), "residual")
-    q, h, scale, _ = _forward(x, weight, residual, float(eps), fmt, False)
+    if residual is not None:
+        residual = ops._dense(residual.detach(), "residual")
+    q, scale = torch.empty_like(x, dtype=fmt), x.new_empty(x.shape[:-1], dtype=torch.float32)
+    h, _ = _forward(plan, x, weight, residual, q, scale, False)
     return (q, scale) if h is None else (q, scale, h)
 
 

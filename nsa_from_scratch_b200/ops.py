@@ -99,6 +99,17 @@ def activation_code(name: Optional[str]) -> int:
         raise ValueError(f"unknown activation: {name}") from None
 
 
+class Plans(dict):
+    """What an entry point found out about operands of given shapes, types and devices (never about their addresses or
+    values): checked once, then an argument struct without pointers.  A program meets few; one that meets many starts over."""
+
+    def keep(self, key, plan):
+        if len(self) >= 256:
+            self.clear()
+        self[key] = plan
+        return plan
+
+
 def softmax_scale(D: int, scale: Optional[float]) -> float:
     return float(scale) if scale is not None else 1.0 / math.sqrt(D)
 
