@@ -504,13 +504,15 @@ int nsa_rope_axes(const nsa_rope_axes_args* args, nsa_stream_t stream);
 
 /* y = act(x w^T + bias) + residual:  x [M,K], w [N,K], bias [N], residual and y [M,N].
  * x and w: both bf16 or both fp16 (bias, residual and y share the type); or both e4m3 or both e5m2 with x_scale [M] and w_scale
- * [N] (y, bias and residual in y_dtype).  bias, residual NULL: none.  z (NULL: not wanted; 16-bit operands): act's
- * argument, kept for the backward.  Sums, bias, activation and residual in fp32, one rounding.
- * ws: nsa_linear_ws_bytes(&args) bytes (the pointers may still be NULL when it is asked; negative: bad arguments). */
+ * [N] (y, bias and residual in y_dtype).  bias, residual NULL: none.  slope [M,N] (NULL: not wanted; 16-bit operands with an
+ * activation): act' at act's argument, in x's type, for the backward.  Sums, bias, activation and residual in fp32, one
+ * rounding.
+ * ws: nsa_linear_ws_bytes(&args) bytes, asked with the pointers set (operands that are not 16-byte aligned are copied
+ * there); negative: bad arguments. */
 typedef struct nsa_linear_args {
   const void *x, *w, *bias, *residual;
   const float *x_scale, *w_scale;
-  void *y, *z, *ws;
+  void *y, *slope, *ws;
   int64_t ws_bytes;
   int32_t M, N, K;
   int32_t dtype, y_dtype, act;
@@ -518,24 +520,25 @@ typedef struct nsa_linear_args {
 int64_t nsa_linear_ws_bytes(const nsa_linear_args* args);
 int nsa_linear(const nsa_linear_args* args, nsa_stream_t stream);
 
-/* Gradients of nsa_linear (16-bit operands): dx [M,K], dw [N,K], dbias [N], each NULL if not wanted; residual's is dy. z may be
- * NULL where act is none.  Repeats bit for bit. */
+/* Gradients of nsa_linear (16-bit operands): dx [M,K], dw [N,K], dbias [N], each NULL if not wanted; residual's is dy.  has_act: an
+ * activation stood in the forward, and slope holds what it kept (NULL otherwise).  Repeats bit for bit. */
 typedef struct nsa_linear_bwd_args {
-  const void *dy, *x, *w, *z;
+  const void *dy, *x, *w, *slope;
   void *dx, *dw, *dbias, *ws;
   int64_t ws_bytes;
   int32_t M, N, K;
-  int32_t dtype, act;
+  int32_t dtype, has_act;
 } nsa_linear_bwd_args;
 int64_t nsa_linear_bwd_ws_bytes(const nsa_linear_bwd_args* args);
 int nsa_linear_bwd(const nsa_linear_bwd_args* args, nsa_stream_t stream);
 
 /* Gated feed-forward block:  y = (act(x wg^T) * (x wu^T)) wd^T + residual,  x, residual, y [M,N], wg and wu [F,N], wd [N,F], all of
- * one 16-bit type.  The gated product is held in that type between the two matrix products.  g, u [M,F] (both NULL: not
- * wanted): the two products, kept for the backward.  ws as for nsa_linear. */
+ * one 16-bit type.  The gated product h is held in that type between the two matrix products.  For the backward (all NULL: not
+ * wanted): p = act(x wg^T), s = act'(x wg^T) * (x wu^T) and h, [M,Fp] in that type, Fp being F rounded up to a multiple of 8,
+ * 16-byte aligned.  ws as for nsa_linear. */
 typedef struct nsa_gated_mlp_args {
   const void *x, *wg, *wu, *wd, *residual;
-  void *y, *g, *u, *ws;
+  void *y, *p, *s, *h, *ws;
   int64_t ws_bytes;
   int32_t M, N, F;
   int32_t dtype, act;
@@ -543,13 +546,13 @@ typedef struct nsa_gated_mlp_args {
 int64_t nsa_gated_mlp_ws_bytes(const nsa_gated_mlp_args* args);
 int nsa_gated_mlp(const nsa_gated_mlp_args* args, nsa_stream_t stream);
 
-/* Its gradients: dx [M,N], dwg and dwu [F,N], dwd [N,F], each NULL if not wanted; residual's is dy.  Repeats bit for bit. */
+/* Its gradients, from what the forward kept: dx [M,N], dwg and dwu [F,N], dwd [N,F], each NULL if not wanted; residual's is dy.  Repeats bit for bit. */
 typedef struct nsa_gated_mlp_bwd_args {
-  const void *dy, *x, *wg, *wu, *wd, *g, *u;
+  const void *dy, *x, *wg, *wu, *wd, *p, *s, *h;
   void *dx, *dwg, *dwu, *dwd, *ws;
   int64_t ws_bytes;
   int32_t M, N, F;
-  int32_t dtype, act;
+  int32_t dtype;
 } nsa_gated_mlp_bwd_args;
 int64_t nsa_gated_mlp_bwd_ws_bytes(const nsa_gated_mlp_bwd_args* args);
 int nsa_gated_mlp_bwd(const nsa_gated_mlp_bwd_args* args, nsa_stream_t stream);

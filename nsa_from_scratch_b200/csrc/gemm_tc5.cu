@@ -233,21 +233,40 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
     const int quarter = warp & 3, half = (warp - 4) >> 2;
     float* st = stage_f + (warp - 4) * 1024;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    constexpr int STEP = PAIR ? 16 : 32;                                 // result columns a step
+    constexpr int STEPS = NW / 2 / STEP;
+    constexpr int PASSES = PAIR ? 2 : 4, LPR = PAIR ? 2 : 4;             // a pass: LPR lanes of 8 columns to a row
+    constexpr bool RAW = MODE == EPI_PARTIAL || MODE == EPI_PARTIAL2;
+    using E = Epilogue<T, RAW ? EPI_LINEAR : MODE>;
+    const int my_row = lane / LPR, my_col = (lane % LPR) * 8;
     int n = 0;
     bool ok = true;
     for (int t = unit; t < tiles && ok; t += units, ++n) {
       int m0, n0, k0, k1, split;
       place(t, m0, n0, k0, k1, split);
       const int buf = n & 1;
+      const long long row0 = m0 + (int)rank * 128 + quarter * 32;
+      const int col0 = half * (NW / 2);
+      typename E::Row next[PASSES];
+      auto fetch = [&](int c) {                                          // what step c reads from global memory
+        if constexpr (!RAW) {
+#pragma unroll
+          for (int q = 0; q < PASSES; ++q) E::load_row(p.e, row0 + q * (32 / PASSES) + my_row, n0 + col0 + c * STEP + my_col, next[q]);
+        }
+      };
+      fetch(0);                                                          // lands while the tile is still being summed
       ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&tfull[buf]), (n >> 1) & 1, &abort_flag));
       if (!ok) { fail_id = 4; break; }
       tc_fence_after();
-      const long long row0 = m0 + (int)rank * 128 + quarter * 32;
-      constexpr int STEP = PAIR ? 16 : 32;                               // result columns a step
-      constexpr int STEPS = NW / 2 / STEP;
 #pragma unroll 1
       for (int c = 0; c < STEPS; ++c) {
-        const int col = half * (NW / 2) + c * STEP;
+        const int col = col0 + c * STEP;
+        typename E::Row now[PASSES];
+        typename E::Col cv;
+#pragma unroll
+        for (int q = 0; q < PASSES; ++q) now[q] = next[q];
+        if (c + 1 < STEPS) fetch(c + 1);
+        if constexpr (!RAW) E::load_col(p.e, n0 + col + my_col, cv);
         uint32_t v[32];
         if constexpr (PAIR) {
           uint32_t g[16], u[16];
@@ -289,24 +308,19 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
               if (cc + i < p.N) dst[i] = x[i];
           }
         };
-        if constexpr (PAIR) {
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const int r = q * 16 + (lane >> 1), cc = n0 + col + (lane & 1) * 8;
-            float a[8], b[8];
-            get8(r, (lane & 1) * 2, a);
-            get8(r, 4 + (lane & 1) * 2, b);
-            if constexpr (MODE == EPI_PARTIAL2) { put_raw(row0 + r, cc, 0, a); put_raw(row0 + r, cc, 1, b); }
-            else epilogue8<T, EPI_GLU>(p.e, row0 + r, cc, a, b);
-          }
-        } else {
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int r = q * 8 + (lane >> 2), cc = n0 + col + (lane & 3) * 8;
-            float a[8];
-            get8(r, (lane & 3) * 2, a);
-            if constexpr (MODE == EPI_PARTIAL) put_raw(row0 + r, cc, 0, a);
-            else epilogue8<T, MODE>(p.e, row0 + r, cc, a, a);
+        for (int q = 0; q < PASSES; ++q) {
+          const int r = q * (32 / PASSES) + my_row, cc = n0 + col + my_col;
+          float a[8];
+          get8(r, my_col / 4, a);
+          if constexpr (PAIR) {
+            float b[8];
+            get8(r, 4 + my_col / 4, b);
+            if constexpr (RAW) { put_raw(row0 + r, cc, 0, a); put_raw(row0 + r, cc, 1, b); }
+            else E::run(p.e, row0 + r, cc, cv, now[q], a, b);
+          } else {
+            if constexpr (RAW) put_raw(row0 + r, cc, 0, a);
+            else E::run(p.e, row0 + r, cc, cv, now[q], a, a);
           }
         }
         __syncwarp();
@@ -334,6 +348,11 @@ __global__ void __launch_bounds__(256) gemm_join_kernel(const float* __restrict_
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
     const long long row = i / groups;
     const int col = (int)(i % groups) * 8;
+    using E = Epilogue<T, MODE>;
+    typename E::Col cv;
+    typename E::Row rv;
+    E::load_col(e, col, cv);
+    E::load_row(e, row, col, rv);
     float a[PR][8] = {};
     for (int s = 0; s < splits; ++s) {
 #pragma unroll
@@ -350,7 +369,7 @@ __global__ void __launch_bounds__(256) gemm_join_kernel(const float* __restrict_
         }
       }
     }
-    epilogue8<T, MODE>(e, row, col, a[0], a[PR - 1]);
+    E::run(e, row, col, cv, rv, a[0], a[PR - 1]);
   }
 }
 

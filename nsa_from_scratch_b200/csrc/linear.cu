@@ -15,16 +15,17 @@ int sm_count() {
 }
 
 // ---------------------------------------------------------------- gradient through the activation, bias gradient
-// dz = dy * act'(z) (ACT: an activation stands between) and the column sums of dz (part: a row of partial sums per
-// block row).  A thread owns 8 columns and walks the rows of its block row; bound by HBM.
+// dz = dy * slope (slope = act'(z) from the forward; NULL: no activation, nothing is written) and the column sums of dz
+// (part: a row of partial sums per block row; NULL: not wanted).  A thread owns 8 columns and walks the rows of its
+// block row, four under way at a time; bound by HBM.
 template <typename T>
-__global__ void __launch_bounds__(128) act_bwd_kernel(const void* __restrict__ dy, const void* __restrict__ z, void* __restrict__ dz,
-                                                      float* __restrict__ part, int M, int N, long long lddz, int rows, int act, int vec, int vecz) {
+__global__ void __launch_bounds__(128) act_bwd_kernel(const void* __restrict__ dy, const void* __restrict__ slope, void* __restrict__ dz,
+                                                      float* __restrict__ part, int M, int N, long long lddz, int rows, int vec, int vecz) {
   const int c = (blockIdx.x * 128 + threadIdx.x) * 8, n = N - c;
   if (n <= 0) return;
   const int r0 = blockIdx.y * rows, r1 = min(M, r0 + rows);
   float sum[8] = {};
-  constexpr int U = 4;                                        // rows under way at a time
+  constexpr int U = 4;
   for (int r = r0; r < r1; r += U) {
     float d[U][8], v[U][8];
 #pragma unroll
@@ -32,18 +33,14 @@ __global__ void __launch_bounds__(128) act_bwd_kernel(const void* __restrict__ d
       if (r + q >= r1) break;
       const long long at = (long long)(r + q) * N + c;
       load8<T>(dy, at, n, vec, d[q]);
-      if (act != ACT_NONE) load8<T>(z, at, n, vec, v[q]);
+      if (slope != nullptr) load8<T>(slope, at, n, vec, v[q]);
     }
 #pragma unroll
     for (int q = 0; q < U; ++q) {
       if (r + q >= r1) break;
-      if (act != ACT_NONE) {
+      if (slope != nullptr) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          float p, s;
-          act_both(v[q][i], act, p, s);
-          d[q][i] *= s;
-        }
+        for (int i = 0; i < 8; ++i) d[q][i] *= v[q][i];
         store8<T>(dz, (long long)(r + q) * lddz + c, n, vecz, d[q]);
       }
 #pragma unroll
@@ -68,12 +65,12 @@ static ActBwdPlan act_bwd_plan(int M, int N) {
   return p;
 }
 
-static int act_bwd(const void* dy, const void* z, void* dz, long long lddz, float* part, int M, int N, int act, int dtype, cudaStream_t st) {
+static int act_bwd(const void* dy, const void* slope, void* dz, long long lddz, float* part, int M, int N, int dtype, cudaStream_t st) {
   const ActBwdPlan p = act_bwd_plan(M, N);
-  const int vec = N % 8 == 0 && aligned16(dy) && aligned16(z), vecz = lddz % 8 == 0;
+  const int vec = N % 8 == 0 && aligned16(dy) && aligned16(slope), vecz = lddz % 8 == 0;
   const dim3 grid(p.strips, p.groups);
-  if (dtype == NSA_BF16) act_bwd_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(dy, z, dz, part, M, N, lddz, p.rows, act, vec, vecz);
-  else act_bwd_kernel<__half><<<grid, 128, 0, st>>>(dy, z, dz, part, M, N, lddz, p.rows, act, vec, vecz);
+  if (dtype == NSA_BF16) act_bwd_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(dy, slope, dz, part, M, N, lddz, p.rows, vec, vecz);
+  else act_bwd_kernel<__half><<<grid, 128, 0, st>>>(dy, slope, dz, part, M, N, lddz, p.rows, vec, vecz);
   return launch_status("act_bwd");
 }
 
@@ -200,8 +197,8 @@ static int linear_steps(const nsa_linear_args& a, Arena& w) {
   p.e.mode = EPI_LINEAR;
   p.e.act = a.act;
   p.e.bias = a.bias; p.e.residual = a.residual; p.e.xs = a.x_scale; p.e.ws = a.w_scale;
-  p.e.y = a.y; p.e.o1 = a.z;
-  p.e.vec = a.N % 8 == 0 && aligned16(a.bias) && aligned16(a.residual) && aligned16(a.z);
+  p.e.y = a.y; p.e.o1 = a.slope;
+  p.e.vec = a.N % 8 == 0 && aligned16(a.bias) && aligned16(a.residual) && aligned16(a.slope);
   p.e.vecy = a.N % 8 == 0 && aligned16(a.y);
   return gemm(w, p);
 }
@@ -211,14 +208,13 @@ int linear(const nsa_linear_args& a, cudaStream_t st) {
   if (a.M == 0) return NSA_OK;
   NSA_REQUIRE(a.x && a.w && a.y, NSA_ERR_ARG, "linear: NULL pointer");
   NSA_REQUIRE(is8(a.dtype) == (a.x_scale != nullptr) && is8(a.dtype) == (a.w_scale != nullptr), NSA_ERR_ARG, "linear: fp8 operands, and only they, have scales");
-  NSA_REQUIRE(a.z == nullptr || is16(a.dtype), NSA_ERR_UNSUPPORTED, "linear: fp8 operands keep nothing for a backward");
+  NSA_REQUIRE(a.slope == nullptr || (is16(a.dtype) && a.act != NSA_ACT_NONE), NSA_ERR_ARG, "linear: only an activation of 16-bit operands leaves a slope");
   return run_steps("linear", a, linear_steps, st);
 }
 
 static int check_linear_bwd(const nsa_linear_bwd_args& a) {
   NSA_REQUIRE(a.M >= 0 && a.N > 0 && a.K > 0, NSA_ERR_ARG, "linear backward: bad sizes M=%d N=%d K=%d", a.M, a.N, a.K);
   NSA_REQUIRE(is16(a.dtype), NSA_ERR_UNSUPPORTED, "linear backward: dtype %d", a.dtype);
-  NSA_REQUIRE(a.act >= NSA_ACT_NONE && a.act <= NSA_ACT_RELU, NSA_ERR_ARG, "linear backward: activation %d", a.act);
   return NSA_OK;
 }
 
@@ -226,13 +222,13 @@ static int linear_bwd_steps(const nsa_linear_bwd_args& a, Arena& w) {
   const bool run = !w.dry();
   Mat g, x, wt;
   float* part = reinterpret_cast<float*>(w.take((long long)act_bwd_plan(a.M, a.N).groups * a.N * 4));
-  if (a.act != NSA_ACT_NONE) {
+  if (a.has_act) {
     const long long ld = padded(a.N, a.dtype);
     void* dz = w.take((long long)a.M * ld * 2);
     g = Mat{dz, ld};
-    if (run) NSA_TRY(act_bwd(a.dy, a.z, dz, ld, a.dbias ? part : nullptr, a.M, a.N, a.act, a.dtype, w.st));
+    if (run) NSA_TRY(act_bwd(a.dy, a.slope, dz, ld, a.dbias ? part : nullptr, a.M, a.N, a.dtype, w.st));
   } else {
-    if (run && a.dbias) NSA_TRY(act_bwd(a.dy, nullptr, nullptr, 0, part, a.M, a.N, a.act, a.dtype, w.st));
+    if (run && a.dbias) NSA_TRY(act_bwd(a.dy, nullptr, nullptr, 0, part, a.M, a.N, a.dtype, w.st));
     if (a.dx || a.dw || !run) NSA_TRY(operand(w, a.dy, a.M, a.N, a.dtype, &g));
   }
   if (run && a.dbias) NSA_TRY(column_sum(part, a.dbias, act_bwd_plan(a.M, a.N).groups, a.N, a.dtype, w.st));
@@ -253,7 +249,7 @@ int linear_bwd(const nsa_linear_bwd_args& a, cudaStream_t st) {
     NSA_TRY(zero(a.dw, (long long)a.N * a.K * 2, st));
     return zero(a.dbias, (long long)a.N * 2, st);
   }
-  NSA_REQUIRE(a.dy && a.x && a.w && (a.z || a.act == NSA_ACT_NONE), NSA_ERR_ARG, "linear backward: NULL pointer");
+  NSA_REQUIRE(a.dy && a.x && a.w && (a.slope != nullptr) == (a.has_act != 0), NSA_ERR_ARG, "linear backward: NULL pointer");
   return run_steps("linear backward", a, linear_bwd_steps, st);
 }
 
@@ -267,7 +263,7 @@ static int check_mlp(int M, int N, int F, int dtype, int act) {
 
 static int mlp_steps(const nsa_gated_mlp_args& a, Arena& w) {
   const long long ldh = padded(a.F, a.dtype);
-  void* h = w.take((long long)a.M * ldh * 2);
+  void* h = a.h != nullptr ? a.h : w.take((long long)a.M * ldh * 2);
   Mat x, wg, wu, wd;
   NSA_TRY(operand(w, a.x, a.M, a.N, a.dtype, &x));
   NSA_TRY(operand(w, a.wg, a.F, a.N, a.dtype, &wg));
@@ -276,9 +272,8 @@ static int mlp_steps(const nsa_gated_mlp_args& a, Arena& w) {
   p.B[1] = wu.p;
   p.e.mode = EPI_GLU;
   p.e.act = a.act;
-  p.e.y = h; p.e.ldy = ldh; p.e.vecy = 1;
-  p.e.o1 = a.g; p.e.o2 = a.u;
-  p.e.vec = a.F % 8 == 0 && aligned16(a.g) && aligned16(a.u);
+  p.e.y = h; p.e.o1 = a.p; p.e.o2 = a.s;
+  p.e.ldy = ldh; p.e.vecy = 1;
   NSA_TRY(gemm(w, p));
   NSA_TRY(operand(w, a.wd, a.N, a.F, a.dtype, &wd));
   GemmProblem d = problem(Mat{h, ldh}, 0, wd, 0, a.M, a.N, a.F, a.dtype);
@@ -294,23 +289,22 @@ int gated_mlp(const nsa_gated_mlp_args& a, cudaStream_t st) {
   NSA_TRY(check_mlp(a.M, a.N, a.F, a.dtype, a.act));
   if (a.M == 0) return NSA_OK;
   NSA_REQUIRE(a.x && a.wg && a.wu && a.wd && a.y, NSA_ERR_ARG, "gated_mlp: NULL pointer");
-  NSA_REQUIRE((a.g == nullptr) == (a.u == nullptr), NSA_ERR_ARG, "gated_mlp: give both g and u or neither");
+  NSA_REQUIRE((a.p == nullptr) == (a.s == nullptr) && (a.p == nullptr) == (a.h == nullptr), NSA_ERR_ARG, "gated_mlp: give all of p, s and h or none");
+  NSA_REQUIRE(aligned16(a.p) && aligned16(a.s) && aligned16(a.h), NSA_ERR_ARG, "gated_mlp: p, s and h must be 16-byte aligned");
   return run_steps("gated_mlp", a, mlp_steps, st);
 }
 
 static int mlp_bwd_steps(const nsa_gated_mlp_bwd_args& a, Arena& w) {
   const bool run = !w.dry();
   const long long ldh = padded(a.F, a.dtype);
-  void *dg = w.take((long long)a.M * ldh * 2), *du = w.take((long long)a.M * ldh * 2), *h = w.take((long long)a.M * ldh * 2);
+  void *dg = w.take((long long)a.M * ldh * 2), *du = w.take((long long)a.M * ldh * 2);
   Mat dy, x, wg, wu, wd;
   NSA_TRY(operand(w, a.dy, a.M, a.N, a.dtype, &dy));
   NSA_TRY(operand(w, a.wd, a.N, a.F, a.dtype, &wd));
   GemmProblem p = problem(dy, 0, wd, 1, a.M, a.F, a.N, a.dtype);                            // dh = dy wd
   p.e.mode = EPI_GLU_BWD;
-  p.e.act = a.act;
-  p.e.i0 = a.g; p.e.i1 = a.u;
-  p.e.vec = a.F % 8 == 0 && aligned16(a.g) && aligned16(a.u);
-  p.e.y = dg; p.e.o1 = du; p.e.o2 = h;
+  p.e.i0 = a.p; p.e.i1 = a.s;
+  p.e.y = dg; p.e.o1 = du;
   p.e.ldy = ldh; p.e.vecy = 1;
   NSA_TRY(gemm(w, p));
   if (a.dx || !run) {                                                                       // dx = dg wg + du wu
@@ -326,19 +320,20 @@ static int mlp_bwd_steps(const nsa_gated_mlp_bwd_args& a, Arena& w) {
     NSA_TRY(product(w, problem(Mat{dg, ldh}, 1, x, 1, a.F, a.N, a.M, a.dtype), run ? a.dwg : &w));
     NSA_TRY(product(w, problem(Mat{du, ldh}, 1, x, 1, a.F, a.N, a.M, a.dtype), run ? a.dwu : &w));
   }
-  if (a.dwd || !run) NSA_TRY(product(w, problem(dy, 1, Mat{h, ldh}, 1, a.N, a.F, a.M, a.dtype), run ? a.dwd : &w));
+  if (a.dwd || !run) NSA_TRY(product(w, problem(dy, 1, Mat{a.h, ldh}, 1, a.N, a.F, a.M, a.dtype), run ? a.dwd : &w));
   return NSA_OK;
 }
 
 int gated_mlp_bwd(const nsa_gated_mlp_bwd_args& a, cudaStream_t st) {
-  NSA_TRY(check_mlp(a.M, a.N, a.F, a.dtype, a.act));
+  NSA_TRY(check_mlp(a.M, a.N, a.F, a.dtype, 0));
   if (a.M == 0) {
     const long long bytes = (long long)a.N * a.F * 2;
     NSA_TRY(zero(a.dwg, bytes, st));
     NSA_TRY(zero(a.dwu, bytes, st));
     return zero(a.dwd, bytes, st);
   }
-  NSA_REQUIRE(a.dy && a.x && a.wg && a.wu && a.wd && a.g && a.u, NSA_ERR_ARG, "gated_mlp backward: NULL pointer");
+  NSA_REQUIRE(a.dy && a.x && a.wg && a.wu && a.wd && a.p && a.s && a.h, NSA_ERR_ARG, "gated_mlp backward: NULL pointer");
+  NSA_REQUIRE(aligned16(a.p) && aligned16(a.s) && aligned16(a.h), NSA_ERR_ARG, "gated_mlp backward: p, s and h must be 16-byte aligned");
   return run_steps("gated_mlp backward", a, mlp_bwd_steps, st);
 }
 
@@ -447,7 +442,7 @@ int nsa_gated_mlp(const nsa_gated_mlp_args* a, nsa_stream_t stream) {
 }
 int64_t nsa_gated_mlp_bwd_ws_bytes(const nsa_gated_mlp_bwd_args* a) {
   NSA_REQUIRE(a, NSA_ERR_ARG, "gated_mlp backward: NULL argument block");
-  const int rc = check_mlp(a->M, a->N, a->F, a->dtype, a->act);
+  const int rc = check_mlp(a->M, a->N, a->F, a->dtype, 0);
   return rc != NSA_OK ? rc : a->M == 0 ? 0 : ws_bytes(*a, mlp_bwd_steps);
 }
 int nsa_gated_mlp_bwd(const nsa_gated_mlp_bwd_args* a, nsa_stream_t stream) {

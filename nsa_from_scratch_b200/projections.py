@@ -42,8 +42,8 @@ def _meta(*ts: Optional[Tensor]):
 _plans = ops.Plans()
 
 
-def _linear(plan: bytes, x: Tensor, w: Tensor, bias, residual, xs, ws, dtype: torch.dtype, want_z: bool):
-    """(y, z or None); dense operands."""
+def _linear(plan: bytes, x: Tensor, w: Tensor, bias, residual, xs, ws, dtype: torch.dtype, want_slope: bool):
+    """(y, slope or None); dense operands."""
     a = L.LinearArgs.from_buffer_copy(plan)
     y = x.new_empty((*x.shape[:-1], a.N), dtype=dtype)
     a.x, a.w, a.y = x.data_ptr(), w.data_ptr(), y.data_ptr()
@@ -53,27 +53,26 @@ def _linear(plan: bytes, x: Tensor, w: Tensor, bias, residual, xs, ws, dtype: to
         a.residual = residual.data_ptr()
     if xs is not None:
         a.x_scale, a.w_scale = xs.data_ptr(), ws.data_ptr()
-    z = None
-    if want_z:
-        z = torch.empty_like(y)
-        a.z = z.data_ptr()
+    slope = None
+    if want_slope:
+        slope = torch.empty_like(y)
+        a.slope = slope.data_ptr()
     lib = L.load()
     _run(a, lib.nsa_linear_ws_bytes, lib.nsa_linear, "nsa_linear", x)
-    return y, z
+    return y, slope
 
 
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, bias, residual, act, plan):
-        y, z = _linear(plan, x, w, bias, residual, None, None, x.dtype, act != 0 and any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(x, w, z)
-        ctx.act = act
+        y, slope = _linear(plan, x, w, bias, residual, None, None, x.dtype, act != 0 and any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(x, w, slope)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, w, z = ctx.saved_tensors
+        x, w, slope = ctx.saved_tensors
         dy = dy.contiguous()
         N, K = w.shape
         want_x, want_w, want_b, want_r = ctx.needs_input_grad[:4]
@@ -81,8 +80,8 @@ class _LinearFn(torch.autograd.Function):
         dw = torch.empty_like(w) if want_w else None
         db = x.new_empty(N) if want_b else None
         if want_x or want_w or want_b:
-            a = L.LinearBwdArgs(dy.data_ptr(), x.data_ptr(), w.data_ptr(), L.ptr(z), L.ptr(dx), L.ptr(dw), L.ptr(db), None, 0, x.numel() // K, N, K,
-                                L.dtype_code(x.dtype), ctx.act)
+            a = L.LinearBwdArgs(dy.data_ptr(), x.data_ptr(), w.data_ptr(), L.ptr(slope), L.ptr(dx), L.ptr(dw), L.ptr(db), None, 0, x.numel() // K, N, K,
+                                L.dtype_code(x.dtype), slope is not None)
             lib = L.load()
             _run(a, lib.nsa_linear_bwd_ws_bytes, lib.nsa_linear_bwd, "nsa_linear_bwd", x)
         return dx, dw, db, dy if want_r else None, None, None
@@ -92,7 +91,7 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, *, activati
            residual: Optional[Tensor] = None) -> Tensor:
     """act(x weight^T + bias) + residual.  x [..., K], weight [N, K], bias [N], residual [..., N], all bf16 or all fp16;
     activation None, "silu", "gelu_tanh" or "relu".  Returns [..., N] in x's dtype: fp32 sums and epilogue, one rounding.
-    Differentiable wrt x, weight, bias and residual (act's argument is kept in x's dtype for the backward)."""
+    Differentiable wrt x, weight, bias and residual (act' is kept in x's dtype for the backward)."""
     key = ("linear", activation, *_meta(x, weight, bias, residual))
     plan = _plans.get(key)
     if plan is None:
@@ -151,43 +150,42 @@ def linear_fp8(x: Tensor, weight: Tensor, x_scale: Tensor, w_scale: Tensor, bias
 
 
 def _mlp(plan: bytes, x, wg, wu, wd, residual, keep):
-    """(y, g or None, u or None); dense operands."""
+    """(y, kept): dense operands; kept is () or (act(g), act'(g) * u, act(g) * u) for the backward, rows padded to a multiple of 8."""
     a = L.GatedMlpArgs.from_buffer_copy(plan)
     y = torch.empty_like(x)
     a.x, a.wg, a.wu, a.wd, a.y = x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), y.data_ptr()
     if residual is not None:
         a.residual = residual.data_ptr()
-    g = u = None
+    kept = ()
     if keep:
-        g, u = x.new_empty((a.M, a.F)), x.new_empty((a.M, a.F))
-        a.g, a.u = g.data_ptr(), u.data_ptr()
+        kept = p, s, h = [x.new_empty((a.M, (a.F + 7) // 8 * 8)) for _ in range(3)]
+        a.p, a.s, a.h = p.data_ptr(), s.data_ptr(), h.data_ptr()
     lib = L.load()
     _run(a, lib.nsa_gated_mlp_ws_bytes, lib.nsa_gated_mlp, "nsa_gated_mlp", x)
-    return y, g, u
+    return y, kept
 
 
 class _GatedMlpFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, wg, wu, wd, residual, act, plan):
-        y, g, u = _mlp(plan, x, wg, wu, wd, residual, any(ctx.needs_input_grad[:4]))
-        ctx.save_for_backward(x, wg, wu, wd, g, u)
-        ctx.act = act
+    def forward(ctx, x, wg, wu, wd, residual, plan):
+        y, kept = _mlp(plan, x, wg, wu, wd, residual, any(ctx.needs_input_grad[:4]))
+        ctx.save_for_backward(x, wg, wu, wd, *kept)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, wg, wu, wd, g, u = ctx.saved_tensors
+        x, wg, wu, wd, *kept = ctx.saved_tensors
         dy = dy.contiguous()
         F, N = wg.shape
         M = x.numel() // N
         grads = [torch.empty_like(t) if want else None for t, want in zip((x, wg, wu, wd), ctx.needs_input_grad)]
         if any(ctx.needs_input_grad[:4]):
-            a = L.GatedMlpBwdArgs(dy.data_ptr(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), g.data_ptr(), u.data_ptr(),
-                                  *(L.ptr(t) for t in grads), None, 0, M, N, F, L.dtype_code(x.dtype), ctx.act)
+            a = L.GatedMlpBwdArgs(dy.data_ptr(), x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), *(t.data_ptr() for t in kept),
+                                  *(L.ptr(t) for t in grads), None, 0, M, N, F, L.dtype_code(x.dtype))
             lib = L.load()
             _run(a, lib.nsa_gated_mlp_bwd_ws_bytes, lib.nsa_gated_mlp_bwd, "nsa_gated_mlp_bwd", x)
-        return (*grads, dy if ctx.needs_input_grad[4] else None, None, None)
+        return (*grads, dy if ctx.needs_input_grad[4] else None, None)
 
 
 def gated_mlp(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, *, activation: Optional[str] = "silu",
@@ -208,14 +206,14 @@ def gated_mlp(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, *, activa
             raise ValueError(f"gated_mlp: x {tuple(x.shape)} and weights {tuple(w_gate.shape)}, {tuple(w_up.shape)}, {tuple(w_down.shape)} do not match")
         _check_rows(residual, "residual", x.shape, x.dtype, "gated_mlp")
         F, N = w_gate.shape
-        plan = _plans.keep(key, (bytes(L.GatedMlpArgs(M=x.numel() // N, N=N, F=F, dtype=L.dtype_code(x.dtype), act=act)), act))
+        plan = _plans.keep(key, bytes(L.GatedMlpArgs(M=x.numel() // N, N=N, F=F, dtype=L.dtype_code(x.dtype), act=act)))
     x, w_gate, w_up, w_down = ops._dense(x, "x"), ops._dense(w_gate, "w_gate"), ops._dense(w_up, "w_up"), ops._dense(w_down, "w_down")
     if residual is not None:
         residual = ops._dense(residual, "residual")
     if torch.is_grad_enabled() and (x.requires_grad or w_gate.requires_grad or w_up.requires_grad or w_down.requires_grad
                                     or (residual is not None and residual.requires_grad)):
-        return _GatedMlpFn.apply(x, w_gate, w_up, w_down, residual, plan[1], plan[0])
-    return _mlp(plan[0], x, w_gate, w_up, w_down, residual, False)[0]
+        return _GatedMlpFn.apply(x, w_gate, w_up, w_down, residual, plan)
+    return _mlp(plan, x, w_gate, w_up, w_down, residual, False)[0]
 
 
 __all__ = ["linear", "linear_fp8", "gated_mlp"]

@@ -307,11 +307,13 @@ def test_linear(nsa, M, N, K, dtype, bias, act, res):
 
 def linear_backward_bounds(x, w, b, act, dy, dtype):
     half, tiny = HALF[dtype], TINY[dtype]
-    _, z, dz_err = linear64(x, w, b, act, None)
-    zerr = dz_err + half * z.abs() + tiny                                      # z is kept in 16 bits
+    _, z, zerr = linear64(x, w, b, act, None)
     s = slope64(z, act)
+    serr = slope_error(z, zerr, act)
+    if act is not None:
+        serr = (1 + half) * serr + half * s.abs() + tiny                        # act' is kept in 16 bits
     g = dy.double() * s
-    gerr = (half * g.abs() + tiny) * (act is not None) + (1 + half) * dy.double().abs() * slope_error(z, zerr, act)
+    gerr = (half * g.abs() + tiny) * (act is not None) + (1 + half) * dy.double().abs() * serr
     out = {}
     for name, a, c, n in (("dx", g, w.double(), w.shape[0]), ("dw", g.T, x.double(), x.shape[0])):
         err = gerr if name == "dx" else gerr.T
@@ -414,7 +416,6 @@ def test_gated_mlp_backward(nsa, M, N, F, dtype, act, res):
     assert all(torch.equal(p, q) for p, q in zip(grads, again))
     xd, wg, wu, wd, dyd = (t.detach().double() for t in (x, *ws, dy))
     g, u, ge, ue = mlp_products(xd, wg, wu)
-    ge, ue = ge + half * g.abs() + tiny, ue + half * u.abs() + tiny             # kept in 16 bits
     a, s = act64(g, act), slope64(g, act)
     ae, se = 1.2 * ge + 4 * FN * (g.abs() + 1) * (act is not None), slope_error(g, ge, act)
     dh = dyd @ wd
@@ -428,8 +429,9 @@ def test_gated_mlp_backward(nsa, M, N, F, dtype, act, res):
         err = hi - v.abs() + 4 * U * hi
         return v, (1 + half) * err + half * v.abs() + tiny
 
-    dg, dge = product((dh, dhe), (u, ue), (s, se))
-    du, due = product((dh, dhe), (a, ae))
+    # act(g), act'(g) u and act(g) u are kept in 16 bits
+    dg, dge = product((dh, dhe), product((u, ue), (s, se)))
+    du, due = product((dh, dhe), product((a, ae)))
     h, he = product((a, ae), (u, ue))
 
     def contract(pairs, n):

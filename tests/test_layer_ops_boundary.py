@@ -68,14 +68,14 @@ def test_c_entry_points_refuse():
     refused(lib.nsa_linear(C.byref(a), None), ARG, "scales")
     a.dtype, a.K = 0, 0
     refused(lib.nsa_linear(C.byref(a), None), ARG, "bad sizes")
-    b = L.LinearBwdArgs(dy=16, x=16, w=16, M=4, N=8, K=8, dtype=0, act=1, ws=16)
-    refused(lib.nsa_linear_bwd(C.byref(b), None), ARG, "NULL pointer")              # no z beside an activation
-    b.z = 16
+    b = L.LinearBwdArgs(dy=16, x=16, w=16, M=4, N=8, K=8, dtype=0, has_act=1, ws=16)
+    refused(lib.nsa_linear_bwd(C.byref(b), None), ARG, "NULL pointer")              # no slope beside an activation
+    b.slope = 16
     refused(lib.nsa_linear_bwd(C.byref(b), None), ARG, "workspace")
     m = L.GatedMlpArgs(x=16, wg=16, wu=16, wd=16, y=16, ws=16, M=4, N=8, F=16, dtype=0, act=1)
     refused(lib.nsa_gated_mlp(C.byref(m), None), ARG, "workspace")
-    m.g = 16
-    refused(lib.nsa_gated_mlp(C.byref(m), None), ARG, "both g and u")
+    m.p = 16
+    refused(lib.nsa_gated_mlp(C.byref(m), None), ARG, "p, s and h")
     m.dtype = 4
     refused(lib.nsa_gated_mlp(C.byref(m), None), UNSUPPORTED, "dtype")
 
