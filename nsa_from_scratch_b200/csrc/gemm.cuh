@@ -48,27 +48,27 @@ template <int ACT> __device__ __forceinline__ void act_one_both(float z, float& 
     d = 1.f;
   }
 }
-// Eight at a time: the choice is made once, so that the eight chains of exp and division run side by side (chosen
-// element by element they ran one after the other: 111 against 84 us for the gated product of 8191 x 2816 x 1024).
-template <int ACT> __device__ __forceinline__ void act8_as(float (&a)[8]) {
+// Several at a time: the choice is made once, so that their chains of exp and division run side by side (chosen element by
+// element they ran one after the other: 111 against 93 us for the gated product of 8191 x 2816 x 1024).
+template <int ACT, int R> __device__ __forceinline__ void act_as(float (&a)[R]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) a[i] = act_one<ACT>(a[i]);
+  for (int i = 0; i < R; ++i) a[i] = act_one<ACT>(a[i]);
 }
-template <int ACT> __device__ __forceinline__ void act8_both_as(float (&a)[8], float (&d)[8]) {
+template <int ACT, int R> __device__ __forceinline__ void act_both_as(float (&a)[R], float (&d)[R]) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) act_one_both<ACT>(a[i], a[i], d[i]);
+  for (int i = 0; i < R; ++i) act_one_both<ACT>(a[i], a[i], d[i]);
 }
-__device__ __forceinline__ void act8(float (&a)[8], int act) {
-  if (act == ACT_SILU) act8_as<ACT_SILU>(a);
-  else if (act == ACT_GELU_TANH) act8_as<ACT_GELU_TANH>(a);
-  else if (act == ACT_RELU) act8_as<ACT_RELU>(a);
+template <int R> __device__ __forceinline__ void act_all(float (&a)[R], int act) {
+  if (act == ACT_SILU) act_as<ACT_SILU>(a);
+  else if (act == ACT_GELU_TANH) act_as<ACT_GELU_TANH>(a);
+  else if (act == ACT_RELU) act_as<ACT_RELU>(a);
 }
 // a = act(a), d = act'(a)
-__device__ __forceinline__ void act8_both(float (&a)[8], float (&d)[8], int act) {
-  if (act == ACT_SILU) act8_both_as<ACT_SILU>(a, d);
-  else if (act == ACT_GELU_TANH) act8_both_as<ACT_GELU_TANH>(a, d);
-  else if (act == ACT_RELU) act8_both_as<ACT_RELU>(a, d);
-  else act8_both_as<ACT_NONE>(a, d);
+template <int R> __device__ __forceinline__ void act_all_both(float (&a)[R], float (&d)[R], int act) {
+  if (act == ACT_SILU) act_both_as<ACT_SILU>(a, d);
+  else if (act == ACT_GELU_TANH) act_both_as<ACT_GELU_TANH>(a, d);
+  else if (act == ACT_RELU) act_both_as<ACT_RELU>(a, d);
+  else act_both_as<ACT_NONE>(a, d);
 }
 
 struct Epi {
@@ -120,99 +120,59 @@ __device__ __forceinline__ void store8(void* p, long long i, int n, int vec, con
   }
 }
 
-// Columns col..col+7 (those below N) of row `row`.  Everything is formed in fp32 and rounded once where it is stored.
-// What the epilogue reads is fetched apart from its use, so that the loads can be sent ahead of the sums.
-template <typename T, int MODE> struct Epilogue {
-  struct Col { float bias[8], ws[8]; };            // of the columns
-  struct Row { uint4 a, b; float xs; };            // of the row: residual, or i0 and i1, where they are read 16 bytes at a time
-
-  static __device__ __forceinline__ void load_col(const Epi& e, int col, Col& c) {
-    if constexpr (MODE == EPI_LINEAR) {
-      const int n = e.N - col;
-      if (n <= 0) return;
-      if (e.bias != nullptr) load8<T>(e.bias, col, n, e.vec, c.bias);
-      if (e.xs != nullptr) {
+// Columns col..col+7 (those below N) of row `row`: a = fp32 sums, b = the second product's (EPI_GLU).  Everything is
+// formed in fp32 and rounded once where it is stored.
+template <typename T, int MODE>
+__device__ __forceinline__ void epilogue8(const Epi& e, long long row, int col, float (&a)[8], const float (&b)[8]) {
+  const int n = e.N - col;
+  if (row >= e.M || n <= 0) return;
+  const long long at = row * e.N + col, ay = row * e.ldy + col;
+  float v[8];
+  if constexpr (MODE == EPI_LINEAR) {
+    if (e.xs != nullptr) {
+      const float s = e.xs[row];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) c.ws[i] = i < n ? e.ws[col + i] : 0.f;
-      }
+      for (int i = 0; i < 8; ++i) a[i] *= i < n ? s * e.ws[col + i] : 0.f;
     }
-  }
-  static __device__ __forceinline__ void load_row(const Epi& e, long long row, int col, Row& r) {
-    if (row >= e.M || col >= e.N) return;
-    if constexpr (MODE == EPI_LINEAR) {
-      if (e.xs != nullptr) r.xs = e.xs[row];
-      if (e.residual != nullptr && e.vec) r.a = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(e.residual) + row * e.N + col);
-    } else if constexpr (MODE == EPI_GLU_BWD) {
-      if (e.vecy) {
-        r.a = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(e.i0) + row * e.ldy + col);
-        r.b = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(e.i1) + row * e.ldy + col);
-      }
+    if (e.bias != nullptr) {
+      load8<T>(e.bias, col, n, e.vec, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] += v[i];
     }
-  }
-  static __device__ __forceinline__ void unpack(const uint4& u, float (&v)[8]) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { const float2 f = Elem<T>::unpack(w[i]); v[2 * i] = f.x; v[2 * i + 1] = f.y; }
-  }
-  // a: the sums, b: the second product's (EPI_GLU)
-  static __device__ __forceinline__ void run(const Epi& e, long long row, int col, const Col& c, const Row& r, float (&a)[8], const float (&b)[8]) {
-    const int n = e.N - col;
-    if (row >= e.M || n <= 0) return;
-    const long long at = row * e.N + col, ay = row * e.ldy + col;
-    if constexpr (MODE == EPI_LINEAR) {
-      if (e.xs != nullptr) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a[i] *= r.xs * c.ws[i];
-      }
-      if (e.bias != nullptr) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a[i] += c.bias[i];
-      }
-      if (e.o1 != nullptr) {
-        float d[8];
-        act8_both(a, d, e.act);
-        store8<T>(e.o1, at, n, e.vec, d);
-      } else {
-        act8(a, e.act);
-      }
-      if (e.residual != nullptr) {
-        float q[8];
-        if (e.vec) unpack(r.a, q);
-        else load8<T>(e.residual, at, n, 0, q);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) a[i] += q[i];
-      }
-      store8<T>(e.y, ay, n, e.vecy, a);
-    } else if constexpr (MODE == EPI_GLU) {
-      if (e.o1 != nullptr) {
-        float d[8];
-        act8_both(a, d, e.act);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) d[i] *= b[i];
-        store8<T>(e.o1, ay, n, e.vecy, a);
-        store8<T>(e.o2, ay, n, e.vecy, d);
-      } else {
-        act8(a, e.act);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) a[i] *= b[i];
-      store8<T>(e.y, ay, n, e.vecy, a);
+    if (e.o1 != nullptr) {
+      act_all_both(a, v, e.act);
+      store8<T>(e.o1, at, n, e.vec, v);
     } else {
-      float p[8], s[8];
-      if (e.vecy) {
-        unpack(r.a, p);
-        unpack(r.b, s);
-      } else {
-        load8<T>(e.i0, ay, n, 0, p);
-        load8<T>(e.i1, ay, n, 0, s);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) { p[i] *= a[i]; s[i] *= a[i]; }
-      store8<T>(e.y, ay, n, e.vecy, s);
-      store8<T>(e.o1, ay, n, e.vecy, p);
+      act_all(a, e.act);
     }
+    if (e.residual != nullptr) {
+      load8<T>(e.residual, at, n, e.vec, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) a[i] += v[i];
+    }
+  } else if constexpr (MODE == EPI_GLU) {
+    if (e.o1 != nullptr) {
+      act_all_both(a, v, e.act);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] *= b[i];
+      store8<T>(e.o1, ay, n, e.vecy, a);
+      store8<T>(e.o2, ay, n, e.vecy, v);
+    } else {
+      act_all(a, e.act);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] *= b[i];
+  } else {
+    load8<T>(e.i0, ay, n, e.vecy, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] *= a[i];
+    store8<T>(e.o1, ay, n, e.vecy, v);
+    load8<T>(e.i1, ay, n, e.vecy, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] *= v[i];
   }
-};
+  store8<T>(e.y, ay, n, e.vecy, a);
+}
 
 static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 

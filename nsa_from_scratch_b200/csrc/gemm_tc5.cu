@@ -1,8 +1,11 @@
 // Matrix product on the 5th-generation tensor cores; operand rows start on 16-byte boundaries (linear.cu pads others).
 //
 // Persistent and warp-specialised: warp 0 brings operand tiles with TMA (128-byte swizzle, zeros outside), warp 1 issues
-// tcgen05.mma, warps 4-11 take the finished sums from TMEM through shared memory to the epilogue.  The sums are double
-// buffered in TMEM, so a tile's epilogue runs under the next tile's products.
+// tcgen05.mma, warps 4-11 take the finished sums from TMEM, a thread to a row, and run the epilogue.  The sums are double
+// buffered in TMEM, so a tile's epilogue runs under the next tile's products.  What the epilogue reads (residual, stored
+// factors) and writes passes through shared memory by TMA, whole boxes at a time, read and overwritten in place: with loads
+// and stores of its own and their bounds and alignment cases in the loop, a step of 32 x 32 results took 2000 clk, most of
+// it fetching instructions.  Results whose rows are not 16-byte aligned leave as fp32 sums for gemm_join_kernel.
 //
 //   CG = 2: a pair of CTAs computes 256 x 256 results; each brings 128 rows of A and half of B's 256 rows, and the pair's
 //           tensor cores read both halves.  Per CTA and 64-deep step that is 32 KB from L2 for 256 x 128 x 64 products a
@@ -35,8 +38,22 @@ __device__ __forceinline__ uint32_t map_to_rank(uint32_t addr, uint32_t rank) {
 __device__ __forceinline__ void cluster_sync() {
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;\n" ::: "memory");
 }
+// relaxed: what it announces is that TMEM was read, which the tcgen05 fences order
 __device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_addr) : "memory");
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];\n" ::"r"(cluster_addr) : "memory");
+}
+// shared memory -> global, tracked by the issuing thread's bulk groups; what lies outside the tensor is not written
+__device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
+  asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];\n" ::"l"(map), "r"(src), "r"(c0), "r"(c1) : "memory");
+}
+__device__ __forceinline__ void group_sync(int id) { asm volatile("bar.sync %0, 128;\n" ::"r"(id) : "memory"); }
+__device__ __forceinline__ uint4 lds128(uint32_t a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];\n" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ void sts128(uint32_t a, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 // `bar` is a shared::cluster address: with CG = 2 the pair's first CTA counts the bytes of both
 template <int CG>
@@ -77,23 +94,46 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
 #undef NSA_MMA
 }
 
+// ---------------------------------------------------------------- 16 columns of a row
+template <typename T> __device__ __forceinline__ void put16(uint32_t p0, uint32_t p1, const float (&a)[16]) {
+  sts128(p0, make_uint4(Elem<T>::pack(a[0], a[1]), Elem<T>::pack(a[2], a[3]), Elem<T>::pack(a[4], a[5]), Elem<T>::pack(a[6], a[7])));
+  sts128(p1, make_uint4(Elem<T>::pack(a[8], a[9]), Elem<T>::pack(a[10], a[11]), Elem<T>::pack(a[12], a[13]), Elem<T>::pack(a[14], a[15])));
+}
+template <typename T> __device__ __forceinline__ void get16(uint32_t p0, uint32_t p1, float (&a)[16]) {
+  const uint4 u[2] = {lds128(p0), lds128(p1)};
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { const float2 f = Elem<T>::unpack(w[j]); a[8 * i + 2 * j] = f.x; a[8 * i + 2 * j + 1] = f.y; }
+  }
+}
+template <typename T> __device__ __forceinline__ void add8(float* a, const uint4& u) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) { const float2 f = Elem<T>::unpack(w[j]); a[2 * j] += f.x; a[2 * j + 1] += f.y; }
+}
+
 // ---------------------------------------------------------------- kernel
 struct GemmTcParams {
   CUtensorMap tmA[2], tmB[2];
+  CUtensorMap tmY, tmO1, tmO2, tmI0, tmI1;      // results and inputs of the epilogue (I0: residual in EPI_LINEAR)
   Epi e;
-  float* part;              // PARTIAL: [splits][products][M][N] fp32
-  int M, N;
+  float* part;              // PARTIAL: [splits][products][M][ldp] fp32
+  int M, N, ldp;
   int tiles_m, tiles_n;
   int ksteps, segments;     // 128-byte steps of one segment
   int splits, per_split;    // the steps of all segments, dealt out to `splits` tiles
 };
 
-constexpr int EPI_PARTIAL = 3, EPI_PARTIAL2 = 4;       // raw sums of one product / of a gated pair, for the joining kernel
+// EPI_SLOPE: EPI_LINEAR that also writes act' (e.o1).  EPI_PARTIAL, EPI_PARTIAL2: raw sums of one product, of a gated pair,
+// for the joining kernel.
+constexpr int EPI_SLOPE = 3, EPI_PARTIAL = 4, EPI_PARTIAL2 = 5;
 
 template <int CG, int BN> struct TcShape {
   static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / CG * 128;
-  static constexpr int STAGES = 196608 / (A_BYTES + B_BYTES) > 6 ? 6 : 196608 / (A_BYTES + B_BYTES);
-  static constexpr int SMEM = STAGES * (A_BYTES + B_BYTES) + 8 * 4096 + 1024;
+  static constexpr int STAGES = 5, EPI_BYTES = 32768;             // EPI_BYTES: of each of the two epilogue groups
+  static constexpr int SMEM = STAGES * (A_BYTES + B_BYTES) + 2 * EPI_BYTES + 1024;
 };
 
 // F: 0 fp16, 1 bf16, 2 e4m3, 3 e5m2;  T: result type
@@ -111,8 +151,7 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   const uint32_t s_tiles = smem_u32(smem);
-  float* stage_f = reinterpret_cast<float*>(smem + S::STAGES * (S::A_BYTES + S::B_BYTES));
-  __shared__ __align__(8) uint64_t full[S::STAGES], empty[S::STAGES], tfull[2], tempty[2];
+  __shared__ __align__(8) uint64_t full[S::STAGES], empty[S::STAGES], tfull[2], tempty[2], loaded[2][2];
   __shared__ uint32_t tmem_s;
   __shared__ int abort_flag;
 
@@ -126,6 +165,7 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
     abort_flag = 0;
     for (int i = 0; i < S::STAGES; ++i) { mbar_init(smem_u32(&full[i]), 1); mbar_init(smem_u32(&empty[i]), 1); }
     for (int i = 0; i < 2; ++i) { mbar_init(smem_u32(&tfull[i]), 1); mbar_init(smem_u32(&tempty[i]), 8 * CG); }
+    for (int i = 0; i < 4; ++i) mbar_init(smem_u32(&loaded[i >> 1][i & 1]), 1);
     fence_barrier_init();
   }
   if (warp == 2) tm_alloc<CG>(smem_u32(&tmem_s), 2 * BN);
@@ -135,6 +175,8 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
   tc_fence_after();
   const uint32_t tmem = tmem_s;
   int fail_id = 0;
+  grid_dep_launch();                                                     // the next product's CTAs may set themselves up as these leave
+  grid_dep_wait();
 
   // tile t: which split of the contraction, which rows and columns (8 tile rows walk the columns together: their B tiles meet in L2)
   auto place = [&](int t, int& m0, int& n0, int& k0, int& k1, int& split) {
@@ -227,105 +269,181 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
     }
   } else if (warp >= 4) {
     // =============================== epilogue ===============================
-    // A warp owns 32 TMEM lanes (rows) and half of the columns.  32 x 32 sums pass through its 4 KB of shared memory, 16-byte
-    // pieces swizzled by row: written by row (a lane's 32 columns), read as 8 columns of 4 lanes to a row, so that
-    // global memory sees runs of 64 bytes.
-    const int quarter = warp & 3, half = (warp - 4) >> 2;
-    float* st = stage_f + (warp - 4) * 1024;
+    // Two groups of four warps, each with half of the tile's columns; a thread owns a row (a TMEM lane).  A group works in
+    // chunks of CW columns, 16 columns of sums at a time.  Its 32 KB of shared memory hold, per chunk and stage, a box of
+    // 128 rows of each tensor that is read or written; inputs are requested a chunk or two ahead, results overwrite them.
+    // A wait that gave up ends the work but not the barriers that the group's warps share.
+    const int quarter = warp & 3, group = (warp - 4) >> 2;
+    const int row = quarter * 32 + lane;
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
-    constexpr int STEP = PAIR ? 16 : 32;                                 // result columns a step
-    constexpr int STEPS = NW / 2 / STEP;
-    constexpr int PASSES = PAIR ? 2 : 4, LPR = PAIR ? 2 : 4;             // a pass: LPR lanes of 8 columns to a row
+    const bool lead = quarter == 0 && lane == 0;
     constexpr bool RAW = MODE == EPI_PARTIAL || MODE == EPI_PARTIAL2;
-    using E = Epilogue<T, RAW ? EPI_LINEAR : MODE>;
-    const int my_row = lane / LPR, my_col = (lane % LPR) * 8;
-    int n = 0;
+    constexpr int GW = NW / 2;                                           // columns of the group
+    constexpr int CW = MODE == EPI_LINEAR ? 64 : 32;                     // columns of a chunk
+    constexpr int NC = RAW ? 1 : GW / CW;
+    constexpr int BOX = 128 * CW * 2;                                    // bytes of a box: 128 rows of CW columns
+    constexpr int STAGE = MODE == EPI_GLU ? 0 : 16384;                   // between the two stages (EPI_GLU: one stage of three boxes)
+    const uint32_t stage0 = s_tiles + S::STAGES * (S::A_BYTES + S::B_BYTES) + group * S::EPI_BYTES;
+    constexpr bool LIN = MODE == EPI_LINEAR || MODE == EPI_SLOPE;
+    const bool inputs = MODE == EPI_GLU_BWD || (LIN && p.e.residual != nullptr);
+    // 16-byte piece j of this thread's row in a box
+    auto piece = [&](uint32_t box, int j) { return CW == 64 ? box + row * 128 + ((j ^ (row & 7)) << 4) : box + row * 64 + ((j ^ ((row >> 1) & 3)) << 4); };
+    int n = 0, cnt = 0;                                                  // tiles and chunks so far
     bool ok = true;
-    for (int t = unit; t < tiles && ok; t += units, ++n) {
+    for (int t = unit; t < tiles; t += units, ++n) {
       int m0, n0, k0, k1, split;
       place(t, m0, n0, k0, k1, split);
       const int buf = n & 1;
-      const long long row0 = m0 + (int)rank * 128 + quarter * 32;
-      const int col0 = half * (NW / 2);
-      typename E::Row next[PASSES];
-      auto fetch = [&](int c) {                                          // what step c reads from global memory
-        if constexpr (!RAW) {
-#pragma unroll
-          for (int q = 0; q < PASSES; ++q) E::load_row(p.e, row0 + q * (32 / PASSES) + my_row, n0 + col0 + c * STEP + my_col, next[q]);
+      const int mr = m0 + (int)rank * 128, nc0 = n0 + group * GW;
+      auto request = [&](int c, int count) {                             // lead only: the inputs of chunk c of this tile
+        const int st = count & 1;
+        const uint32_t bar = smem_u32(&loaded[group][st]), box = stage0 + st * STAGE;
+        mbar_expect_tx(bar, MODE == EPI_GLU_BWD ? 2 * BOX : BOX);
+        tma_load_2d<1>(box, &p.tmI0, bar, nc0 + c * CW, mr);
+        if constexpr (MODE == EPI_GLU_BWD) tma_load_2d<1>(box + BOX, &p.tmI1, bar, nc0 + c * CW, mr);
+      };
+      if (inputs && lead) {
+        bulk_wait_read<0>();
+        request(0, cnt);
+        if (NC > 1) request(1, cnt + 1);
+      }
+      if (ok) ok = mbar_wait(smem_u32(&tfull[buf]), (n >> 1) & 1, &abort_flag);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) fail_id = 4;
+      tc_fence_after();
+      const uint32_t acc = tmem + lanes + buf * BN + group * GW;
+      const int grow = mr + row;
+      float xs = 1.f;
+      if constexpr (LIN) { if (p.e.xs != nullptr && grow < p.M) xs = p.e.xs[grow]; }
+      auto drained = [&] {                                               // the last sums are in registers: the buffer may be filled again
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (CG == 2) arrive_remote(map_to_rank(smem_u32(&tempty[buf]), 0));
+          else mbar_arrive(smem_u32(&tempty[buf]));
         }
       };
-      fetch(0);                                                          // lands while the tile is still being summed
-      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&tfull[buf]), (n >> 1) & 1, &abort_flag));
-      if (!ok) { fail_id = 4; break; }
-      tc_fence_after();
+      if constexpr (RAW) {
 #pragma unroll 1
-      for (int c = 0; c < STEPS; ++c) {
-        const int col = col0 + c * STEP;
-        typename E::Row now[PASSES];
-        typename E::Col cv;
+        for (int c = 0; c < GW; c += 16) {
 #pragma unroll
-        for (int q = 0; q < PASSES; ++q) now[q] = next[q];
-        if (c + 1 < STEPS) fetch(c + 1);
-        if constexpr (!RAW) E::load_col(p.e, n0 + col + my_col, cv);
-        uint32_t v[32];
-        if constexpr (PAIR) {
-          uint32_t g[16], u[16];
-          tmem_ld16(tmem + lanes + buf * BN + col, g);
-          tmem_ld16(tmem + lanes + buf * BN + NW + col, u);
-          tc_wait_ld();
+          for (int q = 0; q < (PAIR ? 2 : 1); ++q) {
+            uint32_t v[16];
+            tmem_ld16(acc + c + q * NW, v);
+            tc_wait_ld();
+            float* dst = p.part + (((long long)split * (PAIR ? 2 : 1) + q) * p.M + grow) * p.ldp + nc0 + c;
 #pragma unroll
-          for (int i = 0; i < 16; ++i) { v[i] = g[i]; v[16 + i] = u[i]; }
-        } else {
-          tmem_ld32(tmem + lanes + buf * BN + col, v);
-          tc_wait_ld();
-        }
-        if (c == STEPS - 1) {                                            // everything is in registers: the buffer may be filled again
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) {
-            if constexpr (CG == 2) arrive_remote(map_to_rank(smem_u32(&tempty[buf]), 0));
-            else mbar_arrive(smem_u32(&tempty[buf]));
+            for (int i = 0; i < 16; i += 4)
+              if (grow < p.M && nc0 + c + i < p.ldp) *reinterpret_cast<uint4*>(dst + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
           }
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-          *reinterpret_cast<uint4*>(st + lane * 32 + ((i ^ (lane & 7)) << 2)) = make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
-        __syncwarp();
-        auto get8 = [&](int r, int piece, float (&x)[8]) {
-          const float4 lo = *reinterpret_cast<const float4*>(st + r * 32 + ((piece ^ (r & 7)) << 2));
-          const float4 hi = *reinterpret_cast<const float4*>(st + r * 32 + (((piece + 1) ^ (r & 7)) << 2));
-          x[0] = lo.x; x[1] = lo.y; x[2] = lo.z; x[3] = lo.w; x[4] = hi.x; x[5] = hi.y; x[6] = hi.z; x[7] = hi.w;
-        };
-        auto put_raw = [&](long long row, int cc, int product, const float (&x)[8]) {
-          if (row >= p.M) return;
-          float* dst = p.part + (((long long)split * (PAIR ? 2 : 1) + product) * p.M + row) * p.N + cc;
-          if (p.N % 4 == 0 && cc + 8 <= p.N) {
-            reinterpret_cast<float4*>(dst)[0] = make_float4(x[0], x[1], x[2], x[3]);
-            reinterpret_cast<float4*>(dst)[1] = make_float4(x[4], x[5], x[6], x[7]);
+        drained();
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < NC; ++c, ++cnt) {
+          const int st = cnt & 1;
+          const uint32_t box = stage0 + st * STAGE;
+          if (inputs) {
+            if (ok) ok = mbar_wait(smem_u32(&loaded[group][st]), (cnt >> 1) & 1, &abort_flag);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) fail_id = 5;
           } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-              if (cc + i < p.N) dst[i] = x[i];
+            if (lead) { if constexpr (MODE == EPI_GLU) bulk_wait_read<0>(); else bulk_wait_read<1>(); }
+            group_sync(1 + group);                                       // the boxes that are about to be written have left
           }
-        };
+#pragma unroll 1
+          for (int h = 0; h < CW / 16; ++h) {
+            const int col = c * CW + h * 16;
+            float a[16];
+            {
+              uint32_t v[16];
+              tmem_ld16(acc + col, v);
+              if constexpr (MODE == EPI_GLU) {
+                uint32_t w[16];
+                tmem_ld16(acc + NW + col, w);
+                tc_wait_ld();
+                float d[16];
 #pragma unroll
-        for (int q = 0; q < PASSES; ++q) {
-          const int r = q * (32 / PASSES) + my_row, cc = n0 + col + my_col;
-          float a[8];
-          get8(r, my_col / 4, a);
-          if constexpr (PAIR) {
-            float b[8];
-            get8(r, 4 + my_col / 4, b);
-            if constexpr (RAW) { put_raw(row0 + r, cc, 0, a); put_raw(row0 + r, cc, 1, b); }
-            else E::run(p.e, row0 + r, cc, cv, now[q], a, b);
-          } else {
-            if constexpr (RAW) put_raw(row0 + r, cc, 0, a);
-            else E::run(p.e, row0 + r, cc, cv, now[q], a, a);
+                for (int i = 0; i < 16; ++i) a[i] = __uint_as_float(v[i]);
+                if (p.e.o1 != nullptr) {
+                  act_all_both(a, d, p.e.act);
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) d[i] *= __uint_as_float(w[i]);
+                  put16<T>(piece(box + BOX, 2 * h), piece(box + BOX, 2 * h + 1), a);
+                  put16<T>(piece(box + 2 * BOX, 2 * h), piece(box + 2 * BOX, 2 * h + 1), d);
+                } else {
+                  act_all(a, p.e.act);
+                }
+#pragma unroll
+                for (int i = 0; i < 16; ++i) a[i] *= __uint_as_float(w[i]);
+              } else {
+                tc_wait_ld();
+#pragma unroll
+                for (int i = 0; i < 16; ++i) a[i] = __uint_as_float(v[i]);
+              }
+            }
+            const uint32_t p0 = piece(box, 2 * h), p1 = piece(box, 2 * h + 1);
+            if constexpr (LIN) {
+              const int gc = nc0 + col;                                  // columns come in eights: N is a multiple of 8
+              if (p.e.xs != nullptr) {
+#pragma unroll
+                for (int i = 0; i < 16; i += 4)
+                  if (gc + i < p.N) {
+                    const float4 w = *reinterpret_cast<const float4*>(p.e.ws + gc + i);
+                    a[i] *= xs * w.x; a[i + 1] *= xs * w.y; a[i + 2] *= xs * w.z; a[i + 3] *= xs * w.w;
+                  }
+              }
+              if (p.e.bias != nullptr) {
+#pragma unroll
+                for (int i = 0; i < 16; i += 8)
+                  if (gc + i < p.N) add8<T>(a + i, *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.e.bias) + gc + i));
+              }
+              if constexpr (MODE == EPI_SLOPE) {
+                float d[16];
+                act_all_both(a, d, p.e.act);
+                put16<T>(piece(box + BOX, 2 * h), piece(box + BOX, 2 * h + 1), d);
+              } else {
+                act_all(a, p.e.act);
+              }
+              if (p.e.residual != nullptr) { add8<T>(a, lds128(p0)); add8<T>(a + 8, lds128(p1)); }
+            } else if constexpr (MODE == EPI_GLU_BWD) {
+              float d[16];
+              get16<T>(p0, p1, d);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) d[i] *= a[i];
+              put16<T>(p0, p1, d);                                       // du, over act(g)
+              get16<T>(piece(box + BOX, 2 * h), piece(box + BOX, 2 * h + 1), d);
+#pragma unroll
+              for (int i = 0; i < 16; ++i) a[i] *= d[i];
+              put16<T>(piece(box + BOX, 2 * h), piece(box + BOX, 2 * h + 1), a);      // dg, over act'(g) u
+            }
+            if constexpr (MODE != EPI_GLU_BWD) put16<T>(p0, p1, a);
+          }
+          if (c == NC - 1) drained();
+          fence_proxy_async();
+          group_sync(1 + group);
+          if (lead && ok) {
+            const int gc = nc0 + c * CW;
+            if constexpr (MODE == EPI_GLU_BWD) {
+              tma_store_2d(&p.tmO1, box, gc, mr);
+              tma_store_2d(&p.tmY, box + BOX, gc, mr);
+            } else {
+              tma_store_2d(&p.tmY, box, gc, mr);
+              if constexpr (MODE == EPI_SLOPE) tma_store_2d(&p.tmO1, box + BOX, gc, mr);
+              if constexpr (MODE == EPI_GLU) {
+                if (p.e.o1 != nullptr) { tma_store_2d(&p.tmO1, box + BOX, gc, mr); tma_store_2d(&p.tmO2, box + 2 * BOX, gc, mr); }
+              }
+            }
+            bulk_commit();
+            if (inputs && c + 2 < NC) {
+              bulk_wait_read<0>();                                       // the request overwrites what was just sent
+              request(c + 2, cnt + 2);
+            }
           }
         }
-        __syncwarp();
       }
     }
+    if (lead) bulk_wait_read<0>();                                       // shared memory has been read; the kernel's end sees to the rest
   }
 
   if (fail_id != 0) atomicCAS(&g_gemm_status, 0, fail_id);
@@ -339,37 +457,26 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
 
 // Joins the partial sums of a split contraction, in split order, and runs the epilogue: 8 columns a thread.
 template <typename T, int MODE>
-__global__ void __launch_bounds__(256) gemm_join_kernel(const float* __restrict__ part, const Epi e, int splits) {
+__global__ void __launch_bounds__(256) gemm_join_kernel(const float* __restrict__ part, const Epi e, int splits, int ldp) {
   constexpr int PR = MODE == EPI_GLU ? 2 : 1;
-  const int groups = (e.N + 7) / 8;
+  const int groups = ldp / 8;
   const long long total = (long long)e.M * groups;
-  const long long mn = (long long)e.M * e.N;
+  const long long mn = (long long)e.M * ldp;
   grid_dep_wait();
   for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)gridDim.x * 256) {
     const long long row = i / groups;
     const int col = (int)(i % groups) * 8;
-    using E = Epilogue<T, MODE>;
-    typename E::Col cv;
-    typename E::Row rv;
-    E::load_col(e, col, cv);
-    E::load_row(e, row, col, rv);
     float a[PR][8] = {};
     for (int s = 0; s < splits; ++s) {
 #pragma unroll
       for (int q = 0; q < PR; ++q) {
-        const float* src = part + (s * PR + q) * mn + row * e.N + col;
-        if (e.N % 8 == 0) {
-          const float4 lo = reinterpret_cast<const float4*>(src)[0], hi = reinterpret_cast<const float4*>(src)[1];
-          a[q][0] += lo.x; a[q][1] += lo.y; a[q][2] += lo.z; a[q][3] += lo.w;
-          a[q][4] += hi.x; a[q][5] += hi.y; a[q][6] += hi.z; a[q][7] += hi.w;
-        } else {
-#pragma unroll
-          for (int c = 0; c < 8; ++c)
-            if (col + c < e.N) a[q][c] += src[c];
-        }
+        const float4* src = reinterpret_cast<const float4*>(part + (s * PR + q) * mn + row * ldp + col);
+        const float4 lo = src[0], hi = src[1];
+        a[q][0] += lo.x; a[q][1] += lo.y; a[q][2] += lo.z; a[q][3] += lo.w;
+        a[q][4] += hi.x; a[q][5] += hi.y; a[q][6] += hi.z; a[q][7] += hi.w;
       }
     }
-    E::run(e, row, col, cv, rv, a[0], a[PR - 1]);
+    epilogue8<T, MODE>(e, row, col, a[0], a[PR - 1]);
   }
 }
 
@@ -384,17 +491,19 @@ static PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder() {
   return fn;
 }
 
-// [rows][cols] matrix with `ld` elements between rows; boxes of 128 bytes x `box_rows`, 128-byte swizzle, zeros outside
-static int map_2d(CUtensorMap* m, const void* ptr, long long rows, long long cols, long long ld, int box_rows, int dtype) {
+// [rows][cols] matrix with `ld` elements between rows; boxes of box_cols x box_rows with the swizzle of their 64 or 128
+// bytes; zeros outside
+static int map_2d(CUtensorMap* m, const void* ptr, long long rows, long long cols, long long ld, int box_cols, int box_rows, int dtype) {
   auto enc = tensor_map_encoder();
   NSA_REQUIRE(enc != nullptr, NSA_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
   const int size = dtype == NSA_BF16 || dtype == NSA_FP16 ? 2 : 1;
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)ld * size};
-  cuuint32_t box[2] = {(cuuint32_t)(128 / size), (cuuint32_t)box_rows};
+  cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
   cuuint32_t es[2] = {1, 1};
+  const CUtensorMapSwizzle swizzle = box_cols * size == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   const CUtensorMapDataType dt = dtype == NSA_FP16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : dtype == NSA_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
-  auto encode = [&] { return enc(m, dt, 2, const_cast<void*>(ptr), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+  auto encode = [&] { return enc(m, dt, 2, const_cast<void*>(ptr), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE); };
   CUresult r = encode();
   if (r == CUDA_ERROR_INVALID_CONTEXT) {     // a thread that has not used the runtime yet (autograd's): bind the device's context to it
@@ -409,8 +518,11 @@ static int map_2d(CUtensorMap* m, const void* ptr, long long rows, long long col
 
 static int esize(int dtype) { return dtype == NSA_BF16 || dtype == NSA_FP16 ? 2 : 1; }
 
-// Which kernel and how many ways the contraction is split.
-struct TcPlan { int cg, bn, tiles_m, tiles_n, ksteps, splits, per_split; };
+static int pitch(int N) { return (N + 7) / 8 * 8; }                     // of partial sums
+
+// Which kernel, how many ways the contraction is split, and whether the sums leave raw: where they are split, or where
+// the results' rows do not start on 16-byte boundaries (TMA writes them).
+struct TcPlan { int cg, bn, tiles_m, tiles_n, ksteps, splits, per_split; bool raw; };
 static TcPlan tc_plan(const GemmProblem& p) {
   TcPlan t;
   const int sms = sm_count();
@@ -435,12 +547,13 @@ static TcPlan tc_plan(const GemmProblem& p) {
   }
   t.per_split = (steps + t.splits - 1) / t.splits;
   t.splits = (steps + t.per_split - 1) / t.per_split;
+  t.raw = t.splits > 1 || !p.e.vec || !p.e.vecy;
   return t;
 }
 
 long long gemm_tc5_ws_bytes(const GemmProblem& p) {
   const TcPlan t = tc_plan(p);
-  return t.splits == 1 ? 0 : (long long)t.splits * (p.e.mode == EPI_GLU ? 2 : 1) * p.M * p.N * 4;
+  return t.raw ? (long long)t.splits * (p.e.mode == EPI_GLU ? 2 : 1) * p.M * pitch(p.N) * 4 : 0;
 }
 
 template <int F, typename T, bool A_MN, bool B_MN, int MODE, int CG, int BN>
@@ -460,11 +573,13 @@ static int tc_launch(const GemmTcParams& g, long long tiles, cudaStream_t st) {
   cfg.blockDim = dim3(384);
   cfg.dynamicSmemBytes = S::SMEM;
   cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = CG; at[0].val.clusterDim.y = 1; at[0].val.clusterDim.z = 1;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = CG; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
-  cfg.numAttrs = CG == 2 ? 1 : 0;
+  cfg.numAttrs = CG;
   const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, g);
   if (e != cudaSuccess) return fail(NSA_ERR_CUDA, "gemm_tc5 launch failed: %s", cudaGetErrorString(e));
   return NSA_OK;
@@ -479,15 +594,18 @@ static int tc_shape(const GemmTcParams& g, const TcPlan& t, cudaStream_t st) {
 
 template <int F, typename T>
 static int tc_mode(const GemmTcParams& g, const TcPlan& t, const GemmProblem& p, cudaStream_t st) {
-  const bool split = t.splits > 1;
   if constexpr (F >= 2) {
-    return split ? tc_shape<F, T, false, false, EPI_PARTIAL>(g, t, st) : tc_shape<F, T, false, false, EPI_LINEAR>(g, t, st);
+    return t.raw ? tc_shape<F, T, false, false, EPI_PARTIAL>(g, t, st) : tc_shape<F, T, false, false, EPI_LINEAR>(g, t, st);
   } else {
-    if (p.e.mode == EPI_GLU) return split ? tc_shape<F, T, false, false, EPI_PARTIAL2>(g, t, st) : tc_shape<F, T, false, false, EPI_GLU>(g, t, st);
-    if (p.e.mode == EPI_GLU_BWD) return split ? tc_shape<F, T, false, true, EPI_PARTIAL>(g, t, st) : tc_shape<F, T, false, true, EPI_GLU_BWD>(g, t, st);
-    if (p.a_mn) return split ? tc_shape<F, T, true, true, EPI_PARTIAL>(g, t, st) : tc_shape<F, T, true, true, EPI_LINEAR>(g, t, st);
-    if (p.b_mn) return split ? tc_shape<F, T, false, true, EPI_PARTIAL>(g, t, st) : tc_shape<F, T, false, true, EPI_LINEAR>(g, t, st);
-    return split ? tc_shape<F, T, false, false, EPI_PARTIAL>(g, t, st) : tc_shape<F, T, false, false, EPI_LINEAR>(g, t, st);
+    if (p.e.mode == EPI_GLU) return t.raw ? tc_shape<F, T, false, false, EPI_PARTIAL2>(g, t, st) : tc_shape<F, T, false, false, EPI_GLU>(g, t, st);
+    if (t.raw) {
+      if (p.a_mn) return tc_shape<F, T, true, true, EPI_PARTIAL>(g, t, st);
+      return p.b_mn ? tc_shape<F, T, false, true, EPI_PARTIAL>(g, t, st) : tc_shape<F, T, false, false, EPI_PARTIAL>(g, t, st);
+    }
+    if (p.e.mode == EPI_GLU_BWD) return tc_shape<F, T, false, true, EPI_GLU_BWD>(g, t, st);
+    if (p.a_mn) return tc_shape<F, T, true, true, EPI_LINEAR>(g, t, st);
+    if (p.b_mn) return tc_shape<F, T, false, true, EPI_LINEAR>(g, t, st);
+    return p.e.o1 != nullptr ? tc_shape<F, T, false, false, EPI_SLOPE>(g, t, st) : tc_shape<F, T, false, false, EPI_LINEAR>(g, t, st);
   }
 }
 
@@ -495,9 +613,9 @@ template <typename T>
 static int join(const float* part, const GemmProblem& p, int splits, cudaStream_t st) {
   const long long want = ((long long)p.M * ((p.N + 7) / 8) + 255) / 256, cap = 8LL * sm_count();
   const dim3 grid((unsigned)(want < cap ? want : cap));
-  if (p.e.mode == EPI_GLU) return launch_pdl("gemm_join", gemm_join_kernel<T, EPI_GLU>, grid, 256, 0, st, part, p.e, splits);
-  if (p.e.mode == EPI_GLU_BWD) return launch_pdl("gemm_join", gemm_join_kernel<T, EPI_GLU_BWD>, grid, 256, 0, st, part, p.e, splits);
-  return launch_pdl("gemm_join", gemm_join_kernel<T, EPI_LINEAR>, grid, 256, 0, st, part, p.e, splits);
+  if (p.e.mode == EPI_GLU) return launch_pdl("gemm_join", gemm_join_kernel<T, EPI_GLU>, grid, 256, 0, st, part, p.e, splits, pitch(p.N));
+  if (p.e.mode == EPI_GLU_BWD) return launch_pdl("gemm_join", gemm_join_kernel<T, EPI_GLU_BWD>, grid, 256, 0, st, part, p.e, splits, pitch(p.N));
+  return launch_pdl("gemm_join", gemm_join_kernel<T, EPI_LINEAR>, grid, 256, 0, st, part, p.e, splits, pitch(p.N));
 }
 
 int gemm_tc5(const GemmProblem& p, void* ws, cudaStream_t st) {
@@ -509,15 +627,25 @@ int gemm_tc5(const GemmProblem& p, void* ws, cudaStream_t st) {
   const int pair = p.e.mode == EPI_GLU;
   const int brows = pair ? t.bn / 2 : t.bn / t.cg;                     // rows of a box of B
   for (int i = 0; i < p.segments; ++i) {
-    rc = p.a_mn ? map_2d(&g.tmA[i], p.A[i], p.K, p.M, p.lda, ke, p.dtype) : map_2d(&g.tmA[i], p.A[i], p.M, p.K, p.lda, 128, p.dtype);
+    rc = p.a_mn ? map_2d(&g.tmA[i], p.A[i], p.K, p.M, p.lda, ke, ke, p.dtype) : map_2d(&g.tmA[i], p.A[i], p.M, p.K, p.lda, ke, 128, p.dtype);
     if (rc != NSA_OK) return rc;
-    rc = p.b_mn ? map_2d(&g.tmB[i], p.B[i], p.K, p.N, p.ldb, ke, p.dtype) : map_2d(&g.tmB[i], p.B[i], p.N, p.K, p.ldb, brows, p.dtype);
+    rc = p.b_mn ? map_2d(&g.tmB[i], p.B[i], p.K, p.N, p.ldb, ke, ke, p.dtype) : map_2d(&g.tmB[i], p.B[i], p.N, p.K, p.ldb, ke, brows, p.dtype);
     if (rc != NSA_OK) return rc;
   }
-  if (pair && (rc = map_2d(&g.tmB[1], p.B[1], p.N, p.K, p.ldb, brows, p.dtype)) != NSA_OK) return rc;
+  if (pair && (rc = map_2d(&g.tmB[1], p.B[1], p.N, p.K, p.ldb, ke, brows, p.dtype)) != NSA_OK) return rc;
+  if (!t.raw) {
+    const bool gated = p.e.mode != EPI_LINEAR;
+    const int cw = gated || p.e.o1 != nullptr ? 32 : 64;
+    auto box = [&](CUtensorMap* m, const void* ptr, long long ld) { return ptr == nullptr ? NSA_OK : map_2d(m, ptr, p.M, p.N, ld, cw, 128, p.out_dtype); };
+    if ((rc = box(&g.tmY, p.e.y, p.e.ldy)) != NSA_OK) return rc;
+    if ((rc = box(&g.tmO1, p.e.o1, gated ? p.e.ldy : p.N)) != NSA_OK) return rc;
+    if ((rc = box(&g.tmO2, p.e.o2, p.e.ldy)) != NSA_OK) return rc;
+    if ((rc = box(&g.tmI0, gated ? p.e.i0 : p.e.residual, gated ? p.e.ldy : p.N)) != NSA_OK) return rc;
+    if ((rc = box(&g.tmI1, p.e.i1, p.e.ldy)) != NSA_OK) return rc;
+  }
   g.e = p.e;
   g.part = reinterpret_cast<float*>(ws);
-  g.M = p.M; g.N = p.N;
+  g.M = p.M; g.N = p.N; g.ldp = pitch(p.N);
   g.tiles_m = t.tiles_m; g.tiles_n = t.tiles_n;
   g.ksteps = t.ksteps; g.segments = p.segments;
   g.splits = t.splits; g.per_split = t.per_split;
@@ -526,7 +654,7 @@ int gemm_tc5(const GemmProblem& p, void* ws, cudaStream_t st) {
   else if (p.dtype == NSA_FP16) rc = tc_mode<0, __half>(g, t, p, st);
   else if (p.dtype == NSA_FP8_E4M3) rc = bf ? tc_mode<2, __nv_bfloat16>(g, t, p, st) : tc_mode<2, __half>(g, t, p, st);
   else rc = bf ? tc_mode<3, __nv_bfloat16>(g, t, p, st) : tc_mode<3, __half>(g, t, p, st);
-  if (rc != NSA_OK || t.splits == 1) return rc;
+  if (rc != NSA_OK || !t.raw) return rc;
   return bf ? join<__nv_bfloat16>(g.part, p, t.splits, st) : join<__half>(g.part, p, t.splits, st);
 }
 

@@ -198,7 +198,7 @@ static int linear_steps(const nsa_linear_args& a, Arena& w) {
   p.e.act = a.act;
   p.e.bias = a.bias; p.e.residual = a.residual; p.e.xs = a.x_scale; p.e.ws = a.w_scale;
   p.e.y = a.y; p.e.o1 = a.slope;
-  p.e.vec = a.N % 8 == 0 && aligned16(a.bias) && aligned16(a.residual) && aligned16(a.slope);
+  p.e.vec = a.N % 8 == 0 && aligned16(a.bias) && aligned16(a.residual) && aligned16(a.slope) && aligned16(a.w_scale);
   p.e.vecy = a.N % 8 == 0 && aligned16(a.y);
   return gemm(w, p);
 }
@@ -273,7 +273,7 @@ static int mlp_steps(const nsa_gated_mlp_args& a, Arena& w) {
   p.e.mode = EPI_GLU;
   p.e.act = a.act;
   p.e.y = h; p.e.o1 = a.p; p.e.o2 = a.s;
-  p.e.ldy = ldh; p.e.vecy = 1;
+  p.e.ldy = ldh; p.e.vec = p.e.vecy = 1;
   NSA_TRY(gemm(w, p));
   NSA_TRY(operand(w, a.wd, a.N, a.F, a.dtype, &wd));
   GemmProblem d = problem(Mat{h, ldh}, 0, wd, 0, a.M, a.N, a.F, a.dtype);
@@ -305,7 +305,7 @@ static int mlp_bwd_steps(const nsa_gated_mlp_bwd_args& a, Arena& w) {
   p.e.mode = EPI_GLU_BWD;
   p.e.i0 = a.p; p.e.i1 = a.s;
   p.e.y = dg; p.e.o1 = du;
-  p.e.ldy = ldh; p.e.vecy = 1;
+  p.e.ldy = ldh; p.e.vec = p.e.vecy = 1;
   NSA_TRY(gemm(w, p));
   if (a.dx || !run) {                                                                       // dx = dg wg + du wu
     NSA_TRY(operand(w, a.wg, a.F, a.N, a.dtype, &wg));
