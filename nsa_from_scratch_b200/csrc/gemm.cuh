@@ -179,6 +179,8 @@ static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t
 int sm_count();                                                            // of the current device (linear.cu)
 long long gemm_tc5_ws_bytes(const GemmProblem& p);                       // gemm_tc5.cu
 int gemm_tc5(const GemmProblem& p, void* ws, cudaStream_t st);
+long long gemm_tc5_group_ws_bytes(const GemmProblem* p, int count);
+int gemm_tc5_group(const GemmProblem* p, int count, void* ws, cudaStream_t st);
 int column_sum(const float* part, void* out, int parts, int N, int dt, cudaStream_t st);   // norm.cu
 
 }  // namespace nsa

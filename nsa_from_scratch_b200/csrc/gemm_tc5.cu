@@ -8,9 +8,12 @@
 // it fetching instructions.  Results whose rows are not 16-byte aligned leave as fp32 sums for gemm_join_kernel.
 //
 //   CG = 2: a pair of CTAs computes 256 x 256 results; each brings 128 rows of A and half of B's 256 rows, and the pair's
-//           tensor cores read both halves.  Per CTA and 64-deep step that is 32 KB from L2 for 256 x 128 x 64 products a
-//           CTA; one CTA alone on 128 x 256 would need 48 KB, more than L2 delivers at the tensor cores' pace.
-//   CG = 1: one CTA computes 128 x 128 results: problems with few tiles.
+//           tensor cores read both halves: 32 KB a CTA and 64-deep step.  An SM receives 64 bytes a clk from L2, so that is
+//           512 clk, where the products take 405 (measured: 405 while the ring is full, 510 in the long run).
+//   CG = 1: one CTA computes 128 x 128 results: up to 128 rows.  The same 32 KB for half of the pair's share, so larger
+//           problems stay on pairs however few tiles that leaves.
+//
+// A launch takes up to four products of the same kind (a layer's gradients): their tiles share the SMs' rounds.
 //
 // EPI_GLU computes both products in one tile: the B rows of a tile are BN/2 rows of each weight, so that g and u of a
 // column stand BN/2 columns apart in the same TMEM lane.
@@ -115,15 +118,22 @@ template <typename T> __device__ __forceinline__ void add8(float* a, const uint4
 }
 
 // ---------------------------------------------------------------- kernel
+struct TcProduct {
+  CUtensorMap tmA[2], tmB[2], tmY;
+  int M, N;
+  int tiles_m, tiles_n, first;                  // first: number of its first tile
+  int ksteps, segments;                         // 128-byte steps of one segment
+  int a_mn, b_mn;
+};
+constexpr int TC_PRODUCTS = 4;
 struct GemmTcParams {
-  CUtensorMap tmA[2], tmB[2];
-  CUtensorMap tmY, tmO1, tmO2, tmI0, tmI1;      // results and inputs of the epilogue (I0: residual in EPI_LINEAR)
+  TcProduct pr[TC_PRODUCTS];
+  CUtensorMap tmO1, tmO2, tmI0, tmI1;           // further results and inputs of the epilogue (I0: residual in EPI_LINEAR); one product
   Epi e;
-  float* part;              // PARTIAL: [splits][products][M][ldp] fp32
-  int M, N, ldp;
-  int tiles_m, tiles_n;
-  int ksteps, segments;     // 128-byte steps of one segment
-  int splits, per_split;    // the steps of all segments, dealt out to `splits` tiles
+  float* part;                                  // PARTIAL: [splits][products][M][ldp] fp32; one product
+  int ldp;
+  int products, tiles;                          // tiles: of all products and splits
+  int splits, per_split;                        // the steps of all segments, dealt out to `splits` tiles
 };
 
 // EPI_SLOPE: EPI_LINEAR that also writes act' (e.o1).  EPI_PARTIAL, EPI_PARTIAL2: raw sums of one product, of a gated pair,
@@ -137,7 +147,7 @@ template <int CG, int BN> struct TcShape {
 };
 
 // F: 0 fp16, 1 bf16, 2 e4m3, 3 e5m2;  T: result type
-template <int F, typename T, bool A_MN, bool B_MN, int MODE, int CG, int BN>
+template <int F, typename T, int MODE, int CG, int BN>
 __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant__ GemmTcParams p) {
   using S = TcShape<CG, BN>;
   constexpr bool F8 = F >= 2;
@@ -145,8 +155,7 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
   constexpr bool PAIR = MODE == EPI_GLU || MODE == EPI_PARTIAL2;     // two products a tile
   constexpr int NW = PAIR ? BN / 2 : BN;                             // result columns of a tile
   constexpr int BROWS = BN / CG;                                     // B rows that this CTA brings
-  constexpr uint32_t IDESC = idesc_f16(F8 ? F - 2 : F, 128 * CG, BN, A_MN, B_MN);
-  static_assert(!F8 || (!A_MN && !B_MN), "fp8 operands are k-major");
+  constexpr uint32_t IDESC = idesc_f16(F8 ? F - 2 : F, 128 * CG, BN, 0, 0);
 
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -158,8 +167,6 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t rank = CG == 2 ? cluster_rank() : 0;
   const int unit = blockIdx.x / CG, units = gridDim.x / CG;
-  const int tiles = p.tiles_m * p.tiles_n * p.splits;
-  const int all_steps = p.ksteps * p.segments;
 
   if (tid == 0) {
     abort_flag = 0;
@@ -178,33 +185,46 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
   grid_dep_launch();                                                     // the next product's CTAs may set themselves up as these leave
   grid_dep_wait();
 
-  // tile t: which split of the contraction, which rows and columns (8 tile rows walk the columns together: their B tiles meet in L2)
-  auto place = [&](int t, int& m0, int& n0, int& k0, int& k1, int& split) {
-    const int mn = p.tiles_m * p.tiles_n;
-    split = t / mn;
-    t -= split * mn;
-    const int group = 8 * p.tiles_n, g = t / group, first = g * 8, rows = min(8, p.tiles_m - first);
+  // tile t: whose it is, which split of the contraction, which rows and columns (8 tile rows walk the columns together: their
+  // B tiles meet in L2)
+  struct Place { const TcProduct* pr; int m0, n0, k0, k1, split; };
+  auto place = [&](int t) {
+    Place w;
+    int i = 0;
+    while (i + 1 < p.products && t >= p.pr[i + 1].first) ++i;
+    w.pr = &p.pr[i];
+    t -= w.pr->first;
+    const int mn = w.pr->tiles_m * w.pr->tiles_n;
+    w.split = t / mn;
+    t -= w.split * mn;
+    const int group = 8 * w.pr->tiles_n, g = t / group, first = g * 8, rows = min(8, w.pr->tiles_m - first);
     t -= g * group;
-    m0 = (first + t % rows) * 128 * CG;
-    n0 = t / rows * NW;
-    k0 = split * p.per_split;
-    k1 = min(all_steps, k0 + p.per_split);
+    w.m0 = (first + t % rows) * 128 * CG;
+    w.n0 = t / rows * NW;
+    const int steps = w.pr->ksteps * w.pr->segments;
+    w.k0 = w.split * p.per_split;
+    w.k1 = p.splits == 1 ? steps : min(steps, w.k0 + p.per_split);
+    return w;
   };
 
   if (warp == 0) {
     // =============================== TMA producer ===============================
     const bool leader = elect_one();
     if (leader) {
-      for (int i = 0; i < p.segments; ++i) { tma_prefetch_desc(&p.tmA[i]); tma_prefetch_desc(&p.tmB[i]); }
-      if constexpr (PAIR) tma_prefetch_desc(&p.tmB[1]);
+      for (int i = 0; i < p.products; ++i) {
+        tma_prefetch_desc(&p.pr[i].tmA[0]);
+        tma_prefetch_desc(&p.pr[i].tmB[0]);
+        if (p.pr[i].segments == 2) { tma_prefetch_desc(&p.pr[i].tmA[1]); tma_prefetch_desc(&p.pr[i].tmB[1]); }
+      }
+      if constexpr (PAIR) tma_prefetch_desc(&p.pr[0].tmB[1]);
     }
     __syncwarp();
     int it = 0;
     bool ok = true;
-    for (int t = unit; t < tiles && ok; t += units) {
-      int m0, n0, k0, k1, split;
-      place(t, m0, n0, k0, k1, split);
-      for (int k = k0; k < k1; ++k, ++it) {
+    for (int t = unit; t < p.tiles && ok; t += units) {
+      const Place w = place(t);
+      const int a_mn = w.pr->a_mn, b_mn = w.pr->b_mn, ksteps = w.pr->ksteps, ma = w.m0 + (int)rank * 128, nb = w.n0 + (int)rank * BROWS;
+      for (int k = w.k0; k < w.k1; ++k, ++it) {
         const int s = it % S::STAGES, ph = (it / S::STAGES) & 1;
         ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[s]), ph ^ 1, &abort_flag));
         if (!ok) { fail_id = 1; break; }
@@ -212,23 +232,23 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
           uint32_t bar = smem_u32(&full[s]);
           if (rank == 0) mbar_expect_tx(bar, CG * (S::A_BYTES + S::B_BYTES));
           if constexpr (CG == 2) bar = map_to_rank(bar, 0);
-          const int seg = k >= p.ksteps, kc = (k - seg * p.ksteps) * KE;
+          const int seg = k >= ksteps, kc = (k - seg * ksteps) * KE;
           const uint32_t da = s_tiles + s * (S::A_BYTES + S::B_BYTES), db = da + S::A_BYTES;
-          const int ma = m0 + (int)rank * 128;
-          if constexpr (A_MN) {
-            tma_load_2d<CG>(da, &p.tmA[seg], bar, ma, kc);
-            tma_load_2d<CG>(da + 8192, &p.tmA[seg], bar, ma + 64, kc);
+          const CUtensorMap *ta = &w.pr->tmA[seg], *tb = &w.pr->tmB[seg];
+          if (!F8 && a_mn) {
+            tma_load_2d<CG>(da, ta, bar, ma, kc);
+            tma_load_2d<CG>(da + 8192, ta, bar, ma + 64, kc);
           } else {
-            tma_load_2d<CG>(da, &p.tmA[seg], bar, kc, ma);
+            tma_load_2d<CG>(da, ta, bar, kc, ma);
           }
           if constexpr (PAIR) {
-            if constexpr (CG == 2) tma_load_2d<CG>(db, &p.tmB[rank], bar, kc, n0);
-            else { tma_load_2d<CG>(db, &p.tmB[0], bar, kc, n0); tma_load_2d<CG>(db + S::B_BYTES / 2, &p.tmB[1], bar, kc, n0); }
-          } else if constexpr (B_MN) {
+            if constexpr (CG == 2) tma_load_2d<CG>(db, &w.pr->tmB[rank], bar, kc, w.n0);
+            else { tma_load_2d<CG>(db, &w.pr->tmB[0], bar, kc, w.n0); tma_load_2d<CG>(db + S::B_BYTES / 2, &w.pr->tmB[1], bar, kc, w.n0); }
+          } else if (!F8 && b_mn) {
 #pragma unroll
-            for (int c = 0; c < BROWS / 64; ++c) tma_load_2d<CG>(db + c * 8192, &p.tmB[seg], bar, n0 + (int)rank * BROWS + c * 64, kc);
+            for (int c = 0; c < BROWS / 64; ++c) tma_load_2d<CG>(db + c * 8192, tb, bar, nb + c * 64, kc);
           } else {
-            tma_load_2d<CG>(db, &p.tmB[seg], bar, kc, n0 + (int)rank * BROWS);
+            tma_load_2d<CG>(db, tb, bar, kc, nb);
           }
         }
         __syncwarp();
@@ -240,24 +260,26 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
       const bool leader = elect_one();
       int it = 0, n = 0;
       bool ok = true;
-      for (int t = unit; t < tiles && ok; t += units, ++n) {
-        int m0, n0, k0, k1, split;
-        place(t, m0, n0, k0, k1, split);
+      for (int t = unit; t < p.tiles && ok; t += units, ++n) {
+        const Place w = place(t);
+        const int a_mn = F8 ? 0 : w.pr->a_mn, b_mn = F8 ? 0 : w.pr->b_mn;
+        const uint32_t idesc = IDESC | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16);
+        const int sa = a_mn ? 128 : 2, sb = b_mn ? 128 : 2;               // from one 32-byte (or 16-row) slice of a step to the next
         const int buf = n & 1;
         ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&tempty[buf]), ((n >> 1) & 1) ^ 1, &abort_flag));
         if (!ok) { fail_id = 2; break; }
         tc_fence_after();
         const uint32_t acc = tmem + buf * BN;
-        for (int k = k0; k < k1; ++k, ++it) {
+        for (int k = w.k0; k < w.k1; ++k, ++it) {
           const int s = it % S::STAGES, ph = (it / S::STAGES) & 1;
           ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[s]), ph, &abort_flag));
           if (!ok) { fail_id = 3; break; }
           tc_fence_after();
           if (leader) {
             const uint32_t da = s_tiles + s * (S::A_BYTES + S::B_BYTES);
-            const uint64_t a = smem_desc_sw128(da, A_MN ? 8192 : 16, 1024), b = smem_desc_sw128(da + S::A_BYTES, B_MN ? 8192 : 16, 1024);
+            const uint64_t a = smem_desc_sw128(da, a_mn ? 8192 : 16, 1024), b = smem_desc_sw128(da + S::A_BYTES, b_mn ? 8192 : 16, 1024);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) mma<CG, F8>(acc, a + i * (A_MN ? 128 : 2), b + i * (B_MN ? 128 : 2), IDESC, (k > k0 || i > 0) ? 1u : 0u);
+            for (int i = 0; i < 4; ++i) mma<CG, F8>(acc, a + i * sa, b + i * sb, idesc, (k > w.k0 || i > 0) ? 1u : 0u);
             commit<CG>(smem_u32(&empty[s]));
           }
           __syncwarp();
@@ -290,11 +312,11 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
     auto piece = [&](uint32_t box, int j) { return CW == 64 ? box + row * 128 + ((j ^ (row & 7)) << 4) : box + row * 64 + ((j ^ ((row >> 1) & 3)) << 4); };
     int n = 0, cnt = 0;                                                  // tiles and chunks so far
     bool ok = true;
-    for (int t = unit; t < tiles; t += units, ++n) {
-      int m0, n0, k0, k1, split;
-      place(t, m0, n0, k0, k1, split);
+    for (int t = unit; t < p.tiles; t += units, ++n) {
+      const Place w = place(t);
       const int buf = n & 1;
-      const int mr = m0 + (int)rank * 128, nc0 = n0 + group * GW;
+      const int M = w.pr->M, N = w.pr->N;
+      const int mr = w.m0 + (int)rank * 128, nc0 = w.n0 + group * GW;
       auto request = [&](int c, int count) {                             // lead only: the inputs of chunk c of this tile
         const int st = count & 1;
         const uint32_t bar = smem_u32(&loaded[group][st]), box = stage0 + st * STAGE;
@@ -314,7 +336,7 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
       const uint32_t acc = tmem + lanes + buf * BN + group * GW;
       const int grow = mr + row;
       float xs = 1.f;
-      if constexpr (LIN) { if (p.e.xs != nullptr && grow < p.M) xs = p.e.xs[grow]; }
+      if constexpr (LIN) { if (p.e.xs != nullptr && grow < M) xs = p.e.xs[grow]; }
       auto drained = [&] {                                               // the last sums are in registers: the buffer may be filled again
         tc_fence_before();
         __syncwarp();
@@ -331,10 +353,10 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
             uint32_t v[16];
             tmem_ld16(acc + c + q * NW, v);
             tc_wait_ld();
-            float* dst = p.part + (((long long)split * (PAIR ? 2 : 1) + q) * p.M + grow) * p.ldp + nc0 + c;
+            float* dst = p.part + (((long long)w.split * (PAIR ? 2 : 1) + q) * M + grow) * p.ldp + nc0 + c;
 #pragma unroll
             for (int i = 0; i < 16; i += 4)
-              if (grow < p.M && nc0 + c + i < p.ldp) *reinterpret_cast<uint4*>(dst + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+              if (grow < M && nc0 + c + i < p.ldp) *reinterpret_cast<uint4*>(dst + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
           }
         }
         drained();
@@ -359,8 +381,8 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
               uint32_t v[16];
               tmem_ld16(acc + col, v);
               if constexpr (MODE == EPI_GLU) {
-                uint32_t w[16];
-                tmem_ld16(acc + NW + col, w);
+                uint32_t u[16];
+                tmem_ld16(acc + NW + col, u);
                 tc_wait_ld();
                 float d[16];
 #pragma unroll
@@ -368,14 +390,14 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
                 if (p.e.o1 != nullptr) {
                   act_all_both(a, d, p.e.act);
 #pragma unroll
-                  for (int i = 0; i < 16; ++i) d[i] *= __uint_as_float(w[i]);
+                  for (int i = 0; i < 16; ++i) d[i] *= __uint_as_float(u[i]);
                   put16<T>(piece(box + BOX, 2 * h), piece(box + BOX, 2 * h + 1), a);
                   put16<T>(piece(box + 2 * BOX, 2 * h), piece(box + 2 * BOX, 2 * h + 1), d);
                 } else {
                   act_all(a, p.e.act);
                 }
 #pragma unroll
-                for (int i = 0; i < 16; ++i) a[i] *= __uint_as_float(w[i]);
+                for (int i = 0; i < 16; ++i) a[i] *= __uint_as_float(u[i]);
               } else {
                 tc_wait_ld();
 #pragma unroll
@@ -388,15 +410,15 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
               if (p.e.xs != nullptr) {
 #pragma unroll
                 for (int i = 0; i < 16; i += 4)
-                  if (gc + i < p.N) {
-                    const float4 w = *reinterpret_cast<const float4*>(p.e.ws + gc + i);
-                    a[i] *= xs * w.x; a[i + 1] *= xs * w.y; a[i + 2] *= xs * w.z; a[i + 3] *= xs * w.w;
+                  if (gc + i < N) {
+                    const float4 f = *reinterpret_cast<const float4*>(p.e.ws + gc + i);
+                    a[i] *= xs * f.x; a[i + 1] *= xs * f.y; a[i + 2] *= xs * f.z; a[i + 3] *= xs * f.w;
                   }
               }
               if (p.e.bias != nullptr) {
 #pragma unroll
                 for (int i = 0; i < 16; i += 8)
-                  if (gc + i < p.N) add8<T>(a + i, *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.e.bias) + gc + i));
+                  if (gc + i < N) add8<T>(a + i, *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.e.bias) + gc + i));
               }
               if constexpr (MODE == EPI_SLOPE) {
                 float d[16];
@@ -426,9 +448,9 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
             const int gc = nc0 + c * CW;
             if constexpr (MODE == EPI_GLU_BWD) {
               tma_store_2d(&p.tmO1, box, gc, mr);
-              tma_store_2d(&p.tmY, box + BOX, gc, mr);
+              tma_store_2d(&w.pr->tmY, box + BOX, gc, mr);
             } else {
-              tma_store_2d(&p.tmY, box, gc, mr);
+              tma_store_2d(&w.pr->tmY, box, gc, mr);
               if constexpr (MODE == EPI_SLOPE) tma_store_2d(&p.tmO1, box + BOX, gc, mr);
               if constexpr (MODE == EPI_GLU) {
                 if (p.e.o1 != nullptr) { tma_store_2d(&p.tmO1, box + BOX, gc, mr); tma_store_2d(&p.tmO2, box + 2 * BOX, gc, mr); }
@@ -525,29 +547,27 @@ static int pitch(int N) { return (N + 7) / 8 * 8; }                     // of pa
 struct TcPlan { int cg, bn, tiles_m, tiles_n, ksteps, splits, per_split; bool raw; };
 static TcPlan tc_plan(const GemmProblem& p) {
   TcPlan t;
-  const int sms = sm_count();
   const int pair = p.e.mode == EPI_GLU ? 2 : 1;
-  auto tiles = [&](int cg, int bn, int& tm, int& tn) {
-    tm = (p.M + 128 * cg - 1) / (128 * cg);
-    tn = (p.N + bn / pair - 1) / (bn / pair);
-    return (long long)tm * tn;
-  };
-  t.cg = 2; t.bn = 256;
-  const long long big = tiles(2, 256, t.tiles_m, t.tiles_n);
-  if (big < sms / 2) { t.cg = 1; t.bn = 128; tiles(1, 128, t.tiles_m, t.tiles_n); }
+  t.cg = p.M <= 128 ? 1 : 2;
+  t.bn = t.cg * 128;
+  t.tiles_m = (p.M + 128 * t.cg - 1) / (128 * t.cg);
+  t.tiles_n = (p.N + t.bn / pair - 1) / (t.bn / pair);
   t.ksteps = (p.K * esize(p.dtype) + 127) / 128;
+  const long long n = (long long)t.tiles_m * t.tiles_n, units = sm_count() / t.cg;
   const int steps = t.ksteps * p.segments;
-  const long long n = (long long)t.tiles_m * t.tiles_n, units = sms / t.cg;
+  // Rounds of tiles at 512 clk a step, and 3000 for the epilogue that no other tile hides; splitting adds the sums' way out
+  // and back through L2 (64 bytes a clk and SM) and the joining kernel (6000).  The cheapest of up to 16 ways.
+  t.raw = !p.e.vec || !p.e.vecy;
+  double best = 0;
   t.splits = 1;
-  if (n * 2 <= units && steps >= 8) {
-    long long s = units / n;
-    if (s > steps / 4) s = steps / 4;
-    if (s > 16) s = 16;
-    t.splits = (int)(s < 1 ? 1 : s);
+  t.per_split = steps;
+  for (int s = 1; s <= 16 && s * 4 <= (steps > 4 ? steps : 4); ++s) {
+    const int per = (steps + s - 1) / s, ways = (steps + per - 1) / per;
+    double cost = (double)((n * ways + units - 1) / units) * per * 512 + 3000;
+    if (ways > 1 || t.raw) cost += 6000 + 8.0 * ways * pair * p.M * p.N / (64.0 * sm_count());
+    if (s == 1 || cost < best) { best = cost; t.splits = ways; t.per_split = per; }
   }
-  t.per_split = (steps + t.splits - 1) / t.splits;
-  t.splits = (steps + t.per_split - 1) / t.per_split;
-  t.raw = t.splits > 1 || !p.e.vec || !p.e.vecy;
+  t.raw = t.raw || t.splits > 1;
   return t;
 }
 
@@ -556,10 +576,10 @@ long long gemm_tc5_ws_bytes(const GemmProblem& p) {
   return t.raw ? (long long)t.splits * (p.e.mode == EPI_GLU ? 2 : 1) * p.M * pitch(p.N) * 4 : 0;
 }
 
-template <int F, typename T, bool A_MN, bool B_MN, int MODE, int CG, int BN>
-static int tc_launch(const GemmTcParams& g, long long tiles, cudaStream_t st) {
+template <int F, typename T, int MODE, int CG, int BN>
+static int tc_launch(const GemmTcParams& g, cudaStream_t st) {
   using S = TcShape<CG, BN>;
-  auto fn = gemm_tc5_kernel<F, T, A_MN, B_MN, MODE, CG, BN>;
+  auto fn = gemm_tc5_kernel<F, T, MODE, CG, BN>;
   static bool prepared[64];                   // per device: the attribute outlasts the call, and setting it twice is harmless
   int dev = 0;
   NSA_CUDA_OK(cudaGetDevice(&dev));
@@ -567,9 +587,9 @@ static int tc_launch(const GemmTcParams& g, long long tiles, cudaStream_t st) {
     NSA_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM));
     if (dev < 64) prepared[dev] = true;
   }
-  const long long units = sm_count() / CG;
+  const int units = sm_count() / CG;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((tiles < units ? tiles : units) * CG));
+  cfg.gridDim = dim3((unsigned)((g.tiles < units ? g.tiles : units) * CG));
   cfg.blockDim = dim3(384);
   cfg.dynamicSmemBytes = S::SMEM;
   cfg.stream = st;
@@ -585,28 +605,28 @@ static int tc_launch(const GemmTcParams& g, long long tiles, cudaStream_t st) {
   return NSA_OK;
 }
 
-template <int F, typename T, bool A_MN, bool B_MN, int MODE>
-static int tc_shape(const GemmTcParams& g, const TcPlan& t, cudaStream_t st) {
-  const long long tiles = (long long)t.tiles_m * t.tiles_n * t.splits;
-  if (t.cg == 2) return tc_launch<F, T, A_MN, B_MN, MODE, 2, 256>(g, tiles, st);
-  return tc_launch<F, T, A_MN, B_MN, MODE, 1, 128>(g, tiles, st);
+template <int F, typename T, int MODE>
+static int tc_shape(const GemmTcParams& g, int cg, cudaStream_t st) {
+  return cg == 2 ? tc_launch<F, T, MODE, 2, 256>(g, st) : tc_launch<F, T, MODE, 1, 128>(g, st);
 }
 
+// mode: EPI_*, as the kernel has it
 template <int F, typename T>
-static int tc_mode(const GemmTcParams& g, const TcPlan& t, const GemmProblem& p, cudaStream_t st) {
-  if constexpr (F >= 2) {
-    return t.raw ? tc_shape<F, T, false, false, EPI_PARTIAL>(g, t, st) : tc_shape<F, T, false, false, EPI_LINEAR>(g, t, st);
-  } else {
-    if (p.e.mode == EPI_GLU) return t.raw ? tc_shape<F, T, false, false, EPI_PARTIAL2>(g, t, st) : tc_shape<F, T, false, false, EPI_GLU>(g, t, st);
-    if (t.raw) {
-      if (p.a_mn) return tc_shape<F, T, true, true, EPI_PARTIAL>(g, t, st);
-      return p.b_mn ? tc_shape<F, T, false, true, EPI_PARTIAL>(g, t, st) : tc_shape<F, T, false, false, EPI_PARTIAL>(g, t, st);
-    }
-    if (p.e.mode == EPI_GLU_BWD) return tc_shape<F, T, false, true, EPI_GLU_BWD>(g, t, st);
-    if (p.a_mn) return tc_shape<F, T, true, true, EPI_LINEAR>(g, t, st);
-    if (p.b_mn) return tc_shape<F, T, false, true, EPI_LINEAR>(g, t, st);
-    return p.e.o1 != nullptr ? tc_shape<F, T, false, false, EPI_SLOPE>(g, t, st) : tc_shape<F, T, false, false, EPI_LINEAR>(g, t, st);
+static int tc_mode(const GemmTcParams& g, int cg, int mode, cudaStream_t st) {
+  if (mode == EPI_PARTIAL) return tc_shape<F, T, EPI_PARTIAL>(g, cg, st);
+  if constexpr (F < 2) {
+    if (mode == EPI_PARTIAL2) return tc_shape<F, T, EPI_PARTIAL2>(g, cg, st);
+    if (mode == EPI_GLU) return tc_shape<F, T, EPI_GLU>(g, cg, st);
+    if (mode == EPI_GLU_BWD) return tc_shape<F, T, EPI_GLU_BWD>(g, cg, st);
+    if (mode == EPI_SLOPE) return tc_shape<F, T, EPI_SLOPE>(g, cg, st);
   }
+  return tc_shape<F, T, EPI_LINEAR>(g, cg, st);
+}
+static int tc_types(const GemmTcParams& g, int cg, int mode, int dtype, bool bf, cudaStream_t st) {
+  if (dtype == NSA_BF16) return tc_mode<1, __nv_bfloat16>(g, cg, mode, st);
+  if (dtype == NSA_FP16) return tc_mode<0, __half>(g, cg, mode, st);
+  if (dtype == NSA_FP8_E4M3) return bf ? tc_mode<2, __nv_bfloat16>(g, cg, mode, st) : tc_mode<2, __half>(g, cg, mode, st);
+  return bf ? tc_mode<3, __nv_bfloat16>(g, cg, mode, st) : tc_mode<3, __half>(g, cg, mode, st);
 }
 
 template <typename T>
@@ -618,26 +638,38 @@ static int join(const float* part, const GemmProblem& p, int splits, cudaStream_
   return launch_pdl("gemm_join", gemm_join_kernel<T, EPI_LINEAR>, grid, 256, 0, st, part, p.e, splits, pitch(p.N));
 }
 
-int gemm_tc5(const GemmProblem& p, void* ws, cudaStream_t st) {
-  const TcPlan t = tc_plan(p);
-  NSA_REQUIRE((long long)t.tiles_m * t.tiles_n * t.splits < 2147483647LL, NSA_ERR_ARG, "matrix product: %d x %d results are too many tiles", p.M, p.N);
-  GemmTcParams g;
+// The maps and sizes of one product
+static int tc_product(TcProduct* r, const GemmProblem& p, const TcPlan& t) {
   int rc;
   const int ke = 128 / esize(p.dtype);
   const int pair = p.e.mode == EPI_GLU;
   const int brows = pair ? t.bn / 2 : t.bn / t.cg;                     // rows of a box of B
   for (int i = 0; i < p.segments; ++i) {
-    rc = p.a_mn ? map_2d(&g.tmA[i], p.A[i], p.K, p.M, p.lda, ke, ke, p.dtype) : map_2d(&g.tmA[i], p.A[i], p.M, p.K, p.lda, ke, 128, p.dtype);
+    rc = p.a_mn ? map_2d(&r->tmA[i], p.A[i], p.K, p.M, p.lda, ke, ke, p.dtype) : map_2d(&r->tmA[i], p.A[i], p.M, p.K, p.lda, ke, 128, p.dtype);
     if (rc != NSA_OK) return rc;
-    rc = p.b_mn ? map_2d(&g.tmB[i], p.B[i], p.K, p.N, p.ldb, ke, ke, p.dtype) : map_2d(&g.tmB[i], p.B[i], p.N, p.K, p.ldb, ke, brows, p.dtype);
+    rc = p.b_mn ? map_2d(&r->tmB[i], p.B[i], p.K, p.N, p.ldb, ke, ke, p.dtype) : map_2d(&r->tmB[i], p.B[i], p.N, p.K, p.ldb, ke, brows, p.dtype);
     if (rc != NSA_OK) return rc;
   }
-  if (pair && (rc = map_2d(&g.tmB[1], p.B[1], p.N, p.K, p.ldb, ke, brows, p.dtype)) != NSA_OK) return rc;
+  if (pair && (rc = map_2d(&r->tmB[1], p.B[1], p.N, p.K, p.ldb, ke, brows, p.dtype)) != NSA_OK) return rc;
+  r->M = p.M; r->N = p.N;
+  r->tiles_m = t.tiles_m; r->tiles_n = t.tiles_n; r->first = 0;
+  r->ksteps = t.ksteps; r->segments = p.segments;
+  r->a_mn = p.a_mn; r->b_mn = p.b_mn;
+  return NSA_OK;
+}
+
+int gemm_tc5(const GemmProblem& p, void* ws, cudaStream_t st) {
+  const TcPlan t = tc_plan(p);
+  const long long tiles = (long long)t.tiles_m * t.tiles_n * t.splits;
+  NSA_REQUIRE(tiles < 2147483647LL - 65536, NSA_ERR_ARG, "matrix product: %d x %d results are too many tiles", p.M, p.N);
+  GemmTcParams g;
+  int rc = tc_product(&g.pr[0], p, t);
+  if (rc != NSA_OK) return rc;
+  const bool gated = p.e.mode != EPI_LINEAR, slope = !gated && p.e.o1 != nullptr;
   if (!t.raw) {
-    const bool gated = p.e.mode != EPI_LINEAR;
-    const int cw = gated || p.e.o1 != nullptr ? 32 : 64;
+    const int cw = gated || slope ? 32 : 64;
     auto box = [&](CUtensorMap* m, const void* ptr, long long ld) { return ptr == nullptr ? NSA_OK : map_2d(m, ptr, p.M, p.N, ld, cw, 128, p.out_dtype); };
-    if ((rc = box(&g.tmY, p.e.y, p.e.ldy)) != NSA_OK) return rc;
+    if ((rc = box(&g.pr[0].tmY, p.e.y, p.e.ldy)) != NSA_OK) return rc;
     if ((rc = box(&g.tmO1, p.e.o1, gated ? p.e.ldy : p.N)) != NSA_OK) return rc;
     if ((rc = box(&g.tmO2, p.e.o2, p.e.ldy)) != NSA_OK) return rc;
     if ((rc = box(&g.tmI0, gated ? p.e.i0 : p.e.residual, gated ? p.e.ldy : p.N)) != NSA_OK) return rc;
@@ -645,17 +677,74 @@ int gemm_tc5(const GemmProblem& p, void* ws, cudaStream_t st) {
   }
   g.e = p.e;
   g.part = reinterpret_cast<float*>(ws);
-  g.M = p.M; g.N = p.N; g.ldp = pitch(p.N);
-  g.tiles_m = t.tiles_m; g.tiles_n = t.tiles_n;
-  g.ksteps = t.ksteps; g.segments = p.segments;
+  g.ldp = pitch(p.N);
+  g.products = 1; g.tiles = (int)tiles;
   g.splits = t.splits; g.per_split = t.per_split;
   const bool bf = p.out_dtype == NSA_BF16;
-  if (p.dtype == NSA_BF16) rc = tc_mode<1, __nv_bfloat16>(g, t, p, st);
-  else if (p.dtype == NSA_FP16) rc = tc_mode<0, __half>(g, t, p, st);
-  else if (p.dtype == NSA_FP8_E4M3) rc = bf ? tc_mode<2, __nv_bfloat16>(g, t, p, st) : tc_mode<2, __half>(g, t, p, st);
-  else rc = bf ? tc_mode<3, __nv_bfloat16>(g, t, p, st) : tc_mode<3, __half>(g, t, p, st);
+  const int mode = t.raw ? (p.e.mode == EPI_GLU ? EPI_PARTIAL2 : EPI_PARTIAL) : slope ? EPI_SLOPE : p.e.mode;
+  rc = tc_types(g, t.cg, mode, p.dtype, bf, st);
   if (rc != NSA_OK || !t.raw) return rc;
   return bf ? join<__nv_bfloat16>(g.part, p, t.splits, st) : join<__half>(g.part, p, t.splits, st);
+}
+
+// Several plain products (EPI_LINEAR with nothing around the sums) of one 16-bit type.  One launch where each would run
+// unsplit on CTA pairs or where together they fill the SMs; else one by one.
+static bool groups(const GemmProblem* p, int count) {
+  if (count < 2 || count > TC_PRODUCTS) return false;
+  long long tiles = 0;
+  bool single = true;
+  for (int i = 0; i < count; ++i) {
+    const TcPlan t = tc_plan(p[i]);
+    if (t.cg != 2 || !p[i].e.vec || !p[i].e.vecy) return false;
+    tiles += (long long)t.tiles_m * t.tiles_n;
+    single = single && t.splits == 1;
+  }
+  return tiles < 2147483647LL - 65536 && (single || tiles * 2 >= sm_count());
+}
+
+long long gemm_tc5_group_ws_bytes(const GemmProblem* p, int count) {
+  long long most = 0;
+  if (!groups(p, count))
+    for (int i = 0; i < count; ++i) {
+      const long long n = gemm_tc5_ws_bytes(p[i]);
+      if (n > most) most = n;
+    }
+  return most;
+}
+
+int gemm_tc5_group(const GemmProblem* p, int count, void* ws, cudaStream_t st) {
+  if (!groups(p, count)) {
+    for (int i = 0; i < count; ++i) {
+      const int rc = gemm_tc5(p[i], ws, st);
+      if (rc != NSA_OK) return rc;
+    }
+    return NSA_OK;
+  }
+  GemmTcParams g;
+  g.e = p[0].e;
+  g.part = nullptr;
+  g.ldp = 0;
+  g.products = count;
+  g.splits = 1; g.per_split = 0;
+  // the longest tiles first: the last round is then of the shortest
+  int order[TC_PRODUCTS];
+  for (int i = 0; i < count; ++i) {
+    int j = i;
+    for (; j > 0 && (long long)p[order[j - 1]].K * p[order[j - 1]].segments < (long long)p[i].K * p[i].segments; --j) order[j] = order[j - 1];
+    order[j] = i;
+  }
+  int tiles = 0;
+  for (int i = 0; i < count; ++i) {
+    const GemmProblem& q = p[order[i]];
+    const TcPlan t = tc_plan(q);
+    int rc = tc_product(&g.pr[i], q, t);
+    if (rc == NSA_OK) rc = map_2d(&g.pr[i].tmY, q.e.y, q.M, q.N, q.e.ldy, 64, 128, q.out_dtype);
+    if (rc != NSA_OK) return rc;
+    g.pr[i].first = tiles;
+    tiles += t.tiles_m * t.tiles_n;
+  }
+  g.tiles = tiles;
+  return tc_types(g, 2, EPI_LINEAR, p[0].dtype, p[0].out_dtype == NSA_BF16, st);
 }
 
 int gemm_take_status(int* status) {

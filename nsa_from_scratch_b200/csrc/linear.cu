@@ -164,14 +164,24 @@ static GemmProblem problem(Mat A, int a_mn, Mat B, int b_mn, int M, int N, int K
   p.e.M = M; p.e.N = N; p.e.ldy = N;
   return p;
 }
-// EPI_LINEAR without anything around the sums
-static int product(Arena& w, GemmProblem p, void* out) {
-  if (out == nullptr) return NSA_OK;
-  p.e.mode = EPI_LINEAR;
-  p.e.y = out;
-  p.e.vec = p.e.vecy = p.N % 8 == 0 && aligned16(out);
-  return gemm(w, p);
-}
+// Plain products that are independent of each other, gathered for one launch.
+struct Products {
+  GemmProblem p[4];
+  int count = 0;
+  void add(GemmProblem q, void* out) {
+    q.e.mode = EPI_LINEAR;
+    q.e.y = out;
+    q.e.vec = q.e.vecy = q.N % 8 == 0 && aligned16(out);
+    p[count++] = q;
+  }
+  int run(Arena& w) const {
+    if (count == 0) return NSA_OK;
+    if (!w.dry()) return gemm_tc5_group(p, count, w.base + w.scratch_at, w.st);
+    const long long need = gemm_tc5_group_ws_bytes(p, count);
+    if (need > w.scratch) w.scratch = need;
+    return NSA_OK;
+  }
+};
 
 static int zero(void* p, long long bytes, cudaStream_t st) {
   if (p != nullptr) NSA_CUDA_OK(cudaMemsetAsync(p, 0, (size_t)bytes, st));
@@ -229,18 +239,19 @@ static int linear_bwd_steps(const nsa_linear_bwd_args& a, Arena& w) {
     if (run) NSA_TRY(act_bwd(a.dy, a.slope, dz, ld, a.dbias ? part : nullptr, a.M, a.N, a.dtype, w.st));
   } else {
     if (run && a.dbias) NSA_TRY(act_bwd(a.dy, nullptr, nullptr, 0, part, a.M, a.N, a.dtype, w.st));
-    if (a.dx || a.dw || !run) NSA_TRY(operand(w, a.dy, a.M, a.N, a.dtype, &g));
+    if (a.dx || a.dw) NSA_TRY(operand(w, a.dy, a.M, a.N, a.dtype, &g));
   }
   if (run && a.dbias) NSA_TRY(column_sum(part, a.dbias, act_bwd_plan(a.M, a.N).groups, a.N, a.dtype, w.st));
-  if (a.dx || !run) {
+  Products ps;
+  if (a.dx) {
     NSA_TRY(operand(w, a.w, a.N, a.K, a.dtype, &wt));
-    NSA_TRY(product(w, problem(g, 0, wt, 1, a.M, a.K, a.N, a.dtype), run ? a.dx : &w));
+    ps.add(problem(g, 0, wt, 1, a.M, a.K, a.N, a.dtype), a.dx);
   }
-  if (a.dw || !run) {
+  if (a.dw) {
     NSA_TRY(operand(w, a.x, a.M, a.K, a.dtype, &x));
-    NSA_TRY(product(w, problem(g, 1, x, 1, a.N, a.K, a.M, a.dtype), run ? a.dw : &w));
+    ps.add(problem(g, 1, x, 1, a.N, a.K, a.M, a.dtype), a.dw);
   }
-  return NSA_OK;
+  return ps.run(w);
 }
 
 int linear_bwd(const nsa_linear_bwd_args& a, cudaStream_t st) {
@@ -295,7 +306,6 @@ int gated_mlp(const nsa_gated_mlp_args& a, cudaStream_t st) {
 }
 
 static int mlp_bwd_steps(const nsa_gated_mlp_bwd_args& a, Arena& w) {
-  const bool run = !w.dry();
   const long long ldh = padded(a.F, a.dtype);
   void *dg = w.take((long long)a.M * ldh * 2), *du = w.take((long long)a.M * ldh * 2);
   Mat dy, x, wg, wu, wd;
@@ -307,21 +317,20 @@ static int mlp_bwd_steps(const nsa_gated_mlp_bwd_args& a, Arena& w) {
   p.e.y = dg; p.e.o1 = du;
   p.e.ldy = ldh; p.e.vec = p.e.vecy = 1;
   NSA_TRY(gemm(w, p));
-  if (a.dx || !run) {                                                                       // dx = dg wg + du wu
+  Products ps;
+  if (a.dwg || a.dwu) NSA_TRY(operand(w, a.x, a.M, a.N, a.dtype, &x));
+  if (a.dwg) ps.add(problem(Mat{dg, ldh}, 1, x, 1, a.F, a.N, a.M, a.dtype), a.dwg);
+  if (a.dwu) ps.add(problem(Mat{du, ldh}, 1, x, 1, a.F, a.N, a.M, a.dtype), a.dwu);
+  if (a.dwd) ps.add(problem(dy, 1, Mat{a.h, ldh}, 1, a.N, a.F, a.M, a.dtype), a.dwd);
+  if (a.dx) {                                                                               // dx = dg wg + du wu
     NSA_TRY(operand(w, a.wg, a.F, a.N, a.dtype, &wg));
     NSA_TRY(operand(w, a.wu, a.F, a.N, a.dtype, &wu));
     GemmProblem q = problem(Mat{dg, ldh}, 0, wg, 1, a.M, a.N, a.F, a.dtype);
     q.A[1] = du; q.B[1] = wu.p;
     q.segments = 2;
-    NSA_TRY(product(w, q, run ? a.dx : &w));
+    ps.add(q, a.dx);
   }
-  if (a.dwg || a.dwu || !run) {
-    NSA_TRY(operand(w, a.x, a.M, a.N, a.dtype, &x));
-    NSA_TRY(product(w, problem(Mat{dg, ldh}, 1, x, 1, a.F, a.N, a.M, a.dtype), run ? a.dwg : &w));
-    NSA_TRY(product(w, problem(Mat{du, ldh}, 1, x, 1, a.F, a.N, a.M, a.dtype), run ? a.dwu : &w));
-  }
-  if (a.dwd || !run) NSA_TRY(product(w, problem(dy, 1, Mat{a.h, ldh}, 1, a.N, a.F, a.M, a.dtype), run ? a.dwd : &w));
-  return NSA_OK;
+  return ps.run(w);
 }
 
 int gated_mlp_bwd(const nsa_gated_mlp_bwd_args& a, cudaStream_t st) {
