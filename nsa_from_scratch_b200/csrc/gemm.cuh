@@ -83,7 +83,7 @@ struct Epi {
   void *y, *o1, *o2;             // o1 (LINEAR), o1 and o2 (GLU): NULL: not wanted
 };
 
-// One product; rows of A and B start on 16-byte boundaries.
+// One product.  gemm_tc5: rows of A and B start on 16-byte boundaries.
 struct GemmProblem {
   const void *A[2], *B[2];       // EPI_GLU: B[0], B[1] are the two weights (one segment)
   int segments;                  // 1 or 2
@@ -179,6 +179,8 @@ static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t
 int sm_count();                                                            // of the current device (linear.cu)
 long long gemm_tc5_ws_bytes(const GemmProblem& p);                       // gemm_tc5.cu
 int gemm_tc5(const GemmProblem& p, void* ws, cudaStream_t st);
+bool gemm_skinny_takes(int M, int mode);                                   // gemm_skinny.cu: k-major operands of any alignment
+int gemm_skinny(const GemmProblem& p, bool early, cudaStream_t st);        // early: what runs before it in the stream does not write the weights
 long long gemm_tc5_group_ws_bytes(const GemmProblem* p, int count);
 int gemm_tc5_group(const GemmProblem* p, int count, void* ws, cudaStream_t st);
 int column_sum(const float* part, void* out, int parts, int N, int dt, cudaStream_t st);   // norm.cu

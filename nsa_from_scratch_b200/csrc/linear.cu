@@ -199,9 +199,12 @@ static int check_linear(const nsa_linear_args& a) {
 }
 
 static int linear_steps(const nsa_linear_args& a, Arena& w) {
-  Mat x, wt;
-  NSA_TRY(operand(w, a.x, a.M, a.K, a.dtype, &x));
-  NSA_TRY(operand(w, a.w, a.N, a.K, a.dtype, &wt));
+  const bool few = gemm_skinny_takes(a.M, EPI_LINEAR);
+  Mat x{a.x, a.K}, wt{a.w, a.K};
+  if (!few) {
+    NSA_TRY(operand(w, a.x, a.M, a.K, a.dtype, &x));
+    NSA_TRY(operand(w, a.w, a.N, a.K, a.dtype, &wt));
+  }
   GemmProblem p = problem(x, 0, wt, 0, a.M, a.N, a.K, a.dtype);
   p.out_dtype = a.y_dtype;
   p.e.mode = EPI_LINEAR;
@@ -210,6 +213,7 @@ static int linear_steps(const nsa_linear_args& a, Arena& w) {
   p.e.y = a.y; p.e.o1 = a.slope;
   p.e.vec = a.N % 8 == 0 && aligned16(a.bias) && aligned16(a.residual) && aligned16(a.slope) && aligned16(a.w_scale);
   p.e.vecy = a.N % 8 == 0 && aligned16(a.y);
+  if (few) return w.dry() ? NSA_OK : gemm_skinny(p, false, w.st);
   return gemm(w, p);
 }
 
@@ -275,24 +279,32 @@ static int check_mlp(int M, int N, int F, int dtype, int act) {
 static int mlp_steps(const nsa_gated_mlp_args& a, Arena& w) {
   const long long ldh = padded(a.F, a.dtype);
   void* h = a.h != nullptr ? a.h : w.take((long long)a.M * ldh * 2);
-  Mat x, wg, wu, wd;
-  NSA_TRY(operand(w, a.x, a.M, a.N, a.dtype, &x));
-  NSA_TRY(operand(w, a.wg, a.F, a.N, a.dtype, &wg));
-  NSA_TRY(operand(w, a.wu, a.F, a.N, a.dtype, &wu));
+  const bool few = gemm_skinny_takes(a.M, EPI_GLU), few_down = gemm_skinny_takes(a.M, EPI_LINEAR);
+  Mat x{a.x, a.N}, wg{a.wg, a.N}, wu{a.wu, a.N}, wd{a.wd, a.F};
+  if (!few) {
+    NSA_TRY(operand(w, a.x, a.M, a.N, a.dtype, &x));
+    NSA_TRY(operand(w, a.wg, a.F, a.N, a.dtype, &wg));
+    NSA_TRY(operand(w, a.wu, a.F, a.N, a.dtype, &wu));
+  }
   GemmProblem p = problem(x, 0, wg, 0, a.M, a.F, a.N, a.dtype);
   p.B[1] = wu.p;
   p.e.mode = EPI_GLU;
   p.e.act = a.act;
   p.e.y = h; p.e.o1 = a.p; p.e.o2 = a.s;
   p.e.ldy = ldh; p.e.vec = p.e.vecy = 1;
-  NSA_TRY(gemm(w, p));
-  NSA_TRY(operand(w, a.wd, a.N, a.F, a.dtype, &wd));
+  if (few) {
+    if (!w.dry()) NSA_TRY(gemm_skinny(p, false, w.st));
+  } else {
+    NSA_TRY(gemm(w, p));
+  }
+  if (!few_down) NSA_TRY(operand(w, a.wd, a.N, a.F, a.dtype, &wd));
   GemmProblem d = problem(Mat{h, ldh}, 0, wd, 0, a.M, a.N, a.F, a.dtype);
   d.e.mode = EPI_LINEAR;
   d.e.residual = a.residual;
   d.e.y = a.y;
   d.e.vec = a.N % 8 == 0 && aligned16(a.residual);
   d.e.vecy = a.N % 8 == 0 && aligned16(a.y);
+  if (few_down) return w.dry() ? NSA_OK : gemm_skinny(d, true, w.st);
   return gemm(w, d);
 }
 
