@@ -60,11 +60,11 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_axes_kernel(const RopeParam
   const int tn = min(p.tt, p.T - t0);
   const int all = p.heads[0] + p.heads[1] + p.heads[2], rotated = p.heads[0] + p.heads[1];
   const int h0 = blockIdx.y * p.per_block, h1 = min(all, h0 + p.per_block);
-  if (h0 < rotated) {
+  auto angles = [&] {
     for (int i = threadIdx.x; i < tn * half; i += ROPE_THREADS) {
       const int t = i / half, j = i % half;
       int axis = 0;
-      while (j >= p.sec_end[axis]) ++axis;                          // sec_end[n_axes - 1] == half
+      while (j >= p.sec_end[axis]) ++axis;                            // sec_end[n_axes - 1] == half
       const long long at = ((long long)axis * p.B + b) * p.T + t0 + t;
       const double pos = p.pos64 ? (double)reinterpret_cast<const long long*>(p.pos)[at] : (double)reinterpret_cast<const int*>(p.pos)[at];
       const double turns = pos * (p.inv_freq[j] * 0.15915494309189535);      // 1 / (2 pi)
@@ -72,8 +72,7 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_axes_kernel(const RopeParam
       sincospif((float)(2.0 * (turns - rint(turns))), &s, &c);
       cs[i] = make_float2(c, BACK ? -s : s);
     }
-    __syncthreads();
-  }
+  };
   // where head h (of q, k and v in a row) and token t start on either side
   auto rows = [&](int h, int t, const X*& src, Y*& dst) {
     const int which = h < p.heads[0] ? 0 : (h < rotated ? 1 : 2);
@@ -87,21 +86,26 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_axes_kernel(const RopeParam
   if constexpr (VEC) {
     const int chunks = p.D / 16;
     const int ch = threadIdx.x % chunks, rest = threadIdx.x / chunks, t = rest % p.tt;
-    const int step = ROPE_THREADS / chunks / p.tt, first = h0 + rest / p.tt;      // heads side by side
-    if (t >= tn || rest / p.tt >= step) return;
+    const int step = ROPE_THREADS / chunks / p.tt;                    // heads side by side
+    const bool mine = t < tn && rest / p.tt < step;
     float2 w[8];
-    if (h0 < rotated) {
+    float lo[8], hi[8];
+    const X* src;
+    Y* dst;
+    auto fetch = [&](int h) {
+      if (!mine || h >= h1) return;
+      rows(h, t, src, dst);
+      r_get8(src + ch * 8, lo);
+      r_get8(src + half + ch * 8, hi);
+    };
+    int h = h0 + rest / p.tt;
+    fetch(h);                                                         // on its way while the angles are formed
+    if (h0 < rotated) { angles(); __syncthreads(); }
+    if (h0 < rotated && mine) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) w[e] = cs[t * half + ch * 8 + e];
     }
-#pragma unroll 2
-    for (int h = first; h < h1; h += step) {
-      const X* src;
-      Y* dst;
-      rows(h, t, src, dst);
-      float lo[8], hi[8];
-      r_get8(src + ch * 8, lo);
-      r_get8(src + half + ch * 8, hi);
+    for (; mine && h < h1; h += step) {
       if (h < rotated) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
@@ -112,8 +116,10 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_axes_kernel(const RopeParam
       }
       r_put8(dst + ch * 8, lo);
       r_put8(dst + half + ch * 8, hi);
+      fetch(h + step);
     }
   } else {
+    if (h0 < rotated) { angles(); __syncthreads(); }
     const int per_head = tn * half;
     for (int i = threadIdx.x; i < (h1 - h0) * per_head; i += ROPE_THREADS) {
       const int h = h0 + i / per_head, r = i % per_head, t = r / half, ch = r % half;
@@ -131,16 +137,18 @@ __global__ void __launch_bounds__(ROPE_THREADS) rope_axes_kernel(const RopeParam
 
 template <typename X, typename Y, bool BACK>
 static int rope_launch(RopeParams& p, cudaStream_t st) {
-  // tokens of a block: as many as its threads cover side by side (a power of two, at most 32 and no more than there are)
-  const int side = p.vec ? ROPE_THREADS / (p.D / 16) : 4;
+  // Tokens of a block: a quarter of what its threads cover side by side, so that four heads are under way at a time (a power
+  // of two, no more than there are).  Measured at 32768 tokens, 72 heads of 128: 214 us with 8 tokens, 222 with 32 (one
+  // head), 246 with 2;  2 x 4001 tokens, 14 heads of 64: 13.0 with 16, 16.2 with 32.
+  const int side = p.vec ? ROPE_THREADS / 4 / (p.D / 16) : 4;
   p.tt = 1;
-  while (p.tt * 2 <= side && p.tt < 32 && p.tt < p.T) p.tt *= 2;
+  while (p.tt * 2 <= side && p.tt < p.T) p.tt *= 2;
   const long long tiles = (long long)p.B * ((p.T + p.tt - 1) / p.tt);
   NSA_REQUIRE(tiles < 2147483647LL, NSA_ERR_ARG, "rope_axes: %d x %d tokens do not fit a grid", p.B, p.T);
   const int all = p.heads[0] + p.heads[1] + p.heads[2];
-  // few tokens: the heads are spread over blocks until every SM has several; a block's angles are formed anew in each
-  long long ways = (8LL * sm_count() + tiles - 1) / tiles;
-  if (ways > all) ways = all;
+  // few tokens: the heads are spread over blocks until every SM has two; a block's angles are formed anew in each
+  long long ways = (2LL * sm_count() + tiles - 1) / tiles;
+  if (ways > (all + 3) / 4) ways = (all + 3) / 4;
   p.per_block = (int)((all + ways - 1) / ways);
   const dim3 grid((unsigned)tiles, (unsigned)((all + p.per_block - 1) / p.per_block));
   const size_t smem = (size_t)p.tt * (p.D / 2) * sizeof(float2);
