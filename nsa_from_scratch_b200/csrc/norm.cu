@@ -291,28 +291,24 @@ template <typename T> struct Raw {
   }
 };
 
-// A block walks the rows b, b + grid, ...; its share of dw stays in registers and is written once.  The next row is on its
-// way while this one is summed: with one or two blocks an SM, nothing else hides the loads.
-template <typename X, typename R, int V, bool DH>
-__global__ void __launch_bounds__(V == 1 ? 128 : 512) rms_norm_bwd_kernel(const NormBwdParams p) {
+// A block walks the rows b, b + grid, ...; its share of dw stays in registers and is written once.  A row stays as it was
+// stored (raw) across the barrier of its sum and is unpacked twice: with 64 registers a thread, 1024 threads an SM, so
+// that some rows are on their way while others are summed.
+template <typename X, typename R, int V, bool DH, int T_MAX>
+__global__ void __launch_bounds__(T_MAX, 1024 / T_MAX) rms_norm_bwd_kernel(const NormBwdParams p) {
   __shared__ float part[2][32];
   const int vecs = p.N / 8, T = blockDim.x;
-  float w[V][8], dw[V][8];
+  float dw[V][8];
 #pragma unroll
-  for (int v = 0; v < V; ++v) {
+  for (int v = 0; v < V; ++v)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) w[v][i] = dw[v][i] = 0.f;
-    const int c = threadIdx.x + v * T;
-    if (V < 4 && c < vecs) weight8(p.w, p.wdt, c * 8, w[v]);
-  }
+    for (int i = 0; i < 8; ++i) dw[v][i] = 0.f;
   const float inv_n = 1.f / (float)p.N;
-  Raw<X> ry[V];
-  Raw<R> rh[V], rd[V];
-  float rr = 0.f;
-  auto fetch = [&](long long row) {
-    if (row >= p.rows) return;
-    rr = p.rstd[row];
+  int turn = 0;
+  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
     const long long base = row * p.N;
+    Raw<X> ry[V];
+    Raw<R> rh[V], rd[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = threadIdx.x + v * T;
@@ -322,51 +318,42 @@ __global__ void __launch_bounds__(V == 1 ? 128 : 512) rms_norm_bwd_kernel(const 
         if constexpr (DH) rd[v].load(reinterpret_cast<const R*>(p.dh) + base + c * 8);
       }
     }
-  };
-  constexpr bool AHEAD = V < 4;                             // with 4 vectors the next row and the weights do not fit the registers
-  if (AHEAD) fetch(blockIdx.x);
-  int turn = 0;
-  for (long long row = blockIdx.x; row < p.rows; row += gridDim.x, turn ^= 1) {
-    if (!AHEAD) fetch(row);
-    const long long base = row * p.N;
-    const float r = rr;
-    float u[V][8], n[V][8];
-    Raw<R> d[V];
+    const float r = p.rstd[row];
     float dot = 0.f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = threadIdx.x + v * T;
       if (c < vecs) {
-        ry[v].get(u[v]);
-        rh[v].get(n[v]);
-        if constexpr (DH) d[v] = rd[v];
-        if (!AHEAD) weight8(p.w, p.wdt, c * 8, w[v]);
+        float u[8], n[8], w[8];
+        weight8(p.w, p.wdt, c * 8, w);
+        ry[v].get(u);
+        rh[v].get(n);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-          n[v][i] *= r;
-          dw[v][i] = fmaf(u[v][i], n[v][i], dw[v][i]);
-          u[v][i] *= w[v][i];
-          dot = fmaf(u[v][i], n[v][i], dot);
+          n[i] *= r;
+          dw[v][i] = fmaf(u[i], n[i], dw[v][i]);
+          dot = fmaf(u[i] * w[i], n[i], dot);
         }
       }
     }
-    if (AHEAD) fetch(row + gridDim.x);
     dot = block_sum(dot, part[turn]) * inv_n;               // two sets of slots: a row's are read while the next one's are written
 #pragma unroll
     for (int v = 0; v < V; ++v) {
       const int c = threadIdx.x + v * T;
       if (c < vecs) {
-        float g[8];
+        float u[8], n[8], w[8];
+        weight8(p.w, p.wdt, c * 8, w);
+        ry[v].get(u);
+        rh[v].get(n);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) g[i] = r * (u[v][i] - n[v][i] * dot);
+        for (int i = 0; i < 8; ++i) u[i] = r * (u[i] * w[i] - n[i] * r * dot);
         if constexpr (DH) {
-          float e[8];
-          d[v].get(e);
+          rd[v].get(n);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) g[i] += e[i];
+          for (int i = 0; i < 8; ++i) u[i] += n[i];
         }
-        put8(reinterpret_cast<X*>(p.dx), base + c * 8, g);
-        if (p.dres != nullptr) put8(reinterpret_cast<R*>(p.dres), base + c * 8, g);
+        put8(reinterpret_cast<X*>(p.dx), base + c * 8, u);
+        if (p.dres != nullptr) put8(reinterpret_cast<R*>(p.dres), base + c * 8, u);
       }
     }
   }
@@ -431,12 +418,12 @@ int column_sum(const float* part, void* out, int parts, int N, int dt, cudaStrea
   return launch_status("column_sum");
 }
 
-// Backward: 2 vectors a thread up to 8192 columns, else 4 (the weights and the sums of dw take 16 registers a vector).
-// Blocks: about 512 threads an SM, and no more, since each block leaves a row of partial sums.
-static int bwd_vectors_for(int N) { return N <= 1024 ? 1 : N <= 8192 ? 2 : 4; }
+// Backward: 2 vectors a thread from 2048 columns on, 4 from 8200 on; blocks for 1024 threads an SM, and no more, since each
+// leaves a row of partial sums.
+static int bwd_vectors_for(int N) { return N < 2048 ? 1 : N <= 8192 ? 2 : 4; }
 static int norm_bwd_blocks(long long rows, int N) {
   const int T = threads_for(N, bwd_vectors_for(N));
-  const long long want = (long long)sm_count() * (T >= 512 ? 1 : 512 / T);
+  const long long want = (long long)sm_count() * (T >= 512 ? 2 : 1024 / T);
   return (int)(rows < want ? rows : want);
 }
 long long rms_norm_bwd_ws_bytes(long long rows, int N) { return (long long)norm_bwd_blocks(rows, N) * N * 4; }
@@ -447,9 +434,10 @@ static int norm_bwd_launch(const NormBwdParams& p, int blocks, cudaStream_t st) 
   if (!vec) rms_norm_bwd_any_kernel<X, R><<<blocks, 256, 0, st>>>(p);
   else {
     const int V = bwd_vectors_for(p.N), T = threads_for(p.N, V);
-    if (V == 1) rms_norm_bwd_kernel<X, R, 1, DH><<<blocks, T, 0, st>>>(p);
-    else if (V == 2) rms_norm_bwd_kernel<X, R, 2, DH><<<blocks, T, 0, st>>>(p);
-    else rms_norm_bwd_kernel<X, R, 4, DH><<<blocks, T, 0, st>>>(p);
+    if (V == 1) rms_norm_bwd_kernel<X, R, 1, DH, 256><<<blocks, T, 0, st>>>(p);
+    else if (V == 2 && T <= 256) rms_norm_bwd_kernel<X, R, 2, DH, 256><<<blocks, T, 0, st>>>(p);
+    else if (V == 2) rms_norm_bwd_kernel<X, R, 2, DH, 512><<<blocks, T, 0, st>>>(p);
+    else rms_norm_bwd_kernel<X, R, 4, DH, 512><<<blocks, T, 0, st>>>(p);
   }
   return launch_status("rms_norm_bwd");
 }
