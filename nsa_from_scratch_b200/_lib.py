@@ -276,5 +276,16 @@ def on_device(t):
     return _NO_GUARD if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
 
 
+def call(fn, args, index: int, what: str) -> None:
+    """fn(&args, current stream) on device `index`, checked: the short way for calls whose host time counts."""
+    if index == torch._C._cuda_getDevice():
+        rc = fn(C.byref(args), torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(C.byref(args), torch._C._cuda_getCurrentRawStream(index))
+    if rc != OK:
+        check(rc, what)
+
+
 def ptr(t) -> int:
     return 0 if t is None else t.data_ptr()

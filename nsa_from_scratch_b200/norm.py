@@ -66,8 +66,7 @@ def _forward(plan: bytes, x: Tensor, weight: Tensor, residual: Optional[Tensor],
     if want_rstd:
         rstd = x.new_empty(a.rows, dtype=torch.float32)
         a.rstd = rstd.data_ptr()
-    with L.on_device(x):
-        L.check(L.load().nsa_rms_norm(C.byref(a), L.stream_ptr()), "nsa_rms_norm")
+    L.call(L.load().nsa_rms_norm, a, x.get_device(), "nsa_rms_norm")
     return h, rstd
 
 
@@ -82,23 +81,23 @@ class _RmsNormFn(torch.autograd.Function):
         return y if h is None else (y, h)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @ops.first_order
     def backward(ctx, dy, dh=None):
         h, weight, rstd = ctx.saved_tensors
         dy = torch.zeros(h.shape, device=h.device, dtype=ctx.x_dtype) if dy is None else dy.contiguous()
         dh = None if dh is None else dh.contiguous()
         N = h.shape[-1]
         rows = h.numel() // N
-        dx = torch.empty(h.shape, device=h.device, dtype=ctx.x_dtype)
+        dx = torch.empty_like(dy)
         dres = torch.empty_like(h) if ctx.stream and h.dtype != ctx.x_dtype else None
         dw = torch.empty_like(weight) if ctx.needs_input_grad[2] else None
         lib = L.load()
         with L.on_device(h):
-            need = int(lib.nsa_rms_norm_bwd_ws_bytes(rows, N))
-            ws = torch.empty(max(need, 1), device=h.device, dtype=torch.uint8)
-            a = L.NormBwdArgs(dy.data_ptr(), L.ptr(dh), h.data_ptr(), weight.data_ptr(), rstd.data_ptr(), dx.data_ptr(), L.ptr(dres), L.ptr(dw),
-                              ws.data_ptr(), need, rows, N, L.dtype_code(ctx.x_dtype), L.dtype_code(h.dtype), L.dtype_code(weight.dtype))
-            L.check(lib.nsa_rms_norm_bwd(C.byref(a), L.stream_ptr()), "nsa_rms_norm_bwd")
+            need = lib.nsa_rms_norm_bwd_ws_bytes(rows, N)
+        ws = h.new_empty(need, dtype=torch.uint8)
+        a = L.NormBwdArgs(dy.data_ptr(), L.ptr(dh), h.data_ptr(), weight.data_ptr(), rstd.data_ptr(), dx.data_ptr(), L.ptr(dres), L.ptr(dw),
+                          ws.data_ptr(), need, rows, N, L.dtype_code(ctx.x_dtype), L.dtype_code(h.dtype), L.dtype_code(weight.dtype))
+        L.call(lib.nsa_rms_norm_bwd, a, h.get_device(), "nsa_rms_norm_bwd")
         # the same values reach x and the residual
         return dx, (dx if dres is None else dres) if ctx.stream else None, dw, None
 

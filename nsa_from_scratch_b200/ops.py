@@ -99,6 +99,17 @@ def activation_code(name: Optional[str]) -> int:
         raise ValueError(f"unknown activation: {name}") from None
 
 
+def first_order(backward):
+    """A Function's backward that runs its kernels outside autograd, as once_differentiable does: its results refuse a second
+    differentiation.  That costs several microseconds, which only a caller who keeps the graph (create_graph) pays."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
+
+    return run
+
+
 class Plans(dict):
     """What an entry point found out about operands of given shapes, types and devices (never about their addresses or
     values): checked once, then an argument struct without pointers.  A program meets few; one that meets many starts over."""

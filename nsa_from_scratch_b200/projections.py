@@ -20,14 +20,17 @@ from . import ops
 
 def _run(a, ws_bytes, call, what: str, like: Tensor) -> None:
     """One library call with the workspace that it asks for; every pointer of `a` is set."""
-    with L.on_device(like):
-        need = ws_bytes(C.byref(a))
-        if need:
-            if need < 0:
-                L.check(int(need), what)
-            ws = like.new_empty(need, dtype=torch.uint8)
-            a.ws, a.ws_bytes = ws.data_ptr(), need
-        L.check(call(C.byref(a), L.stream_ptr()), what)
+    index = like.get_device()
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return _run(a, ws_bytes, call, what, like)
+    need = ws_bytes(C.byref(a))
+    if need:
+        if need < 0:
+            L.check(int(need), what)
+        ws = like.new_empty(need, dtype=torch.uint8)
+        a.ws, a.ws_bytes = ws.data_ptr(), need
+    L.call(call, a, index, what)
 
 
 def _check_rows(t: Optional[Tensor], name: str, shape, dtype, what: str) -> None:
@@ -70,7 +73,7 @@ class _LinearFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @ops.first_order
     def backward(ctx, dy):
         x, w, slope = ctx.saved_tensors
         dy = dy.contiguous()
@@ -173,7 +176,7 @@ class _GatedMlpFn(torch.autograd.Function):
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @ops.first_order
     def backward(ctx, dy):
         x, wg, wu, wd, *kept = ctx.saved_tensors
         dy = dy.contiguous()

@@ -77,8 +77,7 @@ def _launch(plan: bytes, src, dst, positions: Tensor, inv_freq: Tensor, backward
     a.q, a.k, a.v = src[0].data_ptr(), src[1].data_ptr(), src[2].data_ptr()
     a.q_out, a.k_out, a.v_out = dst[0].data_ptr(), dst[1].data_ptr(), dst[2].data_ptr()
     a.positions, a.inv_freq, a.backward = positions.data_ptr(), inv_freq.data_ptr(), backward
-    with L.on_device(positions):
-        L.check(L.load().nsa_rope_axes(C.byref(a), L.stream_ptr()), "nsa_rope_axes")
+    L.call(L.load().nsa_rope_axes, a, positions.get_device(), "nsa_rope_axes")
 
 
 def _forward(plan, q, k, v, positions, inv_freq, dtype):
@@ -97,7 +96,7 @@ class _RopeAxesFn(torch.autograd.Function):
         return _forward(plan, q, k, v, positions, inv_freq, dtype)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @ops.first_order
     def backward(ctx, dq, dk, dv):
         B, H, T, D = dq.shape
         kv = (B, T, dk.shape[1], D)
