@@ -18,28 +18,30 @@ enum {
   EPI_GLU_BWD = 2   // acc = dh: y = dg = dh * i1, o1 = du = dh * i0, with i0 = act(g) and i1 = act'(g) * u from the forward
 };
 
-// p = act(z), d = act'(z).  exp overflows to infinity for large -z and the quotient is then 0, as it should be.
-__device__ __forceinline__ float sigmoid_f(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
-__device__ __forceinline__ float tanh_f(float z) { return 1.f - __fdividef(2.f, 1.f + __expf(2.f * z)); }
-constexpr float kGeluC = 0.7978845608028654f;   // sqrt(2 / pi)
-constexpr float kGeluA = 0.044715f;             // the cubic's coefficient in gelu's tanh form
-
+// p = act(z), d = act'(z).  Both activations go through s = 1 / (1 + 2^e), e negative multiples of their argument; 2^e
+// overflows to infinity for large negative z, and s is then 0, as it should be.
+//   silu: s = sigmoid(z), p = z s, d = s + p (1 - s)
+//   gelu in its tanh form: 0.5 (1 + tanh(u)) = sigmoid(2 u), u = sqrt(2/pi) (z + 0.044715 z^3), so
+//         s = sigmoid(2 u), p = z s, d = s + p (1 - s) 2 u'(z):  10 operations (through tanh: about 40)
+__device__ __forceinline__ float rcp_f(float x) { float y; asm("rcp.approx.ftz.f32 %0, %1;\n" : "=f"(y) : "f"(x)); return y; }
+constexpr float kGelu1 = 1.5957691216057308f;                 // 2 sqrt(2 / pi)
+constexpr float kGelu3 = kGelu1 * 0.044715f;
 template <int ACT> __device__ __forceinline__ float act_one(float z) {
-  if (ACT == ACT_SILU) return z * sigmoid_f(z);
-  if (ACT == ACT_GELU_TANH) return 0.5f * z * (1.f + tanh_f(kGeluC * (z + kGeluA * z * z * z)));
-  if (ACT == ACT_RELU) return z < 0.f ? 0.f : z;          // a comparison that NaN fails keeps NaN
+  if (ACT == ACT_SILU) return z * rcp_f(1.f + ex2(z * -kLog2e));
+  if (ACT == ACT_GELU_TANH) return z * rcp_f(1.f + ex2(z * fmaf(z * z, -kGelu3 * kLog2e, -kGelu1 * kLog2e)));
+  if (ACT == ACT_RELU) return z < 0.f ? 0.f : z;              // a comparison that NaN fails keeps NaN
   return z;
 }
 template <int ACT> __device__ __forceinline__ void act_one_both(float z, float& p, float& d) {
   if (ACT == ACT_SILU) {
-    const float s = sigmoid_f(z);
+    const float s = rcp_f(1.f + ex2(z * -kLog2e));
     p = z * s;
-    d = s == 1.f ? 1.f : fmaf(p, 1.f - s, s);             // z = inf: slope 1, not inf * 0
+    d = s + fmaf(-p, s, p);
   } else if (ACT == ACT_GELU_TANH) {
-    const float t = tanh_f(kGeluC * (z + kGeluA * z * z * z));
-    p = 0.5f * z * (1.f + t);
-    const float q = 1.f - t * t;
-    d = 0.5f * (1.f + t) + (q == 0.f ? 0.f : 0.5f * z * q * kGeluC * (1.f + 3.f * kGeluA * z * z));
+    const float q = fminf(z * z, 1e30f);                      // finite: times (1 - s) = 0 it has to vanish
+    const float s = rcp_f(1.f + ex2(z * fmaf(q, -kGelu3 * kLog2e, -kGelu1 * kLog2e)));
+    p = z * s;
+    d = fmaf(fmaf(-p, s, p), fmaf(q, 3.f * kGelu3, kGelu1), s);
   } else if (ACT == ACT_RELU) {
     p = z < 0.f ? 0.f : z;
     d = z > 0.f ? 1.f : 0.f;

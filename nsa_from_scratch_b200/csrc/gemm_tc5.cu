@@ -98,6 +98,13 @@ __device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t
 }
 
 // ---------------------------------------------------------------- 16 columns of a row
+// Until here the loads behind v (and u) may still be under way: naming the registers keeps their uses behind the wait.
+__device__ __forceinline__ void wait_loaded(uint32_t (&v)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;\n"
+               : "+r"(v[0]), "+r"(v[1]), "+r"(v[2]), "+r"(v[3]), "+r"(v[4]), "+r"(v[5]), "+r"(v[6]), "+r"(v[7]), "+r"(v[8]), "+r"(v[9]), "+r"(v[10]),
+                 "+r"(v[11]), "+r"(v[12]), "+r"(v[13]), "+r"(v[14]), "+r"(v[15])
+               :: "memory");
+}
 template <typename T> __device__ __forceinline__ void put16(uint32_t p0, uint32_t p1, const float (&a)[16]) {
   sts128(p0, make_uint4(Elem<T>::pack(a[0], a[1]), Elem<T>::pack(a[2], a[3]), Elem<T>::pack(a[4], a[5]), Elem<T>::pack(a[6], a[7])));
   sts128(p1, make_uint4(Elem<T>::pack(a[8], a[9]), Elem<T>::pack(a[10], a[11]), Elem<T>::pack(a[12], a[13]), Elem<T>::pack(a[14], a[15])));
@@ -361,6 +368,13 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
         }
         drained();
       } else {
+        // the next 16 columns leave TMEM while these are worked on
+        uint32_t v[16], u[MODE == EPI_GLU ? 16 : 1];
+        auto load = [&](int col) {
+          tmem_ld16(acc + col, v);
+          if constexpr (MODE == EPI_GLU) tmem_ld16(acc + NW + col, u);
+        };
+        load(0);
 #pragma unroll 1
         for (int c = 0; c < NC; ++c, ++cnt) {
           const int st = cnt & 1;
@@ -376,37 +390,41 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
 #pragma unroll 1
           for (int h = 0; h < CW / 16; ++h) {
             const int col = c * CW + h * 16;
-            float a[16];
-            {
-              uint32_t v[16];
-              tmem_ld16(acc + col, v);
-              if constexpr (MODE == EPI_GLU) {
-                uint32_t u[16];
-                tmem_ld16(acc + NW + col, u);
-                tc_wait_ld();
-                float d[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) a[i] = __uint_as_float(v[i]);
-                if (p.e.o1 != nullptr) {
-                  act_all_both(a, d, p.e.act);
-#pragma unroll
-                  for (int i = 0; i < 16; ++i) d[i] *= __uint_as_float(u[i]);
-                  put16<T>(piece(box + BOX, 2 * h), piece(box + BOX, 2 * h + 1), a);
-                  put16<T>(piece(box + 2 * BOX, 2 * h), piece(box + 2 * BOX, 2 * h + 1), d);
-                } else {
-                  act_all(a, p.e.act);
-                }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) a[i] *= __uint_as_float(u[i]);
-              } else {
-                tc_wait_ld();
-#pragma unroll
-                for (int i = 0; i < 16; ++i) a[i] = __uint_as_float(v[i]);
-              }
-            }
+            float a[16], b[MODE == EPI_GLU ? 16 : 1];
             const uint32_t p0 = piece(box, 2 * h), p1 = piece(box, 2 * h + 1);
+            const int gc = nc0 + col;                                    // columns come in eights: N is a multiple of 8
+            uint4 bias[2] = {}, res[2] = {};                             // asked for ahead of the sums
             if constexpr (LIN) {
-              const int gc = nc0 + col;                                  // columns come in eights: N is a multiple of 8
+              if (p.e.bias != nullptr) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                  if (gc + 8 * i < N) bias[i] = *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.e.bias) + gc + 8 * i);
+              }
+              if (p.e.residual != nullptr) { res[0] = lds128(p0); res[1] = lds128(p1); }
+            }
+            wait_loaded(v);
+            if constexpr (MODE == EPI_GLU) wait_loaded(u);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              a[i] = __uint_as_float(v[i]);
+              if constexpr (MODE == EPI_GLU) b[i] = __uint_as_float(u[i]);
+            }
+            if (col + 16 < GW) load(col + 16);
+            if constexpr (MODE == EPI_GLU) {
+              if (p.e.o1 != nullptr) {
+                float d[16];
+                act_all_both(a, d, p.e.act);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) d[i] *= b[i];
+                put16<T>(piece(box + BOX, 2 * h), piece(box + BOX, 2 * h + 1), a);
+                put16<T>(piece(box + 2 * BOX, 2 * h), piece(box + 2 * BOX, 2 * h + 1), d);
+              } else {
+                act_all(a, p.e.act);
+              }
+#pragma unroll
+              for (int i = 0; i < 16; ++i) a[i] *= b[i];
+            }
+            if constexpr (LIN) {
               if (p.e.xs != nullptr) {
 #pragma unroll
                 for (int i = 0; i < 16; i += 4)
@@ -415,11 +433,7 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
                     a[i] *= xs * f.x; a[i + 1] *= xs * f.y; a[i + 2] *= xs * f.z; a[i + 3] *= xs * f.w;
                   }
               }
-              if (p.e.bias != nullptr) {
-#pragma unroll
-                for (int i = 0; i < 16; i += 8)
-                  if (gc + i < N) add8<T>(a + i, *reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.e.bias) + gc + i));
-              }
+              if (p.e.bias != nullptr) { add8<T>(a, bias[0]); add8<T>(a + 8, bias[1]); }
               if constexpr (MODE == EPI_SLOPE) {
                 float d[16];
                 act_all_both(a, d, p.e.act);
@@ -427,7 +441,7 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
               } else {
                 act_all(a, p.e.act);
               }
-              if (p.e.residual != nullptr) { add8<T>(a, lds128(p0)); add8<T>(a + 8, lds128(p1)); }
+              if (p.e.residual != nullptr) { add8<T>(a, res[0]); add8<T>(a + 8, res[1]); }
             } else if constexpr (MODE == EPI_GLU_BWD) {
               float d[16];
               get16<T>(p0, p1, d);

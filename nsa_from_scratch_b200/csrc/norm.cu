@@ -392,29 +392,32 @@ __global__ void __launch_bounds__(256) rms_norm_bwd_any_kernel(const NormBwdPara
   }
 }
 
-// out[c] = sum over `parts` rows of part[.][c]: 32 columns a block, 8 rows at a time, joined in a fixed order
-__global__ void __launch_bounds__(256) column_sum_kernel(const float* __restrict__ part, void* __restrict__ out, int parts, int N, int dt) {
-  __shared__ float s[8][33];
-  const int c = blockIdx.x * 32 + (threadIdx.x & 31), g = threadIdx.x >> 5;
-  float a0 = 0.f, a1 = 0.f;
+// out[c] = sum over `parts` rows of part[.][c]: 32 columns a block, 32 rows at a time, joined in a fixed order
+__global__ void __launch_bounds__(1024) column_sum_kernel(const float* __restrict__ part, void* __restrict__ out, int parts, int N, int dt) {
+  __shared__ float s[32][33];
+  const int lane = threadIdx.x & 31, c = blockIdx.x * 32 + lane, g = threadIdx.x >> 5;
+  float a[4] = {};
   if (c < N) {
     int r = g;
-    for (; r + 8 < parts; r += 16) { a0 += part[(long long)r * N + c]; a1 += part[(long long)(r + 8) * N + c]; }
-    if (r < parts) a0 += part[(long long)r * N + c];
-  }
-  s[g][threadIdx.x & 31] = a0 + a1;
-  __syncthreads();
-  if (g == 0 && c < N) {
-    float v = 0.f;
+    for (; r + 96 < parts; r += 128)
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v += s[i][threadIdx.x];
-    if (dt == NSA_FP32) reinterpret_cast<float*>(out)[c] = v;
-    else if (dt == NSA_FP16) reinterpret_cast<__half*>(out)[c] = __float2half_rn(v);
-    else reinterpret_cast<__nv_bfloat16*>(out)[c] = __float2bfloat16_rn(v);
+      for (int i = 0; i < 4; ++i) a[i] += part[(long long)(r + 32 * i) * N + c];
+    for (; r < parts; r += 32) a[0] += part[(long long)r * N + c];
+  }
+  s[g][lane] = (a[0] + a[1]) + (a[2] + a[3]);
+  __syncthreads();
+  float v = s[lane][g];                                     // warp g: column g, a row group a lane
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+  const int col = blockIdx.x * 32 + g;
+  if (lane == 0 && col < N) {
+    if (dt == NSA_FP32) reinterpret_cast<float*>(out)[col] = v;
+    else if (dt == NSA_FP16) reinterpret_cast<__half*>(out)[col] = __float2half_rn(v);
+    else reinterpret_cast<__nv_bfloat16*>(out)[col] = __float2bfloat16_rn(v);
   }
 }
 int column_sum(const float* part, void* out, int parts, int N, int dt, cudaStream_t st) {
-  column_sum_kernel<<<(N + 31) / 32, 256, 0, st>>>(part, out, parts, N, dt);
+  column_sum_kernel<<<(N + 31) / 32, 1024, 0, st>>>(part, out, parts, N, dt);
   return launch_status("column_sum");
 }
 
