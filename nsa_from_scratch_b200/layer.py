@@ -10,17 +10,26 @@ to head-major, five element-wise kernels of the rotary embedding, the bf16 casts
 the transpose back).  Here each of q, k, v is read once and written once by `nsa_rope_to_heads`
 (rotation in fp32, one rounding, head-major 16-bit result), the gate logits are read where they lie
 ([B,T,H,3]) and the kernel writes [B,T,H*D] directly.
+
+`NSABlock` is the decoder layer around it (the reference's Llama block, nsa/model/llama_dense.py:19-134 with the attention of
+nsa/model/llama_nsa.py:38-96), in 16 bits, for training, prefill and decoding: norm, projections, rotary embedding with any
+number of position axes, attention, output projection with the residual in its epilogue, norm with the residual's
+addition, gated feed-forward block with the residual in its epilogue.
 """
 from __future__ import annotations
 
-from typing import Optional
+from typing import Optional, Sequence
 
 import torch
 import torch.nn as nn
 from torch import Tensor
 
 from . import ops
+from .decode import KVCache, nsa_decode
 from .forward import _fused_forward, nsa_forward
+from .norm import rms_norm
+from .projections import gated_mlp, linear
+from .rotary import rope_axes_to_heads, rope_frequencies
 
 
 def rope_cache(seq_len: int, head_dim: int, base: float, device, dtype=torch.float32):
@@ -95,5 +104,72 @@ class NSAAttention(nn.Module):
                           gate_logits=gates.permute(0, 2, 1, 3).contiguous().to(kd)).to(x.dtype)
         return self.o_proj(out.transpose(1, 2).contiguous().view(B, T, H * D))
 
+    def attend(self, x: Tensor, positions: Tensor, inv_freq: Tensor, sections: Sequence[int], *, residual: Optional[Tensor] = None,
+               cache: Optional[KVCache] = None) -> Tensor:
+        """The module in bf16 or fp16 on the layer's own operators: x [B,T,hidden] -> [B,T,hidden] (+ residual, in the output
+        projection's epilogue).  positions [axes,B,T], inv_freq and sections as for `rope_axes_to_heads`.  With `cache`
+        (decoding, no gradients) the T positions are appended to it and attend everything it holds; else they attend each
+        other.  Differentiable without a cache; pool="learned" takes the inference routes only."""
+        B, T, _ = x.shape
+        H, Hkv, D = self.n_heads, self.n_kv_heads, self.head_dim
+        cfg = self.nsa_cfg
+        q = linear(x, self.q_proj.weight).view(B, T, H, D)
+        k = linear(x, self.k_proj.weight).view(B, T, Hkv, D)
+        v = linear(x, self.v_proj.weight).view(B, T, Hkv, D)
+        gates = linear(x, self.gate.weight).view(B, T, H, 3)
+        q, k, v = rope_axes_to_heads(q, k, v, positions, inv_freq, sections, dtype=x.dtype)
+        if cache is not None:
+            if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, gates)):
+                raise RuntimeError("NSAAttention.attend: a cached step has no gradients; call it under torch.no_grad()")
+            cache.append(k, v)
+            out = nsa_decode(q, cache, gate_logits=gates.permute(0, 2, 1, 3).contiguous()).transpose(1, 2).contiguous()
+        elif torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, gates)):
+            out = nsa_forward(q, k, v, cfg, gate_logits=gates.permute(0, 2, 1, 3).contiguous()).transpose(1, 2).contiguous()
+        else:
+            learned = getattr(cfg, "pool", "mean") == "learned"
+            scale = float(cfg.scale if cfg.scale is not None else D ** -0.5)
+            out = _fused_forward(q, k, v, cfg, scale, getattr(cfg, "stride_c", None), gates, None, 1.0, 1.0, 1.0, token_major=True,
+                                 pool_proj=(self.pool_proj_k, self.pool_proj_v) if learned else None)
+        return linear(out.view(B, T, H * D), self.o_proj.weight, residual=residual)
 
-__all__ = ["NSAAttention", "nsa_attention_token_major", "rope_cache"]
+
+class NSABlock(nn.Module):
+    """A decoder layer in bf16 or fp16: x + attention(norm(x)), then + feed-forward(norm(.)).  `rope_sections`: frequencies of
+    each position axis, head_dim / 2 in all (default: one axis)."""
+
+    def __init__(self, hidden_size: int, n_heads: int, head_dim: int, nsa_cfg, intermediate_size: int, n_kv_heads: Optional[int] = None, *,
+                 eps: float = 1e-6, activation: Optional[str] = "silu", rope_sections: Optional[Sequence[int]] = None, rope_base: float = 10000.0):
+        super().__init__()
+        self.attn = NSAAttention(hidden_size, n_heads, head_dim, nsa_cfg, n_kv_heads)
+        self.attn_norm = nn.Parameter(torch.ones(hidden_size))
+        self.mlp_norm = nn.Parameter(torch.ones(hidden_size))
+        self.gate_proj = nn.Linear(hidden_size, intermediate_size, bias=False)
+        self.up_proj = nn.Linear(hidden_size, intermediate_size, bias=False)
+        self.down_proj = nn.Linear(intermediate_size, hidden_size, bias=False)
+        self.eps, self.activation = eps, activation
+        self.rope_sections = tuple(rope_sections) if rope_sections is not None else (head_dim // 2,)
+        self.rope_base = rope_base
+        self._inv_freq: Optional[Tensor] = None              # fp64, and stays that when the module is cast
+
+    def new_cache(self, batch: int, max_len: int) -> KVCache:
+        a = self.attn
+        return KVCache(batch, a.n_kv_heads, a.head_dim, max_len, a.nsa_cfg, dtype=a.q_proj.weight.dtype, device=a.q_proj.weight.device)
+
+    def forward(self, x: Tensor, positions: Optional[Tensor] = None, *, cache: Optional[KVCache] = None) -> Tensor:
+        """x [B,T,hidden]; positions [axes,B,T] int32 or int64 (None, with one axis: 0..T-1, or the T positions behind what
+        `cache` holds).  cache (decoding, under torch.no_grad()): the step's keys and values are appended to it."""
+        B, T, _ = x.shape
+        if self._inv_freq is None or self._inv_freq.device != x.device:
+            self._inv_freq = rope_frequencies(self.attn.head_dim, self.rope_base, x.device)
+        if positions is None:
+            if len(self.rope_sections) != 1:
+                raise ValueError(f"NSABlock: {len(self.rope_sections)} position axes need positions")
+            start = 0 if cache is None else cache.length
+            positions = torch.arange(start, start + T, device=x.device).expand(1, B, T).contiguous()
+        h = rms_norm(x, self.attn_norm, eps=self.eps)
+        a = self.attn.attend(h, positions, self._inv_freq, self.rope_sections, cache=cache)
+        h, x = rms_norm(a, self.mlp_norm, residual=x, eps=self.eps)
+        return gated_mlp(h, self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight, activation=self.activation, residual=x)
+
+
+__all__ = ["NSAAttention", "NSABlock", "nsa_attention_token_major", "rope_cache"]
