@@ -143,7 +143,7 @@ struct GemmTcParams {
   int splits, per_split;                        // the steps of all segments, dealt out to `splits` tiles
 };
 
-// EPI_SLOPE: EPI_LINEAR that also writes act' (e.o1).  EPI_PARTIAL, EPI_PARTIAL2: raw sums of one product, of a gated pair,
+// EPI_SLOPE: EPI_LINEAR that also writes act', coded (e.o1).  EPI_PARTIAL, EPI_PARTIAL2: raw sums of one product, of a gated pair,
 // for the joining kernel.
 constexpr int EPI_SLOPE = 3, EPI_PARTIAL = 4, EPI_PARTIAL2 = 5;
 
@@ -437,7 +437,11 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
               if constexpr (MODE == EPI_SLOPE) {
                 float d[16];
                 act_all_both(a, d, p.e.act);
-                put16<T>(piece(box + BOX, 2 * h), piece(box + BOX, 2 * h + 1), d);
+                uint32_t q[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) q[i] = slope_code(d[2 * i]) | (slope_code(d[2 * i + 1]) << 16);
+                sts128(piece(box + BOX, 2 * h), make_uint4(q[0], q[1], q[2], q[3]));
+                sts128(piece(box + BOX, 2 * h + 1), make_uint4(q[4], q[5], q[6], q[7]));
               } else {
                 act_all(a, p.e.act);
               }

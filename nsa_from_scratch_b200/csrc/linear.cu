@@ -15,11 +15,11 @@ int sm_count() {
 }
 
 // ---------------------------------------------------------------- gradient through the activation, bias gradient
-// dz = dy * slope (slope = act'(z) from the forward; NULL: no activation, nothing is written) and the column sums of dz
+// dz = dy * act' (slope: coded by the forward; NULL: no activation, nothing is written) and the column sums of dz
 // (part: a row of partial sums per block row; NULL: not wanted).  A thread owns 8 columns and walks the rows of its
 // block row, four under way at a time; bound by HBM.
 template <typename T>
-__global__ void __launch_bounds__(128) act_bwd_kernel(const void* __restrict__ dy, const void* __restrict__ slope, void* __restrict__ dz,
+__global__ void __launch_bounds__(128) act_bwd_kernel(const void* __restrict__ dy, const uint16_t* __restrict__ slope, void* __restrict__ dz,
                                                       float* __restrict__ part, int M, int N, long long lddz, int rows, int vec, int vecz) {
   const int c = (blockIdx.x * 128 + threadIdx.x) * 8, n = N - c;
   if (n <= 0) return;
@@ -27,20 +27,30 @@ __global__ void __launch_bounds__(128) act_bwd_kernel(const void* __restrict__ d
   float sum[8] = {};
   constexpr int U = 4;
   for (int r = r0; r < r1; r += U) {
-    float d[U][8], v[U][8];
+    float d[U][8];
+    uint32_t v[U][4];
 #pragma unroll
     for (int q = 0; q < U; ++q) {
       if (r + q >= r1) break;
       const long long at = (long long)(r + q) * N + c;
       load8<T>(dy, at, n, vec, d[q]);
-      if (slope != nullptr) load8<T>(slope, at, n, vec, v[q]);
+      if (slope != nullptr) {
+        if (vec) {
+          const uint4 w = *reinterpret_cast<const uint4*>(slope + at);
+          v[q][0] = w.x; v[q][1] = w.y; v[q][2] = w.z; v[q][3] = w.w;
+        } else {
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            v[q][i] = (2 * i < n ? slope[at + 2 * i] : 0u) | ((2 * i + 1 < n ? (uint32_t)slope[at + 2 * i + 1] : 0u) << 16);
+        }
+      }
     }
 #pragma unroll
     for (int q = 0; q < U; ++q) {
       if (r + q >= r1) break;
       if (slope != nullptr) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) d[q][i] *= v[q][i];
+        for (int i = 0; i < 8; ++i) d[q][i] *= slope_value(v[q][i >> 1] >> (16 * (i & 1)));
         store8<T>(dz, (long long)(r + q) * lddz + c, n, vecz, d[q]);
       }
 #pragma unroll
@@ -69,8 +79,8 @@ static int act_bwd(const void* dy, const void* slope, void* dz, long long lddz, 
   const ActBwdPlan p = act_bwd_plan(M, N);
   const int vec = N % 8 == 0 && aligned16(dy) && aligned16(slope), vecz = lddz % 8 == 0;
   const dim3 grid(p.strips, p.groups);
-  if (dtype == NSA_BF16) act_bwd_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(dy, slope, dz, part, M, N, lddz, p.rows, vec, vecz);
-  else act_bwd_kernel<__half><<<grid, 128, 0, st>>>(dy, slope, dz, part, M, N, lddz, p.rows, vec, vecz);
+  if (dtype == NSA_BF16) act_bwd_kernel<__nv_bfloat16><<<grid, 128, 0, st>>>(dy, (const uint16_t*)slope, dz, part, M, N, lddz, p.rows, vec, vecz);
+  else act_bwd_kernel<__half><<<grid, 128, 0, st>>>(dy, (const uint16_t*)slope, dz, part, M, N, lddz, p.rows, vec, vecz);
   return launch_status("act_bwd");
 }
 

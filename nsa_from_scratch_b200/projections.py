@@ -58,7 +58,7 @@ def _linear(plan: bytes, x: Tensor, w: Tensor, bias, residual, xs, ws, dtype: to
         a.x_scale, a.w_scale = xs.data_ptr(), ws.data_ptr()
     slope = None
     if want_slope:
-        slope = torch.empty_like(y)
+        slope = torch.empty_like(y, dtype=torch.int16)
         a.slope = slope.data_ptr()
     lib = L.load()
     _run(a, lib.nsa_linear_ws_bytes, lib.nsa_linear, "nsa_linear", x)
@@ -94,7 +94,7 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, *, activati
            residual: Optional[Tensor] = None) -> Tensor:
     """act(x weight^T + bias) + residual.  x [..., K], weight [N, K], bias [N], residual [..., N], all bf16 or all fp16;
     activation None, "silu", "gelu_tanh" or "relu".  Returns [..., N] in x's dtype: fp32 sums and epilogue, one rounding.
-    Differentiable wrt x, weight, bias and residual (act' is kept in x's dtype for the backward)."""
+    Differentiable wrt x, weight, bias and residual (act' is kept in 16 bits of its own for the backward)."""
     key = ("linear", activation, *_meta(x, weight, bias, residual))
     plan = _plans.get(key)
     if plan is None:

@@ -311,7 +311,9 @@ def linear_backward_bounds(x, w, b, act, dy, dtype):
     s = slope64(z, act)
     serr = slope_error(z, zerr, act)
     if act is not None:
-        serr = (1 + half) * serr + half * s.abs() + tiny                        # act' is kept in 16 bits
+        # act' is kept as q |q| 2^-28: half a step of q is 2^-15, its square root good to 2^-20
+        root = (s.abs() + serr).sqrt()
+        serr = serr + 2 * root * (2.0 ** -15 + FN * root) + (2.0 ** -15 + FN * root) ** 2
     g = dy.double() * s
     gerr = (half * g.abs() + tiny) * (act is not None) + (1 + half) * dy.double().abs() * serr
     out = {}
