@@ -534,11 +534,11 @@ int nsa_linear_bwd(const nsa_linear_bwd_args* args, nsa_stream_t stream);
 
 /* Gated feed-forward block:  y = (act(x wg^T) * (x wu^T)) wd^T + residual,  x, residual, y [M,N], wg and wu [F,N], wd [N,F], all of
  * one 16-bit type.  The gated product h is held in that type between the two matrix products.  For the backward (all NULL: not
- * wanted): p = act(x wg^T), s = act'(x wg^T) * (x wu^T) and h, [M,Fp] in that type, Fp being F rounded up to a multiple of 8,
- * 16-byte aligned.  ws as for nsa_linear. */
+ * wanted), [M,Fp] of 16 bits each, Fp being F rounded up to a multiple of 8, 16-byte aligned: h; the upper halves of p =
+ * act(x wg^T) and s = act'(x wg^T) * (x wu^T) as fp32; low: their next 8 bits, p's in the lower byte.  ws as for nsa_linear. */
 typedef struct nsa_gated_mlp_args {
   const void *x, *wg, *wu, *wd, *residual;
-  void *y, *p, *s, *h, *ws;
+  void *y, *p, *s, *low, *h, *ws;
   int64_t ws_bytes;
   int32_t M, N, F;
   int32_t dtype, act;
@@ -548,7 +548,7 @@ int nsa_gated_mlp(const nsa_gated_mlp_args* args, nsa_stream_t stream);
 
 /* Its gradients, from what the forward kept: dx [M,N], dwg and dwu [F,N], dwd [N,F], each NULL if not wanted; residual's is dy.  Repeats bit for bit. */
 typedef struct nsa_gated_mlp_bwd_args {
-  const void *dy, *x, *wg, *wu, *wd, *p, *s, *h;
+  const void *dy, *x, *wg, *wu, *wd, *p, *s, *low, *h;
   void *dx, *dwg, *dwu, *dwd, *ws;
   int64_t ws_bytes;
   int32_t M, N, F;

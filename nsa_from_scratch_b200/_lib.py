@@ -153,7 +153,7 @@ class GatedMlpArgs(C.Structure):
     """Mirror of `struct nsa_gated_mlp_args`."""
     _fields_ = [
         ("x", C.c_void_p), ("wg", C.c_void_p), ("wu", C.c_void_p), ("wd", C.c_void_p), ("residual", C.c_void_p),
-        ("y", C.c_void_p), ("p", C.c_void_p), ("s", C.c_void_p), ("h", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_int64),
+        ("y", C.c_void_p), ("p", C.c_void_p), ("s", C.c_void_p), ("low", C.c_void_p), ("h", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_int64),
         ("M", C.c_int32), ("N", C.c_int32), ("F", C.c_int32), ("dtype", C.c_int32), ("act", C.c_int32),
     ]
 
@@ -161,7 +161,7 @@ class GatedMlpArgs(C.Structure):
 class GatedMlpBwdArgs(C.Structure):
     """Mirror of `struct nsa_gated_mlp_bwd_args`."""
     _fields_ = [
-        ("dy", C.c_void_p), ("x", C.c_void_p), ("wg", C.c_void_p), ("wu", C.c_void_p), ("wd", C.c_void_p), ("p", C.c_void_p), ("s", C.c_void_p), ("h", C.c_void_p),
+        ("dy", C.c_void_p), ("x", C.c_void_p), ("wg", C.c_void_p), ("wu", C.c_void_p), ("wd", C.c_void_p), ("p", C.c_void_p), ("s", C.c_void_p), ("low", C.c_void_p), ("h", C.c_void_p),
         ("dx", C.c_void_p), ("dwg", C.c_void_p), ("dwu", C.c_void_p), ("dwd", C.c_void_p), ("ws", C.c_void_p), ("ws_bytes", C.c_int64),
         ("M", C.c_int32), ("N", C.c_int32), ("F", C.c_int32), ("dtype", C.c_int32),
     ]

@@ -14,8 +14,8 @@ namespace nsa {
 enum { ACT_NONE = 0, ACT_SILU = 1, ACT_GELU_TANH = 2, ACT_RELU = 3 };
 enum {
   EPI_LINEAR = 0,   // v = acc * xs[m] * ws[n] + bias[n]; o1 = act'(v) (optional, coded); y = act(v) + residual
-  EPI_GLU = 1,      // two products g, u of the same A: y = act(g) * u; optional o1 = act(g), o2 = act'(g) * u
-  EPI_GLU_BWD = 2   // acc = dh: y = dg = dh * i1, o1 = du = dh * i0, with i0 = act(g) and i1 = act'(g) * u from the forward
+  EPI_GLU = 1,      // two products g, u of the same A: y = act(g) * u; optional o1, o2, o3: act(g) and act'(g) * u in 24 bits
+  EPI_GLU_BWD = 2   // acc = dh: y = dg = dh * act'(g) u, o1 = du = dh * act(g), from what the forward left (i0, i1, i2)
 };
 
 // p = act(z), d = act'(z).  Both activations go through s = 1 / (1 + 2^e), e negative multiples of their argument; 2^e
@@ -63,6 +63,14 @@ __device__ __forceinline__ float slope_value(uint32_t code) {
   return q * fabsf(q) * 3.7252902984619140625e-9f;             // 2^-28
 }
 
+// What a gated pair leaves for the backward, p = act(g) and s = act'(g) u: fp32 rounded to its upper 24 bits (2^-16), the upper
+// 16 in an array each, the next 8 of both in a third (p's in the lower byte).  Rounded to 16 bits they would add as much
+// error to the gradients as the roundings that cannot be had without; in fp32 they would take 8 bytes instead of 6.
+__device__ __forceinline__ uint32_t cut24(float v) { return __float_as_uint(v) + 0x80u; }      // infinities and NaN stay what they are
+__device__ __forceinline__ uint32_t low_bytes(uint32_t p, uint32_t s) { return ((p >> 8) & 0xffu) | (s & 0xff00u); }
+__device__ __forceinline__ float join24_p(uint32_t hi, uint32_t low) { return __uint_as_float((hi << 16) | ((low & 0xffu) << 8)); }
+__device__ __forceinline__ float join24_s(uint32_t hi, uint32_t low) { return __uint_as_float((hi << 16) | (low & 0xff00u)); }
+
 // Several at a time: the choice is made once, so that their chains of exp and division run side by side (chosen element by
 // element they ran one after the other: 111 against 93 us for the gated product of 8191 x 2816 x 1024).
 template <int ACT, int R> __device__ __forceinline__ void act_as(float (&a)[R]) {
@@ -89,13 +97,13 @@ template <int R> __device__ __forceinline__ void act_all_both(float (&a)[R], flo
 struct Epi {
   int mode, act;
   int M, N;                      // results are [M][N]
-  long long ldy;                 // elements between rows of y; in the gated modes of o1, o2, i0 and i1 too.  The rest is dense
+  long long ldy;                 // elements between rows of y; in the gated modes of the o's and i's too.  The rest is dense
   int vec;                       // 1: N % 8 == 0 and every 16-bit pointer to a dense matrix is 16-byte aligned
   int vecy;                      // 1: the same of ldy and what it goes with; columns N..ldy-1 of a padded row are then written
   const void *bias, *residual;   // EPI_LINEAR; out type; NULL: none
   const float *xs, *ws;          // EPI_LINEAR: scales per row and per column of the sums; NULL: none
-  const void *i0, *i1;           // EPI_GLU_BWD
-  void *y, *o1, *o2;             // o1 (LINEAR), o1 and o2 (GLU): NULL: not wanted
+  const void *i0, *i1, *i2;      // EPI_GLU_BWD
+  void *y, *o1, *o2, *o3;        // o1 (LINEAR), o1 to o3 (GLU): NULL: not wanted
 };
 
 // One product.  gemm_tc5: rows of A and B start on 16-byte boundaries.
@@ -171,23 +179,29 @@ __device__ __forceinline__ void epilogue8(const Epi& e, long long row, int col, 
   } else if constexpr (MODE == EPI_GLU) {
     if (e.o1 != nullptr) {
       act_all_both(a, v, e.act);
+      uint16_t *op = reinterpret_cast<uint16_t*>(e.o1) + ay, *os = reinterpret_cast<uint16_t*>(e.o2) + ay, *ol = reinterpret_cast<uint16_t*>(e.o3) + ay;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] *= b[i];
-      store8<T>(e.o1, ay, n, e.vecy, a);
-      store8<T>(e.o2, ay, n, e.vecy, v);
+      for (int i = 0; i < 8; ++i)
+        if (i < n) {
+          const uint32_t cp = cut24(a[i]), cs = cut24(v[i] * b[i]);
+          op[i] = (uint16_t)(cp >> 16);
+          os[i] = (uint16_t)(cs >> 16);
+          ol[i] = (uint16_t)low_bytes(cp, cs);
+        }
     } else {
       act_all(a, e.act);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) a[i] *= b[i];
   } else {
-    load8<T>(e.i0, ay, n, e.vecy, v);
+    const uint16_t *ip = reinterpret_cast<const uint16_t*>(e.i0) + ay, *is = reinterpret_cast<const uint16_t*>(e.i1) + ay,
+                   *il = reinterpret_cast<const uint16_t*>(e.i2) + ay;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= a[i];
+    for (int i = 0; i < 8; ++i) {
+      v[i] = i < n ? a[i] * join24_p(ip[i], il[i]) : 0.f;
+      a[i] = i < n ? a[i] * join24_s(is[i], il[i]) : 0.f;
+    }
     store8<T>(e.o1, ay, n, e.vecy, v);
-    load8<T>(e.i1, ay, n, e.vecy, v);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) a[i] *= v[i];
   }
   store8<T>(e.y, ay, n, e.vecy, a);
 }

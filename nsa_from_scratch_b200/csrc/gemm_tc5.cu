@@ -109,15 +109,6 @@ template <typename T> __device__ __forceinline__ void put16(uint32_t p0, uint32_
   sts128(p0, make_uint4(Elem<T>::pack(a[0], a[1]), Elem<T>::pack(a[2], a[3]), Elem<T>::pack(a[4], a[5]), Elem<T>::pack(a[6], a[7])));
   sts128(p1, make_uint4(Elem<T>::pack(a[8], a[9]), Elem<T>::pack(a[10], a[11]), Elem<T>::pack(a[12], a[13]), Elem<T>::pack(a[14], a[15])));
 }
-template <typename T> __device__ __forceinline__ void get16(uint32_t p0, uint32_t p1, float (&a)[16]) {
-  const uint4 u[2] = {lds128(p0), lds128(p1)};
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const uint32_t w[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) { const float2 f = Elem<T>::unpack(w[j]); a[8 * i + 2 * j] = f.x; a[8 * i + 2 * j + 1] = f.y; }
-  }
-}
 template <typename T> __device__ __forceinline__ void add8(float* a, const uint4& u) {
   const uint32_t w[4] = {u.x, u.y, u.z, u.w};
 #pragma unroll
@@ -135,7 +126,7 @@ struct TcProduct {
 constexpr int TC_PRODUCTS = 4;
 struct GemmTcParams {
   TcProduct pr[TC_PRODUCTS];
-  CUtensorMap tmO1, tmO2, tmI0, tmI1;           // further results and inputs of the epilogue (I0: residual in EPI_LINEAR); one product
+  CUtensorMap tmO1, tmO2, tmO3, tmI0, tmI1, tmI2;   // further results and inputs of the epilogue (I0: residual in EPI_LINEAR); one product
   Epi e;
   float* part;                                  // PARTIAL: [splits][products][M][ldp] fp32; one product
   int ldp;
@@ -147,16 +138,17 @@ struct GemmTcParams {
 // for the joining kernel.
 constexpr int EPI_SLOPE = 3, EPI_PARTIAL = 4, EPI_PARTIAL2 = 5;
 
-template <int CG, int BN> struct TcShape {
+template <int MODE, int CG, int BN> struct TcShape {
   static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / CG * 128;
-  static constexpr int STAGES = 5, EPI_BYTES = 32768;             // EPI_BYTES: of each of the two epilogue groups
+  // stages of the operands' ring, and bytes of each of the two epilogue groups (EPI_GLU_BWD: two stages of three boxes)
+  static constexpr int STAGES = MODE == EPI_GLU_BWD ? 4 : 5, EPI_BYTES = MODE == EPI_GLU_BWD ? 49152 : 32768;
   static constexpr int SMEM = STAGES * (A_BYTES + B_BYTES) + 2 * EPI_BYTES + 1024;
 };
 
 // F: 0 fp16, 1 bf16, 2 e4m3, 3 e5m2;  T: result type
 template <int F, typename T, int MODE, int CG, int BN>
 __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant__ GemmTcParams p) {
-  using S = TcShape<CG, BN>;
+  using S = TcShape<MODE, CG, BN>;
   constexpr bool F8 = F >= 2;
   constexpr int KE = F8 ? 128 : 64;                                  // elements of a 128-byte step
   constexpr bool PAIR = MODE == EPI_GLU || MODE == EPI_PARTIAL2;     // two products a tile
@@ -311,7 +303,7 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
     constexpr int CW = MODE == EPI_LINEAR ? 64 : 32;                     // columns of a chunk
     constexpr int NC = RAW ? 1 : GW / CW;
     constexpr int BOX = 128 * CW * 2;                                    // bytes of a box: 128 rows of CW columns
-    constexpr int STAGE = MODE == EPI_GLU ? 0 : 16384;                   // between the two stages (EPI_GLU: one stage of three boxes)
+    constexpr int STAGE = MODE == EPI_GLU ? 0 : S::EPI_BYTES / 2;        // between the two stages (EPI_GLU: one stage of four boxes)
     const uint32_t stage0 = s_tiles + S::STAGES * (S::A_BYTES + S::B_BYTES) + group * S::EPI_BYTES;
     constexpr bool LIN = MODE == EPI_LINEAR || MODE == EPI_SLOPE;
     const bool inputs = MODE == EPI_GLU_BWD || (LIN && p.e.residual != nullptr);
@@ -327,9 +319,12 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
       auto request = [&](int c, int count) {                             // lead only: the inputs of chunk c of this tile
         const int st = count & 1;
         const uint32_t bar = smem_u32(&loaded[group][st]), box = stage0 + st * STAGE;
-        mbar_expect_tx(bar, MODE == EPI_GLU_BWD ? 2 * BOX : BOX);
+        mbar_expect_tx(bar, MODE == EPI_GLU_BWD ? 3 * BOX : BOX);
         tma_load_2d<1>(box, &p.tmI0, bar, nc0 + c * CW, mr);
-        if constexpr (MODE == EPI_GLU_BWD) tma_load_2d<1>(box + BOX, &p.tmI1, bar, nc0 + c * CW, mr);
+        if constexpr (MODE == EPI_GLU_BWD) {
+          tma_load_2d<1>(box + BOX, &p.tmI1, bar, nc0 + c * CW, mr);
+          tma_load_2d<1>(box + 2 * BOX, &p.tmI2, bar, nc0 + c * CW, mr);
+        }
       };
       if (inputs && lead) {
         bulk_wait_read<0>();
@@ -415,9 +410,20 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
                 float d[16];
                 act_all_both(a, d, p.e.act);
 #pragma unroll
-                for (int i = 0; i < 16; ++i) d[i] *= b[i];
-                put16<T>(piece(box + BOX, 2 * h), piece(box + BOX, 2 * h + 1), a);
-                put16<T>(piece(box + 2 * BOX, 2 * h), piece(box + 2 * BOX, 2 * h + 1), d);
+                for (int j = 0; j < 2; ++j) {
+                  uint32_t hp[4], hs[4], lo[4];
+#pragma unroll
+                  for (int i = 0; i < 4; ++i) {
+                    const int k = 8 * j + 2 * i;
+                    const uint32_t p0 = cut24(a[k]), p1 = cut24(a[k + 1]), s0 = cut24(d[k] * b[k]), s1 = cut24(d[k + 1] * b[k + 1]);
+                    hp[i] = __byte_perm(p0, p1, 0x7632);
+                    hs[i] = __byte_perm(s0, s1, 0x7632);
+                    lo[i] = __byte_perm(__byte_perm(p0, s0, 0x0051), __byte_perm(p1, s1, 0x0051), 0x5410);
+                  }
+                  sts128(piece(box + BOX, 2 * h + j), make_uint4(hp[0], hp[1], hp[2], hp[3]));
+                  sts128(piece(box + 2 * BOX, 2 * h + j), make_uint4(hs[0], hs[1], hs[2], hs[3]));
+                  sts128(piece(box + 3 * BOX, 2 * h + j), make_uint4(lo[0], lo[1], lo[2], lo[3]));
+                }
               } else {
                 act_all(a, p.e.act);
               }
@@ -448,14 +454,22 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
               if (p.e.residual != nullptr) { add8<T>(a, res[0]); add8<T>(a + 8, res[1]); }
             } else if constexpr (MODE == EPI_GLU_BWD) {
               float d[16];
-              get16<T>(p0, p1, d);
 #pragma unroll
-              for (int i = 0; i < 16; ++i) d[i] *= a[i];
-              put16<T>(p0, p1, d);                                       // du, over act(g)
-              get16<T>(piece(box + BOX, 2 * h), piece(box + BOX, 2 * h + 1), d);
+              for (int j = 0; j < 2; ++j) {
+                const uint4 hp = lds128(piece(box, 2 * h + j)), hs = lds128(piece(box + BOX, 2 * h + j)), lo = lds128(piece(box + 2 * BOX, 2 * h + j));
+                const uint32_t wp[4] = {hp.x, hp.y, hp.z, hp.w}, ws[4] = {hs.x, hs.y, hs.z, hs.w}, wl[4] = {lo.x, lo.y, lo.z, lo.w};
 #pragma unroll
-              for (int i = 0; i < 16; ++i) a[i] *= d[i];
-              put16<T>(piece(box + BOX, 2 * h), piece(box + BOX, 2 * h + 1), a);      // dg, over act'(g) u
+                for (int i = 0; i < 4; ++i) {
+                  const int k = 8 * j + 2 * i;                           // an fp32's bytes: upper 16 bits, the low byte, nothing
+                  auto join = [](uint32_t hi, uint32_t low, uint32_t bytes) { return __uint_as_float(__byte_perm(hi, low, bytes) & 0xffffff00u); };
+                  d[k] = a[k] * join(wp[i], wl[i], 0x1044);
+                  d[k + 1] = a[k + 1] * join(wp[i], wl[i], 0x3266);
+                  a[k] *= join(ws[i], wl[i], 0x1055);
+                  a[k + 1] *= join(ws[i], wl[i], 0x3277);
+                }
+              }
+              put16<T>(p0, p1, d);                                       // du, over p
+              put16<T>(piece(box + BOX, 2 * h), piece(box + BOX, 2 * h + 1), a);      // dg, over s
             }
             if constexpr (MODE != EPI_GLU_BWD) put16<T>(p0, p1, a);
           }
@@ -471,7 +485,11 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
               tma_store_2d(&w.pr->tmY, box, gc, mr);
               if constexpr (MODE == EPI_SLOPE) tma_store_2d(&p.tmO1, box + BOX, gc, mr);
               if constexpr (MODE == EPI_GLU) {
-                if (p.e.o1 != nullptr) { tma_store_2d(&p.tmO1, box + BOX, gc, mr); tma_store_2d(&p.tmO2, box + 2 * BOX, gc, mr); }
+                if (p.e.o1 != nullptr) {
+                  tma_store_2d(&p.tmO1, box + BOX, gc, mr);
+                  tma_store_2d(&p.tmO2, box + 2 * BOX, gc, mr);
+                  tma_store_2d(&p.tmO3, box + 3 * BOX, gc, mr);
+                }
               }
             }
             bulk_commit();
@@ -596,7 +614,7 @@ long long gemm_tc5_ws_bytes(const GemmProblem& p) {
 
 template <int F, typename T, int MODE, int CG, int BN>
 static int tc_launch(const GemmTcParams& g, cudaStream_t st) {
-  using S = TcShape<CG, BN>;
+  using S = TcShape<MODE, CG, BN>;
   auto fn = gemm_tc5_kernel<F, T, MODE, CG, BN>;
   static bool prepared[64];                   // per device: the attribute outlasts the call, and setting it twice is harmless
   int dev = 0;
@@ -690,8 +708,10 @@ int gemm_tc5(const GemmProblem& p, void* ws, cudaStream_t st) {
     if ((rc = box(&g.pr[0].tmY, p.e.y, p.e.ldy)) != NSA_OK) return rc;
     if ((rc = box(&g.tmO1, p.e.o1, gated ? p.e.ldy : p.N)) != NSA_OK) return rc;
     if ((rc = box(&g.tmO2, p.e.o2, p.e.ldy)) != NSA_OK) return rc;
+    if ((rc = box(&g.tmO3, p.e.o3, p.e.ldy)) != NSA_OK) return rc;
     if ((rc = box(&g.tmI0, gated ? p.e.i0 : p.e.residual, gated ? p.e.ldy : p.N)) != NSA_OK) return rc;
     if ((rc = box(&g.tmI1, p.e.i1, p.e.ldy)) != NSA_OK) return rc;
+    if ((rc = box(&g.tmI2, p.e.i2, p.e.ldy)) != NSA_OK) return rc;
   }
   g.e = p.e;
   g.part = reinterpret_cast<float*>(ws);

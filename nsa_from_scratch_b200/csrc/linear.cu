@@ -300,7 +300,7 @@ static int mlp_steps(const nsa_gated_mlp_args& a, Arena& w) {
   p.B[1] = wu.p;
   p.e.mode = EPI_GLU;
   p.e.act = a.act;
-  p.e.y = h; p.e.o1 = a.p; p.e.o2 = a.s;
+  p.e.y = h; p.e.o1 = a.p; p.e.o2 = a.s; p.e.o3 = a.low;
   p.e.ldy = ldh; p.e.vec = p.e.vecy = 1;
   if (few) {
     if (!w.dry()) NSA_TRY(gemm_skinny(p, false, w.st));
@@ -322,8 +322,9 @@ int gated_mlp(const nsa_gated_mlp_args& a, cudaStream_t st) {
   NSA_TRY(check_mlp(a.M, a.N, a.F, a.dtype, a.act));
   if (a.M == 0) return NSA_OK;
   NSA_REQUIRE(a.x && a.wg && a.wu && a.wd && a.y, NSA_ERR_ARG, "gated_mlp: NULL pointer");
-  NSA_REQUIRE((a.p == nullptr) == (a.s == nullptr) && (a.p == nullptr) == (a.h == nullptr), NSA_ERR_ARG, "gated_mlp: give all of p, s and h or none");
-  NSA_REQUIRE(aligned16(a.p) && aligned16(a.s) && aligned16(a.h), NSA_ERR_ARG, "gated_mlp: p, s and h must be 16-byte aligned");
+  NSA_REQUIRE((a.p == nullptr) == (a.s == nullptr) && (a.p == nullptr) == (a.low == nullptr) && (a.p == nullptr) == (a.h == nullptr), NSA_ERR_ARG,
+              "gated_mlp: give all of p, s, low and h or none");
+  NSA_REQUIRE(aligned16(a.p) && aligned16(a.s) && aligned16(a.low) && aligned16(a.h), NSA_ERR_ARG, "gated_mlp: p, s, low and h must be 16-byte aligned");
   return run_steps("gated_mlp", a, mlp_steps, st);
 }
 
@@ -335,7 +336,7 @@ static int mlp_bwd_steps(const nsa_gated_mlp_bwd_args& a, Arena& w) {
   NSA_TRY(operand(w, a.wd, a.N, a.F, a.dtype, &wd));
   GemmProblem p = problem(dy, 0, wd, 1, a.M, a.F, a.N, a.dtype);                            // dh = dy wd
   p.e.mode = EPI_GLU_BWD;
-  p.e.i0 = a.p; p.e.i1 = a.s;
+  p.e.i0 = a.p; p.e.i1 = a.s; p.e.i2 = a.low;
   p.e.y = dg; p.e.o1 = du;
   p.e.ldy = ldh; p.e.vec = p.e.vecy = 1;
   NSA_TRY(gemm(w, p));
@@ -363,8 +364,8 @@ int gated_mlp_bwd(const nsa_gated_mlp_bwd_args& a, cudaStream_t st) {
     NSA_TRY(zero(a.dwu, bytes, st));
     return zero(a.dwd, bytes, st);
   }
-  NSA_REQUIRE(a.dy && a.x && a.wg && a.wu && a.wd && a.p && a.s && a.h, NSA_ERR_ARG, "gated_mlp backward: NULL pointer");
-  NSA_REQUIRE(aligned16(a.p) && aligned16(a.s) && aligned16(a.h), NSA_ERR_ARG, "gated_mlp backward: p, s and h must be 16-byte aligned");
+  NSA_REQUIRE(a.dy && a.x && a.wg && a.wu && a.wd && a.p && a.s && a.low && a.h, NSA_ERR_ARG, "gated_mlp backward: NULL pointer");
+  NSA_REQUIRE(aligned16(a.p) && aligned16(a.s) && aligned16(a.low) && aligned16(a.h), NSA_ERR_ARG, "gated_mlp backward: p, s, low and h must be 16-byte aligned");
   return run_steps("gated_mlp backward", a, mlp_bwd_steps, st);
 }
 

@@ -153,7 +153,8 @@ def linear_fp8(x: Tensor, weight: Tensor, x_scale: Tensor, w_scale: Tensor, bias
 
 
 def _mlp(plan: bytes, x, wg, wu, wd, residual, keep):
-    """(y, kept): dense operands; kept is () or (act(g), act'(g) * u, act(g) * u) for the backward, rows padded to a multiple of 8."""
+    """(y, kept): dense operands; kept is () or, for the backward, act(g) and act'(g) * u in 24 bits (three tensors)
+    and act(g) * u, rows padded to a multiple of 8."""
     a = L.GatedMlpArgs.from_buffer_copy(plan)
     y = torch.empty_like(x)
     a.x, a.wg, a.wu, a.wd, a.y = x.data_ptr(), wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), y.data_ptr()
@@ -161,8 +162,9 @@ def _mlp(plan: bytes, x, wg, wu, wd, residual, keep):
         a.residual = residual.data_ptr()
     kept = ()
     if keep:
-        kept = p, s, h = [x.new_empty((a.M, (a.F + 7) // 8 * 8)) for _ in range(3)]
-        a.p, a.s, a.h = p.data_ptr(), s.data_ptr(), h.data_ptr()
+        shape = (a.M, (a.F + 7) // 8 * 8)
+        kept = p, s, low, h = *(x.new_empty(shape, dtype=torch.int16) for _ in range(3)), x.new_empty(shape)
+        a.p, a.s, a.low, a.h = p.data_ptr(), s.data_ptr(), low.data_ptr(), h.data_ptr()
     lib = L.load()
     _run(a, lib.nsa_gated_mlp_ws_bytes, lib.nsa_gated_mlp, "nsa_gated_mlp", x)
     return y, kept

@@ -423,7 +423,7 @@ def test_gated_mlp_backward(nsa, M, N, F, dtype, act, res):
     dh = dyd @ wd
     dhe = (N + 2) * U * (dyd.abs() @ wd.abs())
 
-    def product(*fs):
+    def product(*fs, half=half, tiny=tiny):
         """(product, its error) of factors given with theirs, rounded to 16 bits."""
         v, hi = 1.0, 1.0
         for f, e in fs:
@@ -431,9 +431,13 @@ def test_gated_mlp_backward(nsa, M, N, F, dtype, act, res):
         err = hi - v.abs() + 4 * U * hi
         return v, (1 + half) * err + half * v.abs() + tiny
 
-    # act(g), act'(g) u and act(g) u are kept in 16 bits
-    dg, dge = product((dh, dhe), product((u, ue), (s, se)))
-    du, due = product((dh, dhe), product((a, ae)))
+    def kept(*fs):
+        """... to 24 bits."""
+        return product(*fs, half=2.0 ** -16, tiny=0.0)
+
+    # act(g) and act'(g) u are kept in 24 bits, act(g) u in 16
+    dg, dge = product((dh, dhe), kept((u, ue), (s, se)))
+    du, due = product((dh, dhe), kept((a, ae)))
     h, he = product((a, ae), (u, ue))
 
     def contract(pairs, n):

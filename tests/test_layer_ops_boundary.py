@@ -75,7 +75,7 @@ def test_c_entry_points_refuse():
     m = L.GatedMlpArgs(x=16, wg=16, wu=16, wd=16, y=16, ws=16, M=4, N=8, F=16, dtype=0, act=1)
     refused(lib.nsa_gated_mlp(C.byref(m), None), ARG, "workspace")
     m.p = 16
-    refused(lib.nsa_gated_mlp(C.byref(m), None), ARG, "p, s and h")
+    refused(lib.nsa_gated_mlp(C.byref(m), None), ARG, "p, s, low and h")
     m.dtype = 4
     refused(lib.nsa_gated_mlp(C.byref(m), None), UNSUPPORTED, "dtype")
 
