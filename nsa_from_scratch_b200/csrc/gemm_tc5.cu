@@ -49,6 +49,9 @@ __device__ __forceinline__ void arrive_remote(uint32_t cluster_addr) {
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, uint32_t src, int c0, int c1) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];\n" ::"l"(map), "r"(src), "r"(c0), "r"(c1) : "memory");
 }
+__device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, uint32_t src, int c0, int c1, int c2) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%2, %3, %4}], [%1];\n" ::"l"(map), "r"(src), "r"(c0), "r"(c1), "r"(c2) : "memory");
+}
 __device__ __forceinline__ void group_sync(int id) { asm volatile("bar.sync %0, 128;\n" ::"r"(id) : "memory"); }
 __device__ __forceinline__ uint4 lds128(uint32_t a) {
   uint4 v;
@@ -128,8 +131,7 @@ struct GemmTcParams {
   TcProduct pr[TC_PRODUCTS];
   CUtensorMap tmO1, tmO2, tmO3, tmI0, tmI1, tmI2;   // further results and inputs of the epilogue (I0: residual in EPI_LINEAR); one product
   Epi e;
-  float* part;                                  // PARTIAL: [splits][products][M][ldp] fp32; one product
-  int ldp;
+  CUtensorMap tmPart;                           // PARTIAL: [splits][products of a pair][M][N] fp32 sums; one product
   int products, tiles;                          // tiles: of all products and splits
   int splits, per_split;                        // the steps of all segments, dealt out to `splits` tiles
 };
@@ -140,8 +142,8 @@ constexpr int EPI_SLOPE = 3, EPI_PARTIAL = 4, EPI_PARTIAL2 = 5;
 
 template <int MODE, int CG, int BN> struct TcShape {
   static constexpr int A_BYTES = 128 * 128, B_BYTES = BN / CG * 128;
-  // stages of the operands' ring, and bytes of each of the two epilogue groups (EPI_GLU_BWD: two stages of three boxes)
-  static constexpr int STAGES = MODE == EPI_GLU_BWD ? 4 : 5, EPI_BYTES = MODE == EPI_GLU_BWD ? 49152 : 32768;
+  // bytes of each of the two epilogue groups (EPI_GLU_BWD: two stages of three boxes), and stages of the operands' ring
+  static constexpr int EPI_BYTES = MODE == EPI_GLU_BWD ? 49152 : 32768, STAGES = (229376 - 2 * EPI_BYTES) / (A_BYTES + B_BYTES);
   static constexpr int SMEM = STAGES * (A_BYTES + B_BYTES) + 2 * EPI_BYTES + 1024;
 };
 
@@ -301,8 +303,8 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
     constexpr bool RAW = MODE == EPI_PARTIAL || MODE == EPI_PARTIAL2;
     constexpr int GW = NW / 2;                                           // columns of the group
     constexpr int CW = MODE == EPI_LINEAR ? 64 : 32;                     // columns of a chunk
-    constexpr int NC = RAW ? 1 : GW / CW;
-    constexpr int BOX = 128 * CW * 2;                                    // bytes of a box: 128 rows of CW columns
+    constexpr int NC = GW / CW;
+    constexpr int BOX = 128 * CW * (RAW ? 4 : 2);                        // bytes of a box: 128 rows of CW columns
     constexpr int STAGE = MODE == EPI_GLU ? 0 : S::EPI_BYTES / 2;        // between the two stages (EPI_GLU: one stage of four boxes)
     const uint32_t stage0 = s_tiles + S::STAGES * (S::A_BYTES + S::B_BYTES) + group * S::EPI_BYTES;
     constexpr bool LIN = MODE == EPI_LINEAR || MODE == EPI_SLOPE;
@@ -348,20 +350,26 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
         }
       };
       if constexpr (RAW) {
+        constexpr int PR = PAIR ? 2 : 1;
 #pragma unroll 1
-        for (int c = 0; c < GW; c += 16) {
+        for (int c = 0; c < NC * PR; ++c, ++cnt) {
+          const uint32_t box = stage0 + (cnt & 1) * STAGE;
+          const int q = PAIR ? c / NC : 0, col = (PAIR ? c % NC : c) * CW;
+          if (lead) bulk_wait_read<1>();
+          group_sync(1 + group);
+          uint32_t v[32];
+          tmem_ld32(acc + q * NW + col, v);
+          tc_wait_ld();
 #pragma unroll
-          for (int q = 0; q < (PAIR ? 2 : 1); ++q) {
-            uint32_t v[16];
-            tmem_ld16(acc + c + q * NW, v);
-            tc_wait_ld();
-            float* dst = p.part + (((long long)w.split * (PAIR ? 2 : 1) + q) * M + grow) * p.ldp + nc0 + c;
-#pragma unroll
-            for (int i = 0; i < 16; i += 4)
-              if (grow < M && nc0 + c + i < p.ldp) *reinterpret_cast<uint4*>(dst + i) = make_uint4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+          for (int i = 0; i < 8; ++i) sts128(box + row * 128 + ((i ^ (row & 7)) << 4), make_uint4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]));
+          if (c == NC * PR - 1) drained();
+          fence_proxy_async();
+          group_sync(1 + group);
+          if (lead && ok) {
+            tma_store_3d(&p.tmPart, box, nc0 + col, mr, w.split * PR + q);
+            bulk_commit();
           }
         }
-        drained();
       } else {
         // the next 16 columns leave TMEM while these are worked on
         uint32_t v[16], u[MODE == EPI_GLU ? 16 : 1];
@@ -574,36 +582,56 @@ static int map_2d(CUtensorMap* m, const void* ptr, long long rows, long long col
   return NSA_OK;
 }
 
-static int esize(int dtype) { return dtype == NSA_BF16 || dtype == NSA_FP16 ? 2 : 1; }
-
 static int pitch(int N) { return (N + 7) / 8 * 8; }                     // of partial sums
+// [slabs][M][N] fp32 partial sums, rows `pitch` apart; boxes of 128 rows x 32 columns
+static int map_part(CUtensorMap* m, void* ptr, int slabs, int M, int N) {
+  auto enc = tensor_map_encoder();
+  NSA_REQUIRE(enc != nullptr, NSA_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
+  cuuint64_t dims[3] = {(cuuint64_t)N, (cuuint64_t)M, (cuuint64_t)slabs};
+  cuuint64_t strides[2] = {(cuuint64_t)pitch(N) * 4, (cuuint64_t)M * pitch(N) * 4};
+  cuuint32_t box[3] = {32, 128, 1};
+  cuuint32_t es[3] = {1, 1, 1};
+  const CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 3, ptr, dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                         CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  NSA_REQUIRE(r == CUDA_SUCCESS, NSA_ERR_CUDA, "cuTensorMapEncodeTiled (partial sums) failed with %d", (int)r);
+  return NSA_OK;
+}
+
+static int esize(int dtype) { return dtype == NSA_BF16 || dtype == NSA_FP16 ? 2 : 1; }
 
 // Which kernel, how many ways the contraction is split, and whether the sums leave raw: where they are split, or where
 // the results' rows do not start on 16-byte boundaries (TMA writes them).
 struct TcPlan { int cg, bn, tiles_m, tiles_n, ksteps, splits, per_split; bool raw; };
-static TcPlan tc_plan(const GemmProblem& p) {
+static TcPlan tc_plan(const GemmProblem& p, bool whole = false) {     // whole: pairs on 256 columns, unsplit
   TcPlan t;
   const int pair = p.e.mode == EPI_GLU ? 2 : 1;
-  t.cg = p.M <= 128 ? 1 : 2;
-  t.bn = t.cg * 128;
-  t.tiles_m = (p.M + 128 * t.cg - 1) / (128 * t.cg);
-  t.tiles_n = (p.N + t.bn / pair - 1) / (t.bn / pair);
-  t.ksteps = (p.K * esize(p.dtype) + 127) / 128;
-  const long long n = (long long)t.tiles_m * t.tiles_n, units = sm_count() / t.cg;
-  const int steps = t.ksteps * p.segments;
-  // Rounds of tiles at 512 clk a step, and 3000 for the epilogue that no other tile hides; splitting adds the sums' way out
-  // and back through L2 (64 bytes a clk and SM) and the joining kernel (6000).  The cheapest of up to 16 ways.
-  t.raw = !p.e.vec || !p.e.vecy;
-  double best = 0;
-  t.splits = 1;
-  t.per_split = steps;
-  for (int s = 1; s <= 16 && s * 4 <= (steps > 4 ? steps : 4); ++s) {
-    const int per = (steps + s - 1) / s, ways = (steps + per - 1) / per;
-    double cost = (double)((n * ways + units - 1) / units) * per * 512 + 3000;
-    if (ways > 1 || t.raw) cost += 6000 + 8.0 * ways * pair * p.M * p.N / (64.0 * sm_count());
-    if (s == 1 || cost < best) { best = cost; t.splits = ways; t.per_split = per; }
+  const bool raw = !p.e.vec || !p.e.vecy;
+  const int ksteps = (p.K * esize(p.dtype) + 127) / 128, steps = ksteps * p.segments;
+  // In clk: rounds of tiles at what a step brings through L2 and shared memory (512 for 256 columns on pairs and for 128 on
+  // one CTA, 384 for 128 on pairs), and the epilogue that no other tile hides; splitting adds the sums' way out and back
+  // (64 bytes a clk and SM) and the joining kernel.  The cheapest of both widths and up to 16 ways.
+  double best = -1;
+  for (int bn = 256; bn >= 128; bn -= 128) {
+    const int cg = !whole && p.M <= 128 ? 1 : 2;
+    if ((cg == 1 && bn == 256) || (whole && bn == 128)) continue;
+    const int tm = (p.M + 128 * cg - 1) / (128 * cg), tn = (p.N + bn / pair - 1) / (bn / pair);
+    const long long n = (long long)tm * tn, units = sm_count() / cg;
+    const int step = cg == 2 && bn == 128 ? 384 : 512;
+    for (int s = 1; s <= 16 && s * 4 <= (steps > 4 ? steps : 4); ++s) {
+      if (whole && s > 1) break;
+      const int per = (steps + s - 1) / s, ways = (steps + per - 1) / per;
+      double cost = (double)((n * ways + units - 1) / units) * per * step + 16 * bn;
+      if (ways > 1 || raw) cost += 5000 + 8.0 * ways * pair * p.M * p.N / (64.0 * sm_count());
+      if (best < 0 || cost < best) {
+        best = cost;
+        t.cg = cg; t.bn = bn;
+        t.tiles_m = tm; t.tiles_n = tn;
+        t.splits = ways; t.per_split = per;
+      }
+    }
   }
-  t.raw = t.raw || t.splits > 1;
+  t.ksteps = ksteps;
+  t.raw = raw || t.splits > 1;
   return t;
 }
 
@@ -642,27 +670,28 @@ static int tc_launch(const GemmTcParams& g, cudaStream_t st) {
 }
 
 template <int F, typename T, int MODE>
-static int tc_shape(const GemmTcParams& g, int cg, cudaStream_t st) {
-  return cg == 2 ? tc_launch<F, T, MODE, 2, 256>(g, st) : tc_launch<F, T, MODE, 1, 128>(g, st);
+static int tc_shape(const GemmTcParams& g, const TcPlan& t, cudaStream_t st) {
+  if (t.cg == 1) return tc_launch<F, T, MODE, 1, 128>(g, st);
+  return t.bn == 256 ? tc_launch<F, T, MODE, 2, 256>(g, st) : tc_launch<F, T, MODE, 2, 128>(g, st);
 }
 
 // mode: EPI_*, as the kernel has it
 template <int F, typename T>
-static int tc_mode(const GemmTcParams& g, int cg, int mode, cudaStream_t st) {
-  if (mode == EPI_PARTIAL) return tc_shape<F, T, EPI_PARTIAL>(g, cg, st);
+static int tc_mode(const GemmTcParams& g, const TcPlan& t, int mode, cudaStream_t st) {
+  if (mode == EPI_PARTIAL) return tc_shape<F, T, EPI_PARTIAL>(g, t, st);
   if constexpr (F < 2) {
-    if (mode == EPI_PARTIAL2) return tc_shape<F, T, EPI_PARTIAL2>(g, cg, st);
-    if (mode == EPI_GLU) return tc_shape<F, T, EPI_GLU>(g, cg, st);
-    if (mode == EPI_GLU_BWD) return tc_shape<F, T, EPI_GLU_BWD>(g, cg, st);
-    if (mode == EPI_SLOPE) return tc_shape<F, T, EPI_SLOPE>(g, cg, st);
+    if (mode == EPI_PARTIAL2) return tc_shape<F, T, EPI_PARTIAL2>(g, t, st);
+    if (mode == EPI_GLU) return tc_shape<F, T, EPI_GLU>(g, t, st);
+    if (mode == EPI_GLU_BWD) return tc_shape<F, T, EPI_GLU_BWD>(g, t, st);
+    if (mode == EPI_SLOPE) return tc_shape<F, T, EPI_SLOPE>(g, t, st);
   }
-  return tc_shape<F, T, EPI_LINEAR>(g, cg, st);
+  return tc_shape<F, T, EPI_LINEAR>(g, t, st);
 }
-static int tc_types(const GemmTcParams& g, int cg, int mode, int dtype, bool bf, cudaStream_t st) {
-  if (dtype == NSA_BF16) return tc_mode<1, __nv_bfloat16>(g, cg, mode, st);
-  if (dtype == NSA_FP16) return tc_mode<0, __half>(g, cg, mode, st);
-  if (dtype == NSA_FP8_E4M3) return bf ? tc_mode<2, __nv_bfloat16>(g, cg, mode, st) : tc_mode<2, __half>(g, cg, mode, st);
-  return bf ? tc_mode<3, __nv_bfloat16>(g, cg, mode, st) : tc_mode<3, __half>(g, cg, mode, st);
+static int tc_types(const GemmTcParams& g, const TcPlan& t, int mode, int dtype, bool bf, cudaStream_t st) {
+  if (dtype == NSA_BF16) return tc_mode<1, __nv_bfloat16>(g, t, mode, st);
+  if (dtype == NSA_FP16) return tc_mode<0, __half>(g, t, mode, st);
+  if (dtype == NSA_FP8_E4M3) return bf ? tc_mode<2, __nv_bfloat16>(g, t, mode, st) : tc_mode<2, __half>(g, t, mode, st);
+  return bf ? tc_mode<3, __nv_bfloat16>(g, t, mode, st) : tc_mode<3, __half>(g, t, mode, st);
 }
 
 template <typename T>
@@ -702,7 +731,9 @@ int gemm_tc5(const GemmProblem& p, void* ws, cudaStream_t st) {
   int rc = tc_product(&g.pr[0], p, t);
   if (rc != NSA_OK) return rc;
   const bool gated = p.e.mode != EPI_LINEAR, slope = !gated && p.e.o1 != nullptr;
-  if (!t.raw) {
+  if (t.raw) {
+    if ((rc = map_part(&g.tmPart, ws, (p.e.mode == EPI_GLU ? 2 : 1) * t.splits, p.M, p.N)) != NSA_OK) return rc;
+  } else {
     const int cw = gated || slope ? 32 : 64;
     auto box = [&](CUtensorMap* m, const void* ptr, long long ld) { return ptr == nullptr ? NSA_OK : map_2d(m, ptr, p.M, p.N, ld, cw, 128, p.out_dtype); };
     if ((rc = box(&g.pr[0].tmY, p.e.y, p.e.ldy)) != NSA_OK) return rc;
@@ -714,30 +745,26 @@ int gemm_tc5(const GemmProblem& p, void* ws, cudaStream_t st) {
     if ((rc = box(&g.tmI2, p.e.i2, p.e.ldy)) != NSA_OK) return rc;
   }
   g.e = p.e;
-  g.part = reinterpret_cast<float*>(ws);
-  g.ldp = pitch(p.N);
   g.products = 1; g.tiles = (int)tiles;
   g.splits = t.splits; g.per_split = t.per_split;
   const bool bf = p.out_dtype == NSA_BF16;
   const int mode = t.raw ? (p.e.mode == EPI_GLU ? EPI_PARTIAL2 : EPI_PARTIAL) : slope ? EPI_SLOPE : p.e.mode;
-  rc = tc_types(g, t.cg, mode, p.dtype, bf, st);
+  rc = tc_types(g, t, mode, p.dtype, bf, st);
   if (rc != NSA_OK || !t.raw) return rc;
-  return bf ? join<__nv_bfloat16>(g.part, p, t.splits, st) : join<__half>(g.part, p, t.splits, st);
+  return bf ? join<__nv_bfloat16>((const float*)ws, p, t.splits, st) : join<__half>((const float*)ws, p, t.splits, st);
 }
 
-// Several plain products (EPI_LINEAR with nothing around the sums) of one 16-bit type.  One launch where each would run
-// unsplit on CTA pairs or where together they fill the SMs; else one by one.
+// Several plain products (EPI_LINEAR with nothing around the sums) of one 16-bit type.  One launch of whole tiles where
+// together they fill at least half of the SMs; else one by one.
 static bool groups(const GemmProblem* p, int count) {
   if (count < 2 || count > TC_PRODUCTS) return false;
   long long tiles = 0;
-  bool single = true;
   for (int i = 0; i < count; ++i) {
-    const TcPlan t = tc_plan(p[i]);
-    if (t.cg != 2 || !p[i].e.vec || !p[i].e.vecy) return false;
+    if (p[i].M <= 128 || !p[i].e.vec || !p[i].e.vecy) return false;
+    const TcPlan t = tc_plan(p[i], true);
     tiles += (long long)t.tiles_m * t.tiles_n;
-    single = single && t.splits == 1;
   }
-  return tiles < 2147483647LL - 65536 && (single || tiles * 2 >= sm_count());
+  return tiles < 2147483647LL - 65536 && tiles * 4 >= sm_count();
 }
 
 long long gemm_tc5_group_ws_bytes(const GemmProblem* p, int count) {
@@ -760,8 +787,6 @@ int gemm_tc5_group(const GemmProblem* p, int count, void* ws, cudaStream_t st) {
   }
   GemmTcParams g;
   g.e = p[0].e;
-  g.part = nullptr;
-  g.ldp = 0;
   g.products = count;
   g.splits = 1; g.per_split = 0;
   // the longest tiles first: the last round is then of the shortest
@@ -772,9 +797,10 @@ int gemm_tc5_group(const GemmProblem* p, int count, void* ws, cudaStream_t st) {
     order[j] = i;
   }
   int tiles = 0;
+  TcPlan t = {};
   for (int i = 0; i < count; ++i) {
     const GemmProblem& q = p[order[i]];
-    const TcPlan t = tc_plan(q);
+    t = tc_plan(q, true);
     int rc = tc_product(&g.pr[i], q, t);
     if (rc == NSA_OK) rc = map_2d(&g.pr[i].tmY, q.e.y, q.M, q.N, q.e.ldy, 64, 128, q.out_dtype);
     if (rc != NSA_OK) return rc;
@@ -782,7 +808,7 @@ int gemm_tc5_group(const GemmProblem* p, int count, void* ws, cudaStream_t st) {
     tiles += t.tiles_m * t.tiles_n;
   }
   g.tiles = tiles;
-  return tc_types(g, 2, EPI_LINEAR, p[0].dtype, p[0].out_dtype == NSA_BF16, st);
+  return tc_types(g, t, EPI_LINEAR, p[0].dtype, p[0].out_dtype == NSA_BF16, st);
 }
 
 int gemm_take_status(int* status) {
