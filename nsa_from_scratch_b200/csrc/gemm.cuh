@@ -211,7 +211,7 @@ static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t
 int sm_count();                                                            // of the current device (linear.cu)
 long long gemm_tc5_ws_bytes(const GemmProblem& p);                       // gemm_tc5.cu
 int gemm_tc5(const GemmProblem& p, void* ws, cudaStream_t st);
-bool gemm_skinny_takes(int M, int mode);                                   // gemm_skinny.cu: k-major operands of any alignment
+bool gemm_skinny_takes(int M, int N, int K, int mode);                     // gemm_skinny.cu: k-major operands of any alignment
 int gemm_skinny(const GemmProblem& p, bool early, cudaStream_t st);        // early: what runs before it in the stream does not write the weights
 long long gemm_tc5_group_ws_bytes(const GemmProblem* p, int count);
 int gemm_tc5_group(const GemmProblem* p, int count, void* ws, cudaStream_t st);

@@ -209,7 +209,7 @@ static int check_linear(const nsa_linear_args& a) {
 }
 
 static int linear_steps(const nsa_linear_args& a, Arena& w) {
-  const bool few = gemm_skinny_takes(a.M, EPI_LINEAR);
+  const bool few = gemm_skinny_takes(a.M, a.N, a.K, EPI_LINEAR);
   Mat x{a.x, a.K}, wt{a.w, a.K};
   if (!few) {
     NSA_TRY(operand(w, a.x, a.M, a.K, a.dtype, &x));
@@ -289,7 +289,7 @@ static int check_mlp(int M, int N, int F, int dtype, int act) {
 static int mlp_steps(const nsa_gated_mlp_args& a, Arena& w) {
   const long long ldh = padded(a.F, a.dtype);
   void* h = a.h != nullptr ? a.h : w.take((long long)a.M * ldh * 2);
-  const bool few = gemm_skinny_takes(a.M, EPI_GLU), few_down = gemm_skinny_takes(a.M, EPI_LINEAR);
+  const bool few = gemm_skinny_takes(a.M, a.F, a.N, EPI_GLU), few_down = gemm_skinny_takes(a.M, a.N, a.F, EPI_LINEAR);
   Mat x{a.x, a.N}, wg{a.wg, a.N}, wu{a.wu, a.N}, wd{a.wd, a.F};
   if (!few) {
     NSA_TRY(operand(w, a.x, a.M, a.N, a.dtype, &x));
