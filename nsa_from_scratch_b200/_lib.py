@@ -247,6 +247,28 @@ def load() -> C.CDLL:
     return lib
 
 
+_torch_ops = None
+
+
+def torch_ops():
+    """The compiled torch side of the layer's operators (built first if needed); raises if that is impossible."""
+    global _torch_ops
+    if _torch_ops is None:
+        from . import build as _build
+        load()                       # checks the ABI version of the library that the module links to
+        try:
+            path = _build.build_torch()
+        except RuntimeError:
+            path = _build.TORCH_LIB
+            if not os.path.exists(path):
+                raise                # with a module present (no compiler on this machine) its import decides
+        import importlib.util
+        spec = importlib.util.spec_from_file_location("_nsa_torch", path)
+        _torch_ops = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(_torch_ops)
+    return _torch_ops
+
+
 def check(rc: int, what: str) -> None:
     if rc != OK:
         msg = load().nsa_last_error().decode("utf-8", "replace")
@@ -274,17 +296,6 @@ def on_device(t):
     """Context in which `t`'s device is current.  Almost every call finds it current already, and entering
     torch.cuda.device costs several microseconds of a short launch."""
     return _NO_GUARD if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
-
-
-def call(fn, args, index: int, what: str) -> None:
-    """fn(&args, current stream) on device `index`, checked: the short way for calls whose host time counts."""
-    if index == torch._C._cuda_getDevice():
-        rc = fn(C.byref(args), torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            rc = fn(C.byref(args), torch._C._cuda_getCurrentRawStream(index))
-    if rc != OK:
-        check(rc, what)
 
 
 def ptr(t) -> int:

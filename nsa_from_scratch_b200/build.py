@@ -1,4 +1,5 @@
-"""Builds libnsa_b200.so (the C-ABI library) in-tree with nvcc for sm_100a.
+"""Builds libnsa_b200.so (the C-ABI library) in-tree with nvcc for sm_100a, and _nsa_torch.so beside it: the layer's
+operators on torch tensors, host code over that library (csrc/torch_ops.cpp, compiled for the torch at hand).
 
     python -m nsa_from_scratch_b200.build [--force] [--verbose]
 
@@ -20,6 +21,8 @@ CSRC = os.path.join(PKG, "csrc")
 OBJ = os.path.join(PKG, "_build")
 LIB = os.path.join(PKG, "libnsa_b200.so")
 INC = os.path.join(os.path.dirname(PKG), "include")
+TORCH_LIB = os.path.join(PKG, "_nsa_torch.so")
+TORCH_SRC = os.path.join(CSRC, "torch_ops.cpp")
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
@@ -80,5 +83,39 @@ def build(force: bool = False, verbose: bool = False) -> str:
     return LIB
 
 
+def build_torch(force: bool = False) -> str:
+    """Compile the torch side if its source, the C header, torch or Python changed; return the path of the module."""
+    import sysconfig
+
+    import torch
+
+    build()
+    h = hashlib.sha256(f"{torch.__version__} {torch._C._GLIBCXX_USE_CXX11_ABI} {sys.version}".encode())
+    for f in (TORCH_SRC, os.path.join(INC, "nsa_b200.h"), os.path.abspath(__file__)):
+        h.update(open(f, "rb").read())
+    stamp, dig = os.path.join(OBJ, "torch_stamp"), h.hexdigest()
+    if not force and os.path.exists(TORCH_LIB) and os.path.exists(stamp) and open(stamp).read() == dig:
+        return TORCH_LIB
+    # nvcc's host compiler, as for the library.  $CXX may be another one that links a C++ runtime of its own into the module,
+    # and with two of them in one process the first formatted error message crashes.
+    nvcc = _nvcc()
+    home, cuda = os.path.dirname(torch.__file__), os.path.dirname(os.path.dirname(os.path.realpath(nvcc)))
+    part = f"{TORCH_LIB}.{os.getpid()}"              # renamed when whole: two processes may build at once
+    cmd = [nvcc, "-O2", "-std=c++17", "-shared", "-cudart", "none", "-Xcompiler", "-fPIC,-fvisibility=hidden", "-DTORCH_EXTENSION_NAME=_nsa_torch",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-I{d}" for d in (os.path.join(home, "include"), os.path.join(home, "include/torch/csrc/api/include"), os.path.join(cuda, "include"),
+                                sysconfig.get_paths()["include"])),
+           TORCH_SRC, "-o", part, f"-L{home}/lib", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", f"-L{PKG}",
+           "-Xlinker", "-l:libnsa_b200.so", "-Xlinker", "-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"nvcc failed on torch_ops.cpp:\n{r.stderr[-4000:]}")
+    os.replace(part, TORCH_LIB)
+    with open(stamp, "w") as f:
+        f.write(dig)
+    return TORCH_LIB
+
+
 if __name__ == "__main__":
     print(build(force="--force" in sys.argv, verbose="--verbose" in sys.argv))
+    print(build_torch(force="--force" in sys.argv))

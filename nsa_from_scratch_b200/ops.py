@@ -84,41 +84,11 @@ def _need_cuda(*ts: Tensor) -> None:
             raise RuntimeError("nsa_from_scratch_b200 kernels need CUDA tensors (there is no CPU path)")
 
 
-def _same_device(x: Tensor, **others: Optional[Tensor]) -> None:
-    """Every operand lies where `x` does."""
-    for name, t in others.items():
-        if t is not None and t.device != x.device:
-            _need_cuda(t)
-            raise ValueError(f"{name} is on {t.device}, the first operand on {x.device}")
-
-
 def activation_code(name: Optional[str]) -> int:
     try:
         return L.ACTIVATIONS[name]
     except KeyError:
         raise ValueError(f"unknown activation: {name}") from None
-
-
-def first_order(backward):
-    """A Function's backward that runs its kernels outside autograd, as once_differentiable does: its results refuse a second
-    differentiation.  That costs several microseconds, which only a caller who keeps the graph (create_graph) pays."""
-    guarded = torch.autograd.function.once_differentiable(backward)
-
-    def run(ctx, *grads):
-        return guarded(ctx, *grads) if torch.is_grad_enabled() else backward(ctx, *grads)
-
-    return run
-
-
-class Plans(dict):
-    """What an entry point found out about operands of given shapes, types and devices (never about their addresses or
-    values): checked once, then an argument struct without pointers.  A program meets few; one that meets many starts over."""
-
-    def keep(self, key, plan):
-        if len(self) >= 256:
-            self.clear()
-        self[key] = plan
-        return plan
 
 
 def softmax_scale(D: int, scale: Optional[float]) -> float:

@@ -519,3 +519,12 @@ def test_empty(nsa):
     assert nsa.linear_fp8(q, q.new_zeros(8, 64), s, s.new_ones(8)).shape == (0, 8)
     p = randn(1, 0, 2, 64)
     assert nsa.rope_axes_to_heads(p, p, p, torch.zeros(1, 1, 0, dtype=torch.int64, device="cuda"), nsa.rope_frequencies(64), (32,))[0].shape == (1, 2, 0, 64)
+
+
+def test_more_rows_than_32_bits_count(nsa):
+    """The products' sizes are 32-bit numbers: more rows are refused, not wrapped."""
+    x, w = torch.empty(1 << 31, 1, device="cuda", dtype=torch.bfloat16), randn(8, 1)
+    for call in (lambda: nsa.linear(x, w), lambda: nsa.gated_mlp(x, w, w, w.T.contiguous()),
+                 lambda: nsa.linear_fp8(x.view(torch.float8_e4m3fn)[:, :1].contiguous(), w.to(torch.float8_e4m3fn), torch.empty(1 << 31, device="cuda"), torch.ones(8, device="cuda"))):
+        with pytest.raises(ValueError, match="32-bit"):
+            call()

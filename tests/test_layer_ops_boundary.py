@@ -91,6 +91,13 @@ def test_no_cpu_path():
         nsa.rope_axes_to_heads(q, q, q, torch.zeros(1, 1, 2, dtype=torch.int64), torch.zeros(4), (4,))
 
 
+def test_torch_side_shares_the_cxx_runtime():
+    """A module that brings a C++ runtime of its own into torch's process crashes at its first formatted message."""
+    from nsa_from_scratch_b200 import build
+    L.torch_ops()
+    assert b"libstdc++.so.6" in open(build.TORCH_LIB, "rb").read()
+
+
 def test_rope_frequencies():
     f = nsa.rope_frequencies(64, 10000.0, device="cpu")
     assert f.dtype == torch.float64 and f.shape == (32,) and float(f[0]) == 1.0 and abs(float(f[16]) - 0.01) < 1e-15
