@@ -7,6 +7,8 @@
 //
 // Bound by HBM.  A block owns a row: every element is read once, 16 bytes a load, and stays in registers (fp32) between
 // the sum and the result.  V = vectors of 8 elements per thread.  Sums are fp32, formed in a fixed order.
+// 16384 x 8192 bf16 with the residual and an fp8 result: 171 us = 5.5 TB/s (a plain copy reaches 6.5); 250 with one vector
+// a thread, 173 with four, 178 with streaming loads and stores.  8189 x 4096 fp16: 46 us = 5.8 TB/s.
 #include "gemm.cuh"
 
 namespace nsa {
@@ -293,7 +295,8 @@ template <typename T> struct Raw {
 
 // A block walks the rows b, b + grid, ...; its share of dw stays in registers and is written once.  A row stays as it was
 // stored (raw) across the barrier of its sum and is unpacked twice: with 64 registers a thread, 1024 threads an SM, so
-// that some rows are on their way while others are summed.
+// that some rows are on their way while others are summed.  8189 x 4096 fp16 with dh: 49 us = 5.5 TB/s; 60 with the next row
+// held in registers, 62 with a cp.async ring, 65 with two rows at a time.
 template <typename X, typename R, int V, bool DH, int T_MAX>
 __global__ void __launch_bounds__(T_MAX, 1024 / T_MAX) rms_norm_bwd_kernel(const NormBwdParams p) {
   __shared__ float part[2][32];
