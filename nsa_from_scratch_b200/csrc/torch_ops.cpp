@@ -68,6 +68,14 @@ template <typename A> Tensor workspace(A& a, int64_t need, const char* what, con
   a.ws_bytes = need;
   return ws;
 }
+// Bits of the tensor inputs whose gradients this backward is asked for; the inputs of bit i in `present` have an edge.
+int64_t asked(AutogradContext* ctx, int64_t present) {
+  int64_t bits = 0;
+  size_t edge = 0;
+  for (int i = 0; present >> i; ++i)
+    if (present >> i & 1) bits |= (int64_t)ctx->needs_input_grad(edge++) << i;
+  return bits;
+}
 // The results of a backward under create_graph: they refuse a second differentiation instead of passing for constants.
 variable_list first_order(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
@@ -128,7 +136,7 @@ struct RmsNorm : Function<RmsNorm> {
     const Tensor y = at::empty_like(x), rstd = at::empty({a.rows}, x.options().dtype(at::kFloat));
     const Tensor h = launch_norm(a, x, res, y, Tensor(), rstd);
     ctx->save_for_backward({h.defined() ? h : x, w, rstd});
-    ctx->saved_data["flags"] = (int64_t)(code(x.scalar_type()) | (h.defined() ? 16 : 0) | (w.requires_grad() ? 32 : 0));
+    ctx->saved_data["flags"] = (int64_t)(code(x.scalar_type()) | (h.defined() ? 16 : 0));
     ctx->set_materialize_grads(false);
     return h.defined() ? variable_list{y, h} : variable_list{y};
   }
@@ -143,7 +151,7 @@ struct RmsNorm : Function<RmsNorm> {
     const Tensor dh = has_stream && grads[1].defined() ? grads[1].contiguous() : Tensor();
     const Tensor dx = at::empty(h.sizes(), h.options().dtype(xt));
     const Tensor dres = has_stream && h.scalar_type() != xt ? at::empty_like(h) : Tensor();
-    const Tensor dw = flags & 32 ? at::empty_like(w) : Tensor();
+    const Tensor dw = ctx->needs_input_grad(1) ? at::empty_like(w) : Tensor();
     nsa_norm_bwd_args a = {};
     a.dy = dy.data_ptr(); a.dh = ptr(dh); a.h = h.data_ptr(); a.weight = w.data_ptr(); a.rstd = (const float*)rstd.data_ptr();
     a.dx = dx.data_ptr(); a.dres = ptr(dres); a.dweight = ptr(dw);
@@ -278,13 +286,19 @@ variable_list rope_axes(const Tensor& q, const Tensor& k, const Tensor& v, const
 }
 
 // ---------------------------------------------------------------- projections
+// t, where it is given, is [lead..., last] (last < 0: [lead...]) of dtype
 void rows_like(const optional<Tensor>& t, const char* name, at::IntArrayRef lead, int64_t last, const Tensor& x, at::ScalarType dtype, const char* what) {
   if (!given(t)) return;
   operand(*t, name, x);
-  bool same = t->scalar_type() == dtype && t->dim() == (int64_t)lead.size() + (last >= 0 ? 1 : 0);
-  for (size_t i = 0; same && i < lead.size(); ++i) same = t->size((int64_t)i) == lead[i];
-  if (last >= 0) same = same && t->size(-1) == last;
-  TORCH_CHECK_VALUE(same, what, ": ", name, " must be [", lead, last >= 0 ? ", " + std::to_string(last) : std::string(), "] ", dtype, ", got ", t->sizes(), " ", t->scalar_type());
+  auto same = [&] {
+    const size_t n = lead.size();
+    if (t->scalar_type() != dtype || (size_t)t->dim() != n + (last >= 0) || t->sizes().slice(0, n) != lead) return false;
+    return last < 0 || t->size(-1) == last;
+  };
+  if (same()) return;
+  auto shape = lead.vec();
+  if (last >= 0) shape.push_back(last);
+  TORCH_CHECK_VALUE(false, what, ": ", name, " must be ", at::IntArrayRef(shape), " ", dtype, ", got ", t->sizes(), " ", t->scalar_type());
 }
 nsa_linear_args check_linear(const Tensor& x, const Tensor& w, const optional<Tensor>& bias, const optional<Tensor>& res, const optional<Tensor>& xs,
                              const optional<Tensor>& ws, int64_t act, int64_t y_dtype, const char* what) {
@@ -328,17 +342,16 @@ Tensor launch_linear(nsa_linear_args a, const Tensor& x, Tensor* slope) {
 struct Linear : Function<Linear> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const optional<Tensor>& bias, const optional<Tensor>& res, int64_t act) {
     const nsa_linear_args a = check_linear(x, w, bias, res, {}, {}, act, code(x.scalar_type()), "linear");
-    const int64_t need = (x.requires_grad() ? 1 : 0) | (w.requires_grad() ? 2 : 0) | (wants(bias) ? 4 : 0) | (wants(res) ? 8 : 0);
     Tensor slope;
-    const Tensor y = launch_linear(a, x, act != NSA_ACT_NONE && (need & 7) ? &slope : nullptr);
+    const Tensor y = launch_linear(a, x, act != NSA_ACT_NONE && (x.requires_grad() || w.requires_grad() || wants(bias)) ? &slope : nullptr);
     ctx->save_for_backward({x, w, slope});
-    ctx->saved_data["need"] = need;
+    ctx->saved_data["present"] = (int64_t)(3 | (given(bias) ? 4 : 0) | (given(res) ? 8 : 0));
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &slope = saved[2];
-    const int64_t need = ctx->saved_data["need"].toInt();
+    const int64_t need = asked(ctx, ctx->saved_data["present"].toInt());
     const c10::cuda::CUDAGuard guard(x.device());
     const Tensor dy = grads[0].contiguous();
     Tensor dx, dw, db;
@@ -406,16 +419,15 @@ Tensor launch_mlp(nsa_gated_mlp_args a, const Tensor& x, Tensor* kept) {
 struct GatedMlp : Function<GatedMlp> {
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, const optional<Tensor>& res, int64_t act) {
     const nsa_gated_mlp_args a = check_mlp(x, wg, wu, wd, res, act);
-    const int64_t need = (x.requires_grad() ? 1 : 0) | (wg.requires_grad() ? 2 : 0) | (wu.requires_grad() ? 4 : 0) | (wd.requires_grad() ? 8 : 0) | (wants(res) ? 16 : 0);
     Tensor kept[4];
-    const Tensor y = launch_mlp(a, x, need & 15 ? kept : nullptr);
+    const Tensor y = launch_mlp(a, x, x.requires_grad() || wg.requires_grad() || wu.requires_grad() || wd.requires_grad() ? kept : nullptr);
     ctx->save_for_backward({x, wg, wu, wd, kept[0], kept[1], kept[2], kept[3]});
-    ctx->saved_data["need"] = need;
+    ctx->saved_data["present"] = (int64_t)(15 | (given(res) ? 16 : 0));
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto s = ctx->get_saved_variables();
-    const int64_t need = ctx->saved_data["need"].toInt();
+    const int64_t need = asked(ctx, ctx->saved_data["present"].toInt());
     const c10::cuda::CUDAGuard guard(s[0].device());
     const Tensor dy = grads[0].contiguous();
     Tensor d[4];

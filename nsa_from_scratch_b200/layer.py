@@ -151,6 +151,15 @@ class NSABlock(nn.Module):
         self.rope_base = rope_base
         self._inv_freq: Optional[Tensor] = None              # fp64, and stays that when the module is cast
 
+    def _frequencies(self, device: torch.device) -> Tensor:
+        if self._inv_freq is not None and self._inv_freq.device == device:
+            return self._inv_freq
+        with torch.inference_mode(False):                    # a later training step saves it for its backward
+            f = rope_frequencies(self.attn.head_dim, self.rope_base, device)
+        if not torch.cuda.is_current_stream_capturing():     # in a capture it holds nothing until the replay
+            self._inv_freq = f
+        return f
+
     def new_cache(self, batch: int, max_len: int) -> KVCache:
         a = self.attn
         return KVCache(batch, a.n_kv_heads, a.head_dim, max_len, a.nsa_cfg, dtype=a.q_proj.weight.dtype, device=a.q_proj.weight.device)
@@ -159,15 +168,14 @@ class NSABlock(nn.Module):
         """x [B,T,hidden]; positions [axes,B,T] int32 or int64 (None, with one axis: 0..T-1, or the T positions behind what
         `cache` holds).  cache (decoding, under torch.no_grad()): the step's keys and values are appended to it."""
         B, T, _ = x.shape
-        if self._inv_freq is None or self._inv_freq.device != x.device:
-            self._inv_freq = rope_frequencies(self.attn.head_dim, self.rope_base, x.device)
+        inv_freq = self._frequencies(x.device)
         if positions is None:
             if len(self.rope_sections) != 1:
                 raise ValueError(f"NSABlock: {len(self.rope_sections)} position axes need positions")
             start = 0 if cache is None else cache.length
             positions = torch.arange(start, start + T, device=x.device).expand(1, B, T).contiguous()
         h = rms_norm(x, self.attn_norm, eps=self.eps)
-        a = self.attn.attend(h, positions, self._inv_freq, self.rope_sections, cache=cache)
+        a = self.attn.attend(h, positions, inv_freq, self.rope_sections, cache=cache)
         h, x = rms_norm(a, self.mlp_norm, residual=x, eps=self.eps)
         return gated_mlp(h, self.gate_proj.weight, self.up_proj.weight, self.down_proj.weight, activation=self.activation, residual=x)
 

@@ -316,6 +316,66 @@ def test_no_second_differentiation(nsa):
         g.sum().backward()
 
 
+def test_no_second_differentiation_of_any(nsa):
+    x, s, w = randn(8, 64, seed=1).requires_grad_(True), randn(64, 64, seed=2), randn(64, seed=3)
+    q = randn(1, 8, 2, 64, seed=4).requires_grad_(True)
+    pos, inv = torch.arange(8, device="cuda").view(1, 1, 8), nsa.rope_frequencies(64)
+    for leaf, out in ((x, lambda: nsa.rms_norm(x, w)), (x, lambda: nsa.rms_norm(x, w, residual=x)[0]), (x, lambda: nsa.gated_mlp(x, s, s, s)),
+                      (q, lambda: nsa.rope_axes_to_heads(q, q, q, pos, inv, (32,))[1])):
+        g, = torch.autograd.grad(out().float().square().sum(), leaf, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            g.sum().backward()
+
+
+def test_only_the_gradients_asked_for(nsa):
+    """torch.autograd.grad for some of the inputs: the same values, and no memory for the others' gradients."""
+    x, dy = randn(48, 64, seed=1).requires_grad_(True), randn(48, 4096, seed=2)
+    w, b = randn(4096, 64, seed=3).requires_grad_(True), randn(4096, seed=4).requires_grad_(True)
+    wg, wu, wd = (randn(4096, 64, seed=5 + i).requires_grad_(True) for i in range(3))
+    wd = wd.detach().T.contiguous().requires_grad_(True)
+    for y, leaves, d in ((nsa.linear(x, w, b), (x, w, b), dy), (nsa.gated_mlp(x, wg, wu, wd), (x, wg, wu, wd), randn(48, 64, seed=9))):
+        every = torch.autograd.grad(y, leaves, d, retain_graph=True)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        torch.autograd.grad(y, leaves, d, retain_graph=True)
+        most = torch.cuda.max_memory_allocated() - before
+        for leaf, want in zip(leaves, every):
+            torch.cuda.reset_peak_memory_stats()
+            got, = torch.autograd.grad(y, leaf, d, retain_graph=True)
+            assert torch.equal(got, want)
+            assert torch.cuda.max_memory_allocated() - before < most
+
+
+def test_block_first_used_in_inference_mode_then_trained(nsa):
+    blk = nsa.NSABlock(64, 2, 64, nsa.NSAConfig(block_size_c=64, top_k=2, window_size=64), 96, n_kv_heads=1).cuda().bfloat16()
+    x = randn(1, 70, 64, seed=1)
+    with torch.inference_mode():
+        first = blk(x)
+    blk(x).float().square().mean().backward()
+    assert blk.gate_proj.weight.grad is not None and torch.equal(blk(x).detach(), blk(x).detach())
+    assert torch.isfinite(first).all()
+
+
+def test_block_first_used_in_a_capture(nsa):
+    """A block whose first call is captured: what it makes for itself there is filled at replay, and is no eager call's."""
+    cfg = nsa.NSAConfig(block_size_c=64, top_k=2, window_size=64)
+    blk = nsa.NSABlock(64, 2, 64, cfg, 96, n_kv_heads=1).cuda().bfloat16()
+    twin = nsa.NSABlock(64, 2, 64, cfg, 96, n_kv_heads=1).cuda().bfloat16()
+    twin.load_state_dict(blk.state_dict())
+    x = randn(1, 70, 64, seed=1)
+    pos = torch.arange(70, device="cuda").view(1, 1, 70)
+    with torch.no_grad():
+        want = twin(x, pos)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = blk(x, pos)
+        assert torch.equal(blk(x, pos), want)              # before any replay
+        g.replay()
+        assert torch.equal(y, want)
+
+
 def test_status_word_of_the_products(nsa):
     from nsa_from_scratch_b200 import _lib as L, ops
     lib = L.load()
