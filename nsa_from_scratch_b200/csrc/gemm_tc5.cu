@@ -20,8 +20,10 @@
 //
 // Measured: 8192 x 9216 x 8192 e4m3 404 us = 3.06 PFLOP/s (tensor pipe busy 90 %); the gated pair of 2048 x 11008 x 4096 bf16 235 us =
 // 1.57 PFLOP/s (85 %) and of 8192 x 22016 x 8192 at the board's power limit, 1.39 PFLOP/s for the whole block; both gradients of
-// 4001 x 4096 x 4096 in one launch 171 us = 1.57 PFLOP/s (86 %).  With a contraction of only 16 steps the epilogue shows: the gated pair
-// of 8191 x 2816 x 1024 that keeps its factors takes 88 us (55 %), the product that forms their gradients 64 us (35 %).
+// 4001 x 4096 x 4096 in one launch 171 us = 1.57 PFLOP/s (86 %).  With a contraction of only 16 steps the results' way out shows: the
+// gated pair of 8191 x 2816 x 1024 takes 64 us, and 88 (55 %) when it keeps its factors, the product that forms their gradients
+// 64 (35 %).  Their epilogues end in time, but 128 KB of results (and 192 of factors) an SM and tile share L2 with 512 KB of
+// operands, whose loads then stall; boxes of 64 instead of 32 columns and stores by the threads instead of TMA measure the same.
 //
 // Every wait is bounded; a wait that gives up raises the CTA's abort flag and the device status word, and the CTA still
 // frees its TMEM.
