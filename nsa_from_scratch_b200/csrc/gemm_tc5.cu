@@ -91,10 +91,10 @@ template <int CG> __device__ __forceinline__ void tm_dealloc(uint32_t taddr, uin
   if constexpr (CG == 2) asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;\n" ::"r"(taddr), "r"(ncols) : "memory");
   else tmem_dealloc(taddr, ncols);
 }
-// one arrival on `bar` (of both CTAs of a pair) when every product issued so far is done
-template <int CG> __device__ __forceinline__ void commit(uint32_t bar) {
+// one arrival on `bar` (of both CTAs of a pair: `first` is the rank of its first) when every product issued so far is done
+template <int CG> __device__ __forceinline__ void commit(uint32_t bar, uint32_t first = 0) {
   if constexpr (CG == 2)
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(bar), "h"((uint16_t)3) : "memory");
+    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n" ::"r"(bar), "h"((uint16_t)(3u << first)) : "memory");
   else tc_commit(bar);
 }
 template <int CG, bool F8>
@@ -528,6 +528,166 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
   if (warp == 2) { tc_fence_after(); tm_dealloc<CG>(tmem, 2 * BN); }
 }
 
+// ---------------------------------------------------------------- few tiles: a cluster shares a tile's contraction
+// The S = p.splits pairs of a cluster each take a part of the contraction of one tile of 256 x 128, and hand the sums round
+// through distributed shared memory: part q writes what it has of the columns of part s, 1/S of the tile's, into s's shared
+// memory; s adds the parts in their order and runs the epilogue on its columns.  One launch, and no sums through L2: 256 x 4096 x
+// 4096 bf16 15.6 us (17.6 through the joining kernel), 256 x 1024 x 1024 7.8 (9.3), 300 x 2048 x 2048 11.1 (12.4).
+struct GemmClusterParams {
+  TcProduct pr;
+  Epi e;
+  int splits, per_split;
+};
+// Tiles of 256 columns would leave room for three stages of the ring, and twice as much to exchange: slower in every case.
+// Single CTAs, for up to 128 rows: 0 to 1 us faster than joining at 4096 x 4096, slower at 1024 x 1024; they keep to that.
+// Sums: 16-byte pieces of 4 columns, a column of 128 rows each (a warp writes 512 bytes in a row), 16 bytes apart for the reading.
+constexpr int CLUSTER_BN = 128;
+struct ClusterShape {
+  static constexpr int A_BYTES = 128 * 128, B_BYTES = CLUSTER_BN / 2 * 128, PIECE = 128 * 16 + 16, SUMS = CLUSTER_BN / 4 * PIECE;
+  static constexpr int STAGES = (229376 - SUMS) / (A_BYTES + B_BYTES), SMEM = STAGES * (A_BYTES + B_BYTES) + SUMS + 1024;
+};
+__device__ __forceinline__ void sts128_cluster(uint32_t a, uint4 v) {
+  asm volatile("st.shared::cluster.v4.u32 [%0], {%1,%2,%3,%4};\n" ::"r"(a), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+
+template <int F, typename T, int MODE>
+__global__ void __launch_bounds__(384, 1) gemm_cluster_kernel(const __grid_constant__ GemmClusterParams p) {
+  using S = ClusterShape;
+  constexpr int CG = 2, BN = CLUSTER_BN;
+  constexpr bool F8 = F >= 2, PAIR = MODE == EPI_GLU;
+  constexpr int KE = F8 ? 128 : 64, NW = PAIR ? BN / 2 : BN, BROWS = BN / CG;
+  constexpr uint32_t IDESC = idesc_f16(F8 ? F - 2 : F, 128 * CG, BN, 0, 0);
+  extern __shared__ unsigned char smem_raw[];
+  const uint32_t s_tiles = (smem_u32(smem_raw) + 1023) & ~1023u, s_sums = s_tiles + S::STAGES * (S::A_BYTES + S::B_BYTES);
+  __shared__ __align__(8) uint64_t full[S::STAGES], empty[S::STAGES], tfull;
+  __shared__ uint32_t tmem_s;
+  __shared__ int abort_flag;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const uint32_t at = cluster_rank(), rank = at & 1, first = at - rank;     // of the pair
+  const int split = (int)at / CG, tile = blockIdx.x / (CG * p.splits);
+  if (tid == 0) {
+    abort_flag = 0;
+    for (int i = 0; i < S::STAGES; ++i) { mbar_init(smem_u32(&full[i]), 1); mbar_init(smem_u32(&empty[i]), 1); }
+    mbar_init(smem_u32(&tfull), 1);
+    fence_barrier_init();
+  }
+  if (warp == 2) tm_alloc<CG>(smem_u32(&tmem_s), BN);
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();                                                        // every CTA's barriers and sums may be written from here on
+  tc_fence_after();
+  const uint32_t tmem = tmem_s;
+  int fail_id = 0;
+  grid_dep_launch();
+  grid_dep_wait();
+
+  const int m0 = tile % p.pr.tiles_m * 128 * CG, n0 = tile / p.pr.tiles_m * NW;
+  const int k0 = split * p.per_split, k1 = min(p.pr.ksteps * p.pr.segments, k0 + p.per_split);
+  const int a_mn = F8 ? 0 : p.pr.a_mn, b_mn = F8 ? 0 : p.pr.b_mn;
+  bool ok = true;
+  if (warp == 0) {
+    // =============================== TMA producer ===============================
+    const bool leader = elect_one();
+    const int ma = m0 + (int)rank * 128, nb = n0 + (int)rank * BROWS;
+    for (int k = k0, it = 0; k < k1; ++k, ++it) {
+      const int s = it % S::STAGES, ph = (it / S::STAGES) & 1;
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[s]), ph ^ 1, &abort_flag));
+      if (!ok) { fail_id = 1; break; }
+      if (leader) {
+        if (rank == 0) mbar_expect_tx(smem_u32(&full[s]), CG * (S::A_BYTES + S::B_BYTES));
+        const uint32_t bar = map_to_rank(smem_u32(&full[s]), first);
+        const int seg = k >= p.pr.ksteps, kc = (k - seg * p.pr.ksteps) * KE;
+        const uint32_t da = s_tiles + s * (S::A_BYTES + S::B_BYTES), db = da + S::A_BYTES;
+        const CUtensorMap *ta = &p.pr.tmA[seg], *tb = &p.pr.tmB[seg];
+        if (a_mn) {
+          tma_load_2d<CG>(da, ta, bar, ma, kc);
+          tma_load_2d<CG>(da + 8192, ta, bar, ma + 64, kc);
+        } else {
+          tma_load_2d<CG>(da, ta, bar, kc, ma);
+        }
+        if constexpr (PAIR) {
+          tma_load_2d<CG>(db, &p.pr.tmB[rank], bar, kc, n0);
+        } else if (b_mn) {
+          tma_load_2d<CG>(db, tb, bar, nb, kc);                          // 64 columns
+        } else {
+          tma_load_2d<CG>(db, tb, bar, kc, nb);
+        }
+      }
+      __syncwarp();
+    }
+  } else if (warp == 1 && rank == 0) {
+    // =============================== MMA issuer ===============================
+    const bool leader = elect_one();
+    const uint32_t idesc = IDESC | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16);
+    const int sa = a_mn ? 128 : 2, sb = b_mn ? 128 : 2;
+    for (int k = k0, it = 0; k < k1; ++k, ++it) {
+      const int s = it % S::STAGES, ph = (it / S::STAGES) & 1;
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&full[s]), ph, &abort_flag));
+      if (!ok) { fail_id = 3; break; }
+      tc_fence_after();
+      if (leader) {
+        const uint32_t da = s_tiles + s * (S::A_BYTES + S::B_BYTES);
+        const uint64_t a = smem_desc_sw128(da, a_mn ? 8192 : 16, 1024), b = smem_desc_sw128(da + S::A_BYTES, b_mn ? 8192 : 16, 1024);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) mma<CG, F8>(tmem, a + i * sa, b + i * sb, idesc, (it > 0 || i > 0) ? 1u : 0u);
+        commit<CG>(smem_u32(&empty[s]), first);
+      }
+      __syncwarp();
+    }
+    if (ok && leader) commit<CG>(smem_u32(&tfull), first);
+    __syncwarp();
+  }
+
+  // =============================== the sums go round ===============================
+  const int own = NW / p.splits, pieces = BN / p.splits / 4;             // result columns of a part; pieces of a row of its sums
+  auto slot = [&](int from, int piece, int row) { return s_sums + (from * pieces + piece) * S::PIECE + row * 16; };
+  if (warp >= 4) {
+    const int quarter = warp & 3, row = quarter * 32 + lane;
+    const uint32_t acc = tmem + ((uint32_t)(quarter * 32) << 16);
+    ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&tfull), 0, &abort_flag));
+    if (!ok) fail_id = 4;
+    tc_fence_after();
+#pragma unroll 1
+    for (int i = (warp - 4) >> 2; ok && i < BN / 16; i += 2) {
+      const int half = PAIR ? i / (NW / 16) : 0, col = i * 16 - half * NW, to = col / own;
+      uint32_t v[16];
+      tmem_ld16(acc + i * 16, v);
+      tc_wait_ld();
+      const uint32_t base = map_to_rank(slot(split, (half * own + col - to * own) / 4, row), (uint32_t)(to * CG) + rank);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) sts128_cluster(base + j * S::PIECE, make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]));
+    }
+  }
+  __syncwarp();
+  cluster_sync();
+  if (warp >= 4 && ok) {
+    const int groups = own / 8;                                          // of 8 columns: neighbouring threads share a row
+#pragma unroll 1
+    for (int i = tid - 128; i < 128 * groups; i += 256) {
+      const int row = i / groups, g = i % groups;
+      float a[8] = {}, b[8] = {};
+      auto add = [&](float (&sum)[8], int q, int piece) {
+        const uint4 lo = lds128(slot(q, piece, row)), hi = lds128(slot(q, piece + 1, row));
+        sum[0] += __uint_as_float(lo.x); sum[1] += __uint_as_float(lo.y); sum[2] += __uint_as_float(lo.z); sum[3] += __uint_as_float(lo.w);
+        sum[4] += __uint_as_float(hi.x); sum[5] += __uint_as_float(hi.y); sum[6] += __uint_as_float(hi.z); sum[7] += __uint_as_float(hi.w);
+      };
+      for (int q = 0; q < p.splits; ++q) {
+        add(a, q, 2 * g);
+        if constexpr (PAIR) add(b, q, own / 4 + 2 * g);
+      }
+      epilogue8<T, MODE>(p.e, m0 + (int)rank * 128 + row, n0 + split * own + 8 * g, a, b);
+    }
+  }
+
+  if (fail_id != 0) atomicCAS(&g_gemm_status, 0, fail_id);
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (abort_flag) __nanosleep(1000000);                                  // copies still under way land long before this
+  cluster_sync();
+  if (warp == 2) { tc_fence_after(); tm_dealloc<CG>(tmem, BN); }
+}
+
 // Joins the partial sums of a split contraction, in split order, and runs the epilogue: 8 columns a thread.
 template <typename T, int MODE>
 __global__ void __launch_bounds__(256) gemm_join_kernel(const float* __restrict__ part, const Epi e, int splits, int ldp) {
@@ -608,7 +768,34 @@ static int esize(int dtype) { return dtype == NSA_BF16 || dtype == NSA_FP16 ? 2 
 
 // Which kernel, how many ways the contraction is split, and whether the sums leave raw: where they are split, or where
 // the results' rows do not start on 16-byte boundaries (TMA writes them).
-struct TcPlan { int cg, bn, tiles_m, tiles_n, ksteps, splits, per_split; bool raw; };
+struct TcPlan { int cg, bn, tiles_m, tiles_n, ksteps, splits, per_split; bool raw, cluster; };
+
+// How many clusters of `size` CTAs the device holds at a time, a CTA to an SM
+static int cluster_room(int size) {
+  static int known[64][2];                      // clusters of 4 and of 8; 0: not asked yet
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 0;
+  int* slot = dev < 64 ? &known[dev][size == 8] : nullptr;
+  if (slot != nullptr && *slot != 0) return *slot > 0 ? *slot : 0;
+  auto fn = gemm_cluster_kernel<1, __nv_bfloat16, EPI_LINEAR>;
+  const int smem = ClusterShape::SMEM;
+  int n = 0;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(size * 64);
+  cfg.blockDim = dim3(384);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute at;
+  at.id = cudaLaunchAttributeClusterDimension;
+  at.val.clusterDim.x = size; at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess) {
+    cudaGetLastError();                         // no device here, or none that takes them: the other forms remain
+    n = 0;
+  }
+  if (slot != nullptr) *slot = n > 0 ? n : -1;
+  return n;
+}
 static TcPlan tc_plan(const GemmProblem& p, bool whole = false) {     // whole: pairs on 256 columns, unsplit
   TcPlan t;
   const int pair = p.e.mode == EPI_GLU ? 2 : 1;
@@ -637,8 +824,26 @@ static TcPlan tc_plan(const GemmProblem& p, bool whole = false) {     // whole: 
       }
     }
   }
+  t.cluster = false;
+  // A cluster's parts exchange their sums on chip (5000 clk: from the times above the kernel); all clusters have to be
+  // resident at once, and a part without work would have no sums.
+  if (!whole && p.M > 128) {
+    const int tm = (p.M + 255) / 256, tn = (p.N + CLUSTER_BN / pair - 1) / (CLUSTER_BN / pair);
+    for (int s = 2; s <= 4; s *= 2) {
+      const int per = (steps + s - 1) / s;
+      if ((s - 1) * per >= steps || (long long)tm * tn > cluster_room(2 * s)) continue;
+      const double cost = (double)per * 384 + 5000;
+      if (cost < best) {
+        best = cost;
+        t.cluster = true;
+        t.cg = 2; t.bn = CLUSTER_BN;
+        t.tiles_m = tm; t.tiles_n = tn;
+        t.splits = s; t.per_split = per;
+      }
+    }
+  }
   t.ksteps = ksteps;
-  t.raw = raw || t.splits > 1;
+  t.raw = !t.cluster && (raw || t.splits > 1);
   return t;
 }
 
@@ -674,6 +879,48 @@ static int tc_launch(const GemmTcParams& g, cudaStream_t st) {
   const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, g);
   if (e != cudaSuccess) return fail(NSA_ERR_CUDA, "gemm_tc5 launch failed: %s", cudaGetErrorString(e));
   return NSA_OK;
+}
+
+template <int F, typename T, int MODE>
+static int cluster_launch(const GemmClusterParams& g, cudaStream_t st) {
+  auto fn = gemm_cluster_kernel<F, T, MODE>;
+  constexpr int smem = ClusterShape::SMEM;
+  static bool prepared[64];
+  int dev = 0;
+  NSA_CUDA_OK(cudaGetDevice(&dev));
+  if (dev >= 64 || !prepared[dev]) {
+    NSA_CUDA_OK(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    if (dev < 64) prepared[dev] = true;
+  }
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(g.pr.tiles_m * g.pr.tiles_n * 2 * g.splits));
+  cfg.blockDim = dim3(384);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = 2 * g.splits; at[1].val.clusterDim.y = 1; at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  const cudaError_t e = cudaLaunchKernelEx(&cfg, fn, g);
+  if (e != cudaSuccess) return fail(NSA_ERR_CUDA, "gemm_cluster launch failed: %s", cudaGetErrorString(e));
+  return NSA_OK;
+}
+template <int F, typename T>
+static int cluster_mode(const GemmClusterParams& g, cudaStream_t st) {
+  if constexpr (F < 2) {
+    if (g.e.mode == EPI_GLU) return cluster_launch<F, T, EPI_GLU>(g, st);
+    if (g.e.mode == EPI_GLU_BWD) return cluster_launch<F, T, EPI_GLU_BWD>(g, st);
+  }
+  return cluster_launch<F, T, EPI_LINEAR>(g, st);
+}
+static int cluster_types(const GemmClusterParams& g, int dtype, bool bf, cudaStream_t st) {
+  if (dtype == NSA_BF16) return cluster_mode<1, __nv_bfloat16>(g, st);
+  if (dtype == NSA_FP16) return cluster_mode<0, __half>(g, st);
+  if (dtype == NSA_FP8_E4M3) return bf ? cluster_mode<2, __nv_bfloat16>(g, st) : cluster_mode<2, __half>(g, st);
+  return bf ? cluster_mode<3, __nv_bfloat16>(g, st) : cluster_mode<3, __half>(g, st);
 }
 
 template <int F, typename T, int MODE>
@@ -734,9 +981,17 @@ int gemm_tc5(const GemmProblem& p, void* ws, cudaStream_t st) {
   const TcPlan t = tc_plan(p);
   const long long tiles = (long long)t.tiles_m * t.tiles_n * t.splits;
   NSA_REQUIRE(tiles < 2147483647LL - 65536, NSA_ERR_ARG, "matrix product: %d x %d results are too many tiles", p.M, p.N);
+  int rc;
+  const bool bf = p.out_dtype == NSA_BF16;
+  if (t.cluster) {
+    GemmClusterParams c;
+    if ((rc = tc_product(&c.pr, p, t)) != NSA_OK) return rc;
+    c.e = p.e;
+    c.splits = t.splits; c.per_split = t.per_split;
+    return cluster_types(c, p.dtype, bf, st);
+  }
   GemmTcParams g;
-  int rc = tc_product(&g.pr[0], p, t);
-  if (rc != NSA_OK) return rc;
+  if ((rc = tc_product(&g.pr[0], p, t)) != NSA_OK) return rc;
   const bool gated = p.e.mode != EPI_LINEAR, slope = !gated && p.e.o1 != nullptr;
   if (t.raw) {
     if ((rc = map_part(&g.tmPart, ws, (p.e.mode == EPI_GLU ? 2 : 1) * t.splits, p.M, p.N)) != NSA_OK) return rc;
@@ -754,7 +1009,6 @@ int gemm_tc5(const GemmProblem& p, void* ws, cudaStream_t st) {
   g.e = p.e;
   g.products = 1; g.tiles = (int)tiles;
   g.splits = t.splits; g.per_split = t.per_split;
-  const bool bf = p.out_dtype == NSA_BF16;
   const int mode = t.raw ? (p.e.mode == EPI_GLU ? EPI_PARTIAL2 : EPI_PARTIAL) : slope ? EPI_SLOPE : p.e.mode;
   rc = tc_types(g, t, mode, p.dtype, bf, st);
   if (rc != NSA_OK || !t.raw) return rc;

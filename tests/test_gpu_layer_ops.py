@@ -475,6 +475,29 @@ def test_gated_mlp_difference_quotient(nsa):
         assert abs(float((g.double() * v).sum()) - want) <= 3 * 2.0 ** -11 * float((g.double() * v).abs().sum()) + 1e-6
 
 
+# ---------------------------------------------------------------- few tiles, long contractions
+
+@pytest.mark.parametrize("M,N,K", [(129, 136, 1024), (200, 1160, 1000), (256, 1024, 1024), (300, 264, 2056), (150, 33, 999), (512, 520, 776), (256, 128, 320),
+                                   (257, 2048, 4096), (1024, 1024, 1024), (131, 1, 8192)])
+def test_few_tiles(nsa, M, N, K):
+    """Shapes whose contraction is split over the CTAs of a cluster, evenly or not, with ragged tiles and rows off the
+    16-byte grid: every epilogue, the gradients (operands of the other majorness) and fp8."""
+    test_linear(nsa, M, N, K, torch.bfloat16, True, "silu", True)
+    test_linear(nsa, M, N, K, torch.float16, False, None, False)
+    test_linear_fp8(nsa, M, N, K, torch.float8_e4m3fn, torch.bfloat16, True, None, True)
+    test_linear_fp8(nsa, M, N, K, torch.float8_e5m2, torch.float16, False, "silu", False)
+    test_linear_backward(nsa, M, N, K, torch.float16, True, "gelu_tanh", True)
+    test_linear_backward(nsa, M, N, K, torch.bfloat16, False, None, False)
+
+
+@pytest.mark.parametrize("M,N,F", [(129, 1024, 264), (200, 256, 700), (300, 2056, 136), (256, 768, 2048), (150, 999, 33)])
+def test_few_tiles_of_a_gated_block(nsa, M, N, F):
+    test_gated_mlp(nsa, M, N, F, torch.bfloat16, "silu", True)
+    test_gated_mlp(nsa, M, N, F, torch.float16, None, False)
+    test_gated_mlp_backward(nsa, M, N, F, torch.float16, "gelu_tanh", False)
+    test_gated_mlp_backward(nsa, M, N, F, torch.bfloat16, "relu", True)
+
+
 # ---------------------------------------------------------------- refusals
 
 def test_refusals(nsa):
