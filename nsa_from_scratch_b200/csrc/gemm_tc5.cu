@@ -532,7 +532,8 @@ __global__ void __launch_bounds__(384, 1) gemm_tc5_kernel(const __grid_constant_
 // The S = p.splits pairs of a cluster each take a part of the contraction of one tile of 256 x 128, and hand the sums round
 // through distributed shared memory: part q writes what it has of the columns of part s, 1/S of the tile's, into s's shared
 // memory; s adds the parts in their order and runs the epilogue on its columns.  One launch, and no sums through L2: 256 x 4096 x
-// 4096 bf16 15.6 us (17.6 through the joining kernel), 256 x 1024 x 1024 7.8 (9.3), 300 x 2048 x 2048 11.1 (12.4).
+// 4096 bf16 15.1 us (17.8 through the joining kernel), 256 x 1024 x 1024 7.7 (9.3), 1024 x 1024 x 1024 8.8 (9.8 whole), 300 x 2048 x
+// 2048 11.1 (12.4).
 struct GemmClusterParams {
   TcProduct pr;
   Epi e;
