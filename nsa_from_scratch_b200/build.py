@@ -105,7 +105,7 @@ def build_torch(force: bool = False) -> str:
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
            *(f"-I{d}" for d in (os.path.join(home, "include"), os.path.join(home, "include/torch/csrc/api/include"), os.path.join(cuda, "include"),
                                 sysconfig.get_paths()["include"])),
-           TORCH_SRC, "-o", part, f"-L{home}/lib", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python", f"-L{PKG}",
+           TORCH_SRC, "-o", part, f"-L{home}/lib", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python", f"-L{PKG}",
            "-Xlinker", "-l:libnsa_b200.so", "-Xlinker", "-rpath,$ORIGIN"]
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:

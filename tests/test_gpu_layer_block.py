@@ -376,6 +376,34 @@ def test_block_first_used_in_a_capture(nsa):
         assert torch.equal(y, want)
 
 
+def test_first_calls_of_a_process_captured(nsa):
+    """Nothing that an operator sets up for itself on its first call stands in the way of a capture."""
+    code = textwrap.dedent("""
+        import torch, nsa_from_scratch_b200 as nsa
+        torch.manual_seed(0)
+        bf = dict(device="cuda", dtype=torch.bfloat16)
+        x, few, w, norm = torch.randn(256, 512, **bf), torch.randn(8, 512, **bf), torch.randn(512, 512, **bf) / 24, torch.ones(512, **bf)
+        wg, wu, wd = torch.randn(1408, 512, **bf) / 24, torch.randn(1408, 512, **bf) / 24, torch.randn(512, 1408, **bf) / 38
+        q, pos, inv = torch.randn(2, 128, 4, 64, **bf), torch.arange(128, device="cuda").repeat(1, 2, 1), nsa.rope_frequencies(64)
+        torch.cuda.synchronize()
+        def run():
+            h, r = nsa.rms_norm(x, norm, residual=x)
+            a = nsa.linear(h, w, residual=r)
+            (e, es), (k, ks) = nsa.rms_norm_fp8(x, norm), nsa.quantize_rows_to_fp8(w)
+            return (a, nsa.gated_mlp(a, wg, wu, wd, residual=a), nsa.linear(few, w), nsa.gated_mlp(few, wg, wu, wd), nsa.linear_fp8(e, k, es, ks),
+                    *nsa.rope_axes_to_heads(q, q, q, pos, inv, (32,)))
+        with torch.no_grad():
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                got = run()
+            g.replay()
+            torch.cuda.synchronize()
+            print("SAME", all(torch.equal(a, b) for a, b in zip(got, run())))
+    """)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300, cwd=__file__.rsplit("/tests/", 1)[0])
+    assert r.returncode == 0 and "SAME True" in r.stdout, (r.returncode, r.stdout[-500:], r.stderr[-1500:])
+
+
 def test_status_word_of_the_products(nsa):
     from nsa_from_scratch_b200 import _lib as L, ops
     lib = L.load()
