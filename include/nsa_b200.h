@@ -441,8 +441,9 @@ int nsa_select_blocks_cached(const void* Qb, const void* Kb, int32_t* idx, int B
 /* ---------------------------------------------------------------- the layer around the attention
  * What a decoder layer computes before, between and after its attention calls (the reference leaves these to plain
  * torch modules, nsa/model/llama_dense.py:19-134): norm, rotary embedding, projections, gated feed-forward block.
- * Rows are dense; pointers may have any alignment (16-byte aligned rows take the fast kernels).  Workspaces are
- * device memory, 256-byte aligned, contents free before and after. */
+ * Rows are dense; pointers need no more than their elements' alignment (16-byte aligned rows take the fast kernels).
+ * Workspaces are device memory, 256-byte aligned, contents free before and after.  Pointers and workspaces off
+ * these alignments are refused. */
 #define NSA_ACT_NONE 0
 #define NSA_ACT_SILU 1
 #define NSA_ACT_GELU_TANH 2 /* 0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */
@@ -521,7 +522,7 @@ int64_t nsa_linear_ws_bytes(const nsa_linear_args* args);
 int nsa_linear(const nsa_linear_args* args, nsa_stream_t stream);
 
 /* Gradients of nsa_linear (16-bit operands): dx [M,K], dw [N,K], dbias [N], each NULL if not wanted; residual's is dy.  has_act: an
- * activation stood in the forward, and slope holds what it kept (NULL otherwise).  Repeats bit for bit. */
+ * activation stood in the forward, and slope holds what it kept (NULL otherwise).  ws as for nsa_linear.  Repeats bit for bit. */
 typedef struct nsa_linear_bwd_args {
   const void *dy, *x, *w, *slope;
   void *dx, *dw, *dbias, *ws;
@@ -546,7 +547,8 @@ typedef struct nsa_gated_mlp_args {
 int64_t nsa_gated_mlp_ws_bytes(const nsa_gated_mlp_args* args);
 int nsa_gated_mlp(const nsa_gated_mlp_args* args, nsa_stream_t stream);
 
-/* Its gradients, from what the forward kept: dx [M,N], dwg and dwu [F,N], dwd [N,F], each NULL if not wanted; residual's is dy.  Repeats bit for bit. */
+/* Its gradients, from what the forward kept: dx [M,N], dwg and dwu [F,N], dwd [N,F], each NULL if not wanted; residual's is dy.
+ * ws as for nsa_linear.  Repeats bit for bit. */
 typedef struct nsa_gated_mlp_bwd_args {
   const void *dy, *x, *wg, *wu, *wd, *p, *s, *low, *h;
   void *dx, *dwg, *dwu, *dwd, *ws;

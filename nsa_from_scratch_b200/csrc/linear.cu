@@ -114,11 +114,14 @@ static int run_steps(const char* what, const Args& a, int (*steps)(const Args&, 
   if (rc != NSA_OK) return rc;
   const long long need = count.bytes();
   NSA_REQUIRE(a.ws_bytes >= need && (a.ws != nullptr || need == 0), NSA_ERR_ARG, "%s: workspace of %lld bytes, %lld needed", what, (long long)a.ws_bytes, need);
+  NSA_REQUIRE(need == 0 || (reinterpret_cast<uintptr_t>(a.ws) & 255) == 0, NSA_ERR_ARG, "%s: the workspace is not 256-byte aligned", what);
   static unsigned char none[16];     // stands for a workspace of no bytes
   Arena w{a.ws != nullptr ? reinterpret_cast<unsigned char*>(a.ws) : none, count.at, st};
   return steps(a, w);
 }
 
+// Every pointer given lies on a multiple of `size`: what no kernel can do without, whichever path it takes
+template <typename... P> static bool on(int size, const P*... p) { return ((reinterpret_cast<uintptr_t>(p) % size == 0) && ...); }
 static bool is16(int dt) { return dt == NSA_BF16 || dt == NSA_FP16; }
 static bool is8(int dt) { return dt == NSA_FP8_E4M3 || dt == NSA_FP8_E5M2; }
 static int elem(int dt) { return is16(dt) ? 2 : 1; }
@@ -233,6 +236,7 @@ int linear(const nsa_linear_args& a, cudaStream_t st) {
   NSA_REQUIRE(a.x && a.w && a.y, NSA_ERR_ARG, "linear: NULL pointer");
   NSA_REQUIRE(is8(a.dtype) == (a.x_scale != nullptr) && is8(a.dtype) == (a.w_scale != nullptr), NSA_ERR_ARG, "linear: fp8 operands, and only they, have scales");
   NSA_REQUIRE(a.slope == nullptr || (is16(a.dtype) && a.act != NSA_ACT_NONE), NSA_ERR_ARG, "linear: only an activation of 16-bit operands leaves a slope");
+  NSA_REQUIRE(on(elem(a.dtype), a.x, a.w) && on(2, a.bias, a.residual, a.y, a.slope) && on(4, a.x_scale, a.w_scale), NSA_ERR_ARG, "linear: a pointer is not aligned to its elements");
   return run_steps("linear", a, linear_steps, st);
 }
 
@@ -275,6 +279,7 @@ int linear_bwd(const nsa_linear_bwd_args& a, cudaStream_t st) {
     return zero(a.dbias, (long long)a.N * 2, st);
   }
   NSA_REQUIRE(a.dy && a.x && a.w && (a.slope != nullptr) == (a.has_act != 0), NSA_ERR_ARG, "linear backward: NULL pointer");
+  NSA_REQUIRE(on(2, a.dy, a.x, a.w, a.slope, a.dx, a.dw, a.dbias), NSA_ERR_ARG, "linear backward: a pointer is not aligned to its elements");
   return run_steps("linear backward", a, linear_bwd_steps, st);
 }
 
@@ -325,6 +330,7 @@ int gated_mlp(const nsa_gated_mlp_args& a, cudaStream_t st) {
   NSA_REQUIRE((a.p == nullptr) == (a.s == nullptr) && (a.p == nullptr) == (a.low == nullptr) && (a.p == nullptr) == (a.h == nullptr), NSA_ERR_ARG,
               "gated_mlp: give all of p, s, low and h or none");
   NSA_REQUIRE(aligned16(a.p) && aligned16(a.s) && aligned16(a.low) && aligned16(a.h), NSA_ERR_ARG, "gated_mlp: p, s, low and h must be 16-byte aligned");
+  NSA_REQUIRE(on(2, a.x, a.wg, a.wu, a.wd, a.residual, a.y), NSA_ERR_ARG, "gated_mlp: a pointer is not aligned to its elements");
   return run_steps("gated_mlp", a, mlp_steps, st);
 }
 
@@ -366,6 +372,7 @@ int gated_mlp_bwd(const nsa_gated_mlp_bwd_args& a, cudaStream_t st) {
   }
   NSA_REQUIRE(a.dy && a.x && a.wg && a.wu && a.wd && a.p && a.s && a.low && a.h, NSA_ERR_ARG, "gated_mlp backward: NULL pointer");
   NSA_REQUIRE(aligned16(a.p) && aligned16(a.s) && aligned16(a.low) && aligned16(a.h), NSA_ERR_ARG, "gated_mlp backward: p, s, low and h must be 16-byte aligned");
+  NSA_REQUIRE(on(2, a.dy, a.x, a.wg, a.wu, a.wd, a.dx, a.dwg, a.dwu, a.dwd), NSA_ERR_ARG, "gated_mlp backward: a pointer is not aligned to its elements");
   return run_steps("gated_mlp backward", a, mlp_bwd_steps, st);
 }
 
@@ -376,6 +383,7 @@ int quantize_rows(const void*, void*, float*, long long, int, int, int, cudaStre
 int rope_axes(const nsa_rope_axes_args&, cudaStream_t);
 
 static bool is_real(int dt) { return is16(dt) || dt == NSA_FP32; }
+static int bytes_of(int dt) { return dt == NSA_FP32 ? 4 : elem(dt); }
 
 }  // namespace nsa
 
@@ -395,6 +403,9 @@ int nsa_rms_norm(const nsa_norm_args* a, nsa_stream_t stream) {
               a->res_dtype, a->x_dtype);
   if (a->rows == 0) return NSA_OK;
   NSA_REQUIRE(a->x && a->weight && a->y && (a->scale != nullptr || !is8(a->y_dtype)), NSA_ERR_ARG, "rms_norm: NULL pointer");
+  NSA_REQUIRE(on(bytes_of(a->x_dtype), a->x) && on(bytes_of(a->y_dtype), a->y) && on(bytes_of(a->w_dtype), a->weight) &&
+                  (a->residual == nullptr || on(bytes_of(a->res_dtype), a->residual, a->h)) && on(4, a->scale, a->rstd),
+              NSA_ERR_ARG, "rms_norm: a pointer is not aligned to its elements");
   return rms_norm(*a, (cudaStream_t)stream);
 }
 
@@ -412,6 +423,9 @@ int nsa_rms_norm_bwd(const nsa_norm_bwd_args* a, nsa_stream_t stream) {
   NSA_REQUIRE(a->dy && a->h && a->weight && a->rstd && a->dx && a->ws, NSA_ERR_ARG, "rms_norm backward: NULL pointer");
   const long long need = rms_norm_bwd_ws_bytes(a->rows, a->hidden);
   NSA_REQUIRE(a->ws_bytes >= need, NSA_ERR_ARG, "rms_norm backward: workspace of %lld bytes, %lld needed", (long long)a->ws_bytes, need);
+  NSA_REQUIRE((reinterpret_cast<uintptr_t>(a->ws) & 255) == 0, NSA_ERR_ARG, "rms_norm backward: the workspace is not 256-byte aligned");
+  NSA_REQUIRE(on(bytes_of(a->x_dtype), a->dy, a->dx) && on(bytes_of(a->res_dtype), a->dh, a->h, a->dres) && on(bytes_of(a->w_dtype), a->weight, a->dweight) && on(4, a->rstd),
+              NSA_ERR_ARG, "rms_norm backward: a pointer is not aligned to its elements");
   return rms_norm_bwd(*a, (cudaStream_t)stream);
 }
 
@@ -421,6 +435,7 @@ int nsa_quantize_rows_fp8(const void* x, void* q, float* scale, int64_t rows, in
   NSA_REQUIRE(is8(fmt), NSA_ERR_ARG, "quantize_rows: format %d", fmt);
   if (rows == 0) return NSA_OK;
   NSA_REQUIRE(x && q && scale, NSA_ERR_ARG, "quantize_rows: NULL pointer");
+  NSA_REQUIRE(on(bytes_of(x_dtype), x) && on(4, scale), NSA_ERR_ARG, "quantize_rows: a pointer is not aligned to its elements");
   return quantize_rows(x, q, scale, rows, n, x_dtype, fmt, (cudaStream_t)stream);
 }
 
@@ -442,6 +457,9 @@ int nsa_rope_axes(const nsa_rope_axes_args* a, nsa_stream_t stream) {
   NSA_REQUIRE(a->q && a->k && a->v && a->q_out && a->k_out && a->v_out && a->positions && a->inv_freq, NSA_ERR_ARG, "rope_axes: NULL pointer");
   NSA_REQUIRE(a->q_batch >= 0 && a->q_token >= 0 && a->k_batch >= 0 && a->k_token >= 0 && a->v_batch >= 0 && a->v_token >= 0, NSA_ERR_ARG,
               "rope_axes: negative pitch");
+  const int in = bytes_of(a->backward ? a->y_dtype : a->x_dtype), out = bytes_of(a->backward ? a->x_dtype : a->y_dtype);
+  NSA_REQUIRE(on(in, a->q, a->k, a->v) && on(out, a->q_out, a->k_out, a->v_out) && on(a->pos64 ? 8 : 4, a->positions) && on(8, a->inv_freq), NSA_ERR_ARG,
+              "rope_axes: a pointer is not aligned to its elements");
   return rope_axes(*a, (cudaStream_t)stream);
 }
 

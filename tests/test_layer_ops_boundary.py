@@ -80,6 +80,36 @@ def test_c_entry_points_refuse():
     refused(lib.nsa_gated_mlp(C.byref(m), None), UNSUPPORTED, "dtype")
 
 
+def test_c_entry_points_refuse_misaligned_pointers():
+    """Off its elements' alignment no kernel can read a pointer; the host says so before anything is launched."""
+    lib, A = L.load(), 1 << 20
+    norm = dict(x=A, weight=A, y=A, rstd=A, rows=2, hidden=8, x_dtype=0, res_dtype=4, w_dtype=4, y_dtype=0, eps=1e-6, residual=A, h=A)
+    for name, at in (("x", A + 1), ("weight", A + 2), ("y", A + 1), ("h", A + 2), ("residual", A + 2), ("rstd", A + 2)):
+        refused(lib.nsa_rms_norm(C.byref(L.NormArgs(**{**norm, name: at})), None), ARG, "aligned")
+    back = dict(dy=A, h=A, weight=A, rstd=A, dx=A, ws=A, ws_bytes=1 << 20, rows=2, hidden=8, x_dtype=0, res_dtype=0, w_dtype=4)
+    for name, at in (("dy", A + 1), ("h", A + 1), ("dweight", A + 2), ("dx", A + 1), ("ws", A + 16)):
+        refused(lib.nsa_rms_norm_bwd(C.byref(L.NormBwdArgs(**{**back, name: at})), None), ARG, "aligned")
+    refused(lib.nsa_quantize_rows_fp8(A + 1, A, A, 2, 8, 0, 2, None), ARG, "aligned")
+    refused(lib.nsa_quantize_rows_fp8(A, A, A + 2, 2, 8, 0, 2, None), ARG, "aligned")
+    rope = dict(q=A, k=A, v=A, q_out=A, k_out=A, v_out=A, positions=A, inv_freq=A, B=1, T=4, H=2, Hkv=1, D=64, n_axes=1,
+                sections=(C.c_int32 * 8)(32), pos64=1, x_dtype=4, y_dtype=0)
+    for name, at in (("q", A + 2), ("k_out", A + 1), ("positions", A + 4), ("inv_freq", A + 4)):
+        refused(lib.nsa_rope_axes(C.byref(L.RopeAxesArgs(**{**rope, name: at})), None), ARG, "aligned")
+    lin = dict(x=A, w=A, y=A, M=4, N=8, K=8, dtype=0, y_dtype=0, act=0)
+    for name, at in (("x", A + 1), ("w", A + 1), ("bias", A + 1), ("y", A + 1), ("residual", A + 1)):
+        refused(lib.nsa_linear(C.byref(L.LinearArgs(**{**lin, name: at})), None), ARG, "aligned")
+    refused(lib.nsa_linear(C.byref(L.LinearArgs(**{**lin, "dtype": 2, "x_scale": A + 2, "w_scale": A})), None), ARG, "aligned")
+    lb = dict(dy=A, x=A, w=A, dx=A, M=4, N=8, K=8, dtype=0, ws=A, ws_bytes=1 << 30)
+    for name, at in (("dy", A + 1), ("dx", A + 1), ("ws", A + 128)):
+        refused(lib.nsa_linear_bwd(C.byref(L.LinearBwdArgs(**{**lb, name: at})), None), ARG, "aligned")
+    m = dict(x=A, wg=A, wu=A, wd=A, y=A, ws=A, ws_bytes=1 << 30, M=4, N=8, F=16, dtype=0, act=1)
+    for name, at in (("x", A + 1), ("wd", A + 1), ("y", A + 1), ("ws", A + 16)):
+        refused(lib.nsa_gated_mlp(C.byref(L.GatedMlpArgs(**{**m, name: at})), None), ARG, "aligned")
+    mb = dict(dy=A, x=A, wg=A, wu=A, wd=A, p=A, s=A, low=A, h=A, dx=A, ws=A, ws_bytes=1 << 30, M=4, N=8, F=16, dtype=0)
+    for name, at in (("dy", A + 1), ("p", A + 2), ("dx", A + 1), ("ws", A + 16)):
+        refused(lib.nsa_gated_mlp_bwd(C.byref(L.GatedMlpBwdArgs(**{**mb, name: at})), None), ARG, "aligned")
+
+
 def test_no_cpu_path():
     x, w = torch.zeros(4, 8, dtype=torch.bfloat16), torch.zeros(8, 8, dtype=torch.bfloat16)
     for call in (lambda: nsa.rms_norm(x, w[0]), lambda: nsa.rms_norm_fp8(x, w[0]), lambda: nsa.quantize_rows_to_fp8(x), lambda: nsa.linear(x, w),
