@@ -490,6 +490,21 @@ def test_few_tiles(nsa, M, N, K):
     test_linear_backward(nsa, M, N, K, torch.bfloat16, False, None, False)
 
 
+@pytest.mark.parametrize("M,N,K", [(1500, 2051, 200), (512, 2304, 2048), (700, 1530, 1100), (260, 4104, 1024), (2050, 999, 333)])
+def test_more_tiles_than_clusters(nsa, M, N, K):
+    """The same where the tiles no longer fit one round of clusters: whole or joined, off the 16-byte grid too."""
+    test_linear(nsa, M, N, K, torch.float16, True, "gelu_tanh", True)
+    test_linear(nsa, M, N, K, torch.bfloat16, False, None, False)
+    test_linear_fp8(nsa, M, N, K, torch.float8_e4m3fn, torch.float16, True, None, True)
+    test_linear_backward(nsa, M, N, K, torch.bfloat16, True, "silu", True)
+
+
+@pytest.mark.parametrize("M,N,F", [(700, 1000, 1377), (1100, 520, 2200)])
+def test_more_tiles_than_clusters_of_a_gated_block(nsa, M, N, F):
+    test_gated_mlp(nsa, M, N, F, torch.bfloat16, "silu", True)
+    test_gated_mlp_backward(nsa, M, N, F, torch.float16, "silu", False)
+
+
 @pytest.mark.parametrize("M,N,F", [(129, 1024, 264), (200, 256, 700), (300, 2056, 136), (256, 768, 2048), (150, 999, 33)])
 def test_few_tiles_of_a_gated_block(nsa, M, N, F):
     test_gated_mlp(nsa, M, N, F, torch.bfloat16, "silu", True)
