@@ -21,8 +21,9 @@ def rms_norm(x: Tensor, weight: Tensor, *, residual: Optional[Tensor] = None, ep
     """x [..., N] bf16, fp16 or fp32, weight [N] (x's dtype or fp32), residual like x (x's dtype or fp32).
     Returns y in x's dtype; with a residual (y, h), h = x + residual being the new stream in the residual's dtype.
     Differentiable wrt x, residual and weight."""
-    x, weight = ops._dense(x, "x"), ops._dense(weight, "weight")
-    if residual is not None:
+    if not (x.is_contiguous() and weight.is_contiguous()):
+        x, weight = ops._dense(x, "x"), ops._dense(weight, "weight")
+    if residual is not None and not residual.is_contiguous():
         residual = ops._dense(residual, "residual")
     out = L.torch_ops().rms_norm(x, weight, residual, eps)
     return out[0] if residual is None else (out[0], out[1])
@@ -34,8 +35,9 @@ def rms_norm_fp8(x: Tensor, weight: Tensor, *, residual: Optional[Tensor] = None
     per row: y ~= q * scale, scale = max(max|y|, 1e-12) / fmt_max.  Inference only."""
     if fmt not in ops._8:
         raise ValueError(f"unsupported fp8 format: {fmt}")
-    x, weight = ops._dense(x, "x"), ops._dense(weight, "weight")
-    if residual is not None:
+    if not (x.is_contiguous() and weight.is_contiguous()):
+        x, weight = ops._dense(x, "x"), ops._dense(weight, "weight")
+    if residual is not None and not residual.is_contiguous():
         residual = ops._dense(residual, "residual")
     return tuple(L.torch_ops().rms_norm_fp8(x, weight, residual, eps, L.dtype_code(fmt)))
 

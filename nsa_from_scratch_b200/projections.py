@@ -22,10 +22,11 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, *, activati
     """act(x weight^T + bias) + residual.  x [..., K], weight [N, K], bias [N], residual [..., N], all bf16 or all fp16;
     activation None, "silu", "gelu_tanh" or "relu".  Returns [..., N] in x's dtype: fp32 sums and epilogue, one rounding.
     Differentiable wrt x, weight, bias and residual (act' is kept in 16 bits of its own for the backward)."""
-    x, weight = ops._dense(x, "x"), ops._dense(weight, "weight")
-    if bias is not None:
+    if not (x.is_contiguous() and weight.is_contiguous()):
+        x, weight = ops._dense(x, "x"), ops._dense(weight, "weight")
+    if bias is not None and not bias.is_contiguous():
         bias = ops._dense(bias, "bias")
-    if residual is not None:
+    if residual is not None and not residual.is_contiguous():
         residual = ops._dense(residual, "residual")
     return L.torch_ops().linear(x, weight, bias, residual, ops.activation_code(activation))
 
@@ -38,9 +39,9 @@ def linear_fp8(x: Tensor, weight: Tensor, x_scale: Tensor, w_scale: Tensor, bias
     if dtype not in ops._16:
         raise TypeError(f"linear_fp8: the result is bf16 or fp16, not {dtype}")
     x, weight, x_scale, w_scale = ops._dense(x, "x"), ops._dense(weight, "weight"), ops._dense(x_scale, "x_scale"), ops._dense(w_scale, "w_scale")
-    if bias is not None:
+    if bias is not None and not bias.is_contiguous():
         bias = ops._dense(bias, "bias")
-    if residual is not None:
+    if residual is not None and not residual.is_contiguous():
         residual = ops._dense(residual, "residual")
     return L.torch_ops().linear_fp8(x, weight, x_scale, w_scale, bias, residual, ops.activation_code(activation), L.dtype_code(dtype))
 
@@ -50,8 +51,9 @@ def gated_mlp(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, *, activa
     """(act(x w_gate^T) * (x w_up^T)) w_down^T + residual.  x and residual [..., N], w_gate and w_up [F, N], w_down [N, F], all bf16 or all
     fp16; activation as for `linear` (None: the plain product of the two).  fp32 sums; the gated product is rounded to x's
     dtype between the two matrix products, the result once.  Differentiable wrt every tensor."""
-    x, w_gate, w_up, w_down = ops._dense(x, "x"), ops._dense(w_gate, "w_gate"), ops._dense(w_up, "w_up"), ops._dense(w_down, "w_down")
-    if residual is not None:
+    if not (x.is_contiguous() and w_gate.is_contiguous() and w_up.is_contiguous() and w_down.is_contiguous()):
+        x, w_gate, w_up, w_down = ops._dense(x, "x"), ops._dense(w_gate, "w_gate"), ops._dense(w_up, "w_up"), ops._dense(w_down, "w_down")
+    if residual is not None and not residual.is_contiguous():
         residual = ops._dense(residual, "residual")
     return L.torch_ops().gated_mlp(x, w_gate, w_up, w_down, residual, ops.activation_code(activation))
 

@@ -41,8 +41,10 @@ def rope_axes_to_heads(q: Tensor, k: Tensor, v: Tensor, positions: Tensor, inv_f
         raise TypeError(f"rope_axes_to_heads: the result is bf16 or fp16, not {dtype}")
     if inv_freq.dtype == torch.float32:
         inv_freq = inv_freq.to(torch.float64)
-    return tuple(L.torch_ops().rope_axes(_heads(q, "q"), _heads(k, "k"), _heads(v, "v"), ops._dense(positions, "positions"),
-                                         ops._dense(inv_freq, "inv_freq"), sections, L.dtype_code(dtype)))
+    if not (q.is_contiguous() and k.is_contiguous() and v.is_contiguous() and positions.is_contiguous() and inv_freq.is_contiguous()):
+        q, k, v = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
+        positions, inv_freq = ops._dense(positions, "positions"), ops._dense(inv_freq, "inv_freq")
+    return tuple(L.torch_ops().rope_axes(q, k, v, positions, inv_freq, sections, L.dtype_code(dtype)))
 
 
 __all__ = ["rope_axes_to_heads", "rope_frequencies"]
