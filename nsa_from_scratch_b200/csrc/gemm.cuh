@@ -66,7 +66,9 @@ __device__ __forceinline__ float slope_value(uint32_t code) {
 // What a gated pair leaves for the backward, p = act(g) and s = act'(g) u: fp32 rounded to its upper 24 bits (2^-16), the upper
 // 16 in an array each, the next 8 of both in a third (p's in the lower byte).  Rounded to 16 bits they would add as much
 // error to the gradients as the roundings that cannot be had without; in fp32 they would take 8 bytes instead of 6.
-__device__ __forceinline__ uint32_t cut24(float v) { return __float_as_uint(v) + 0x80u; }      // infinities and NaN stay what they are
+// Infinities stay what they are; NaN is set apart, because half a step on top of the NaN that the arithmetic yields, 0x7fffffff,
+// would make it -0.
+__device__ __forceinline__ uint32_t cut24(float v) { return v != v ? 0x7fc00000u : __float_as_uint(v) + 0x80u; }
 __device__ __forceinline__ uint32_t low_bytes(uint32_t p, uint32_t s) { return ((p >> 8) & 0xffu) | (s & 0xff00u); }
 __device__ __forceinline__ float join24_p(uint32_t hi, uint32_t low) { return __uint_as_float((hi << 16) | ((low & 0xffu) << 8)); }
 __device__ __forceinline__ float join24_s(uint32_t hi, uint32_t low) { return __uint_as_float((hi << 16) | (low & 0xff00u)); }
