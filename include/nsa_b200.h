@@ -506,7 +506,7 @@ int nsa_rope_axes(const nsa_rope_axes_args* args, nsa_stream_t stream);
 /* y = act(x w^T + bias) + residual:  x [M,K], w [N,K], bias [N], residual and y [M,N].
  * x and w: both bf16 or both fp16 (bias, residual and y share the type); or both e4m3 or both e5m2 with x_scale [M] and w_scale
  * [N] (y, bias and residual in y_dtype).  bias, residual NULL: none.  slope [M,N] (NULL: not wanted; 16-bit operands with an
- * activation): act' at act's argument for the backward, 16 bits each: q with act' = q |q| 2^-28.  Sums, bias, activation
+ * activation): act' at act's argument for the backward, 16 bits each: q with act' = q |q| 2^-28, -32768 for NaN.  Sums, bias, activation
  * and residual in fp32, one rounding.
  * ws: nsa_linear_ws_bytes(&args) bytes, asked with the pointers set (operands that are not 16-byte aligned are copied
  * there); negative: bad arguments. */

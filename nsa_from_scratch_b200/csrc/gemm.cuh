@@ -51,16 +51,18 @@ template <int ACT> __device__ __forceinline__ void act_one_both(float z, float& 
   }
 }
 // act' as the backward gets it: a signed 16-bit q with act' = q |q| 2^-28 (it lies in [-0.13, 1.13]).  Half a step of q is 2^-15,
-// so act' is off by 2^-14 sqrt(|act'|): a quarter of an fp16 rounding where it is large, and still 1 % at 10^-5.  Rounded to
-// x's own type it would add as much error to the gradients as the roundings that cannot be had without.
+// so act' is off by 2^-14 sqrt(|act'|): a quarter of an fp16 rounding where it is large, and still 2 % at 10^-5.  Rounded to
+// x's own type it would add as much error to the gradients as the roundings that cannot be had without.  -32768, which no
+// act' of a number needs, is NaN (a NaN argument; silu and gelu at infinite ones).
 __device__ __forceinline__ uint32_t slope_code(float d) {
   float r;
   asm("sqrt.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(fabsf(d) * 268435456.f));
-  return (uint32_t)(uint16_t)(int16_t)__float2int_rn(copysignf(r, d));
+  return d != d ? 0x8000u : (uint32_t)(uint16_t)(int16_t)__float2int_rn(copysignf(r, d));
 }
 __device__ __forceinline__ float slope_value(uint32_t code) {
-  const float q = (float)(int16_t)(uint16_t)code;
-  return q * fabsf(q) * 3.7252902984619140625e-9f;             // 2^-28
+  const uint32_t c = code & 0xffffu;
+  const float q = (float)(int16_t)(uint16_t)c;
+  return c == 0x8000u ? __uint_as_float(0x7fc00000u) : q * fabsf(q) * 3.7252902984619140625e-9f;             // 2^-28
 }
 
 // What a gated pair leaves for the backward, p = act(g) and s = act'(g) u: fp32 rounded to its upper 24 bits (2^-16), the upper

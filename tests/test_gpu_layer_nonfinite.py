@@ -66,3 +66,31 @@ def test_gated_mlp(nsa, M, N, F, dtype, act, where, value):
     assert any(torch.isnan(t).any() for t in ref[1:])
     for a, b, r, name in zip(step(), clean, ref, ("y", "dx", "dwg", "dwu", "dwd")):
         same_elsewhere(a, b, r, name)
+
+
+LINEAR = [(5, 64, 136), (24, 264, 72), (100, 136, 520), (90, 33, 67), (256, 512, 768), (300, 1001, 100), (4000, 1000, 72)]
+
+
+@pytest.mark.parametrize("M,N,K", LINEAR)
+@pytest.mark.parametrize("dtype,act", [(torch.bfloat16, "silu"), (torch.float16, "gelu_tanh"), (torch.float16, None)])
+@pytest.mark.parametrize("where,value", [("x", NAN), ("x", INF), ("w", NAN), ("bias", NAN), ("bias", INF)])
+def test_linear(nsa, M, N, K, dtype, act, where, value):
+    ts = {"x": randn(M, K, seed=1, dtype=dtype), "w": randn(N, K, seed=2, std=K ** -0.5, dtype=dtype), "bias": randn(N, seed=3, dtype=dtype)}
+    dy = randn(M, N, seed=5, dtype=dtype)
+
+    def step():
+        leaves = [t.detach().clone().requires_grad_(True) for t in ts.values()]
+        y = nsa.linear(*leaves, activation=act)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+
+    clean = step()
+    if where == "bias":
+        ts["bias"][min(7, N - 1)] = value
+    else:
+        ts[where][min(3, ts[where].shape[0] - 1), min(7, K - 1)] = value
+    x, w, b = (t.double() for t in ts.values())
+    z = x @ w.T + b
+    dz = dy.double() * slope(z, act)
+    ref = (act64(z, act), dz @ w, dz.T @ x, dz.sum(0))
+    for a, c, r, name in zip(step(), clean, ref, ("y", "dx", "dw", "db")):
+        same_elsewhere(a, c, r, name)
