@@ -443,7 +443,9 @@ int nsa_select_blocks_cached(const void* Qb, const void* Kb, int32_t* idx, int B
  * torch modules, nsa/model/llama_dense.py:19-134): norm, rotary embedding, projections, gated feed-forward block.
  * Rows are dense; pointers need no more than their elements' alignment (16-byte aligned rows take the fast kernels).
  * Workspaces are device memory, 256-byte aligned, contents free before and after.  Pointers and workspaces off
- * these alignments are refused. */
+ * these alignments are refused, and so are sizes M, N, K, F, T and hidden beyond NSA_MAX_SIZE (the kernels count in 32
+ * bits, and step past an end by less than the rest). */
+#define NSA_MAX_SIZE 2147418112 /* 2^31 - 2^16 */
 #define NSA_ACT_NONE 0
 #define NSA_ACT_SILU 1
 #define NSA_ACT_GELU_TANH 2 /* 0.5 z (1 + tanh(sqrt(2/pi) (z + 0.044715 z^3))) */

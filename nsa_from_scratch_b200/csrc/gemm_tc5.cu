@@ -771,6 +771,10 @@ static int esize(int dtype) { return dtype == NSA_BF16 || dtype == NSA_FP16 ? 2 
 // the results' rows do not start on 16-byte boundaries (TMA writes them).
 struct TcPlan { int cg, bn, tiles_m, tiles_n, ksteps, splits, per_split; bool raw, cluster; };
 
+// Most steps of a contraction that one tile takes (16.8 M of 16 bits: 70 ms).  The waits for a finished tile are bounded to about a
+// second, and an fp32 sum of more terms would stop growing; longer contractions (a weight's gradient over that many tokens) are split.
+constexpr int MOST_STEPS = 1 << 18;
+
 // How many clusters of `size` CTAs the device holds at a time, a CTA to an SM
 static int cluster_room(int size) {
   static int known[64][2];                      // clusters of 4 and of 8; 0: not asked yet
@@ -801,10 +805,12 @@ static TcPlan tc_plan(const GemmProblem& p, bool whole = false) {     // whole: 
   TcPlan t;
   const int pair = p.e.mode == EPI_GLU ? 2 : 1;
   const bool raw = !p.e.vec || !p.e.vecy;
-  const int ksteps = (p.K * esize(p.dtype) + 127) / 128, steps = ksteps * p.segments;
+  const int ksteps = (int)(((long long)p.K * esize(p.dtype) + 127) / 128), steps = ksteps * p.segments;     // at most 2^26
+  const int least = (steps + MOST_STEPS - 1) / MOST_STEPS;
   // In clk: rounds of tiles at what a step brings through L2 and shared memory (512 for 256 columns on pairs and for 128 on
   // one CTA, 384 for 128 on pairs), and the epilogue that no other tile hides; splitting adds the sums' way out and back
-  // (64 bytes a clk and SM) and the joining kernel.  The cheapest of both widths and up to 16 ways.
+  // (64 bytes a clk and SM) and the joining kernel.  The cheapest of both widths and up to 16 ways
+  // (the fewest possible where those are more).
   double best = -1;
   for (int bn = 256; bn >= 128; bn -= 128) {
     const int cg = !whole && p.M <= 128 ? 1 : 2;
@@ -812,7 +818,7 @@ static TcPlan tc_plan(const GemmProblem& p, bool whole = false) {     // whole: 
     const int tm = (p.M + 128 * cg - 1) / (128 * cg), tn = (p.N + bn / pair - 1) / (bn / pair);
     const long long n = (long long)tm * tn, units = sm_count() / cg;
     const int step = cg == 2 && bn == 128 ? 384 : 512;
-    for (int s = 1; s <= 16 && s * 4 <= (steps > 4 ? steps : 4); ++s) {
+    for (int s = whole ? 1 : least; s <= (least > 16 ? least : 16) && s * 4 <= (steps > 4 ? steps : 4); ++s) {
       if (whole && s > 1) break;
       const int per = (steps + s - 1) / s, ways = (steps + per - 1) / per;
       double cost = (double)((n * ways + units - 1) / units) * per * step + 16 * bn;
@@ -832,7 +838,7 @@ static TcPlan tc_plan(const GemmProblem& p, bool whole = false) {     // whole: 
     const int tm = (p.M + 255) / 256, tn = (p.N + CLUSTER_BN / pair - 1) / (CLUSTER_BN / pair);
     for (int s = 2; s <= 4; s *= 2) {
       const int per = (steps + s - 1) / s;
-      if ((s - 1) * per >= steps || (long long)tm * tn > cluster_room(2 * s)) continue;
+      if (per > MOST_STEPS || (s - 1) * per >= steps || (long long)tm * tn > cluster_room(2 * s)) continue;
       const double cost = (double)per * 384 + 5000;
       if (cost < best) {
         best = cost;
@@ -1024,6 +1030,7 @@ static bool groups(const GemmProblem* p, int count) {
   for (int i = 0; i < count; ++i) {
     if (p[i].M <= 128 || !p[i].e.vec || !p[i].e.vecy) return false;
     const TcPlan t = tc_plan(p[i], true);
+    if (t.ksteps * p[i].segments > MOST_STEPS) return false;
     tiles += (long long)t.tiles_m * t.tiles_n;
   }
   return tiles < 2147483647LL - 65536 && tiles * 4 >= sm_count();

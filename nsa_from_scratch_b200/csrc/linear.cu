@@ -23,7 +23,7 @@ __global__ void __launch_bounds__(128) act_bwd_kernel(const void* __restrict__ d
                                                       float* __restrict__ part, int M, int N, long long lddz, int rows, int vec, int vecz) {
   const int c = (blockIdx.x * 128 + threadIdx.x) * 8, n = N - c;
   if (n <= 0) return;
-  const int r0 = blockIdx.y * rows, r1 = min(M, r0 + rows);
+  const int r0 = blockIdx.y * rows, r1 = r0 + min(rows, M - r0);
   float sum[8] = {};
   constexpr int U = 4;
   for (int r = r0; r < r1; r += U) {
@@ -69,9 +69,8 @@ static ActBwdPlan act_bwd_plan(int M, int N) {
   ActBwdPlan p;
   p.strips = (N + 1023) / 1024;
   const int want = (8 * sm_count() + p.strips - 1) / p.strips;                  // eight blocks an SM
-  p.rows = (M + want - 1) / want;
-  if (p.rows < 1) p.rows = 1;
-  p.groups = (M + p.rows - 1) / p.rows;
+  p.rows = (M - 1) / want + 1;                                                  // M > 0; M + rows may pass 32 bits
+  p.groups = (M - 1) / p.rows + 1;
   return p;
 }
 
@@ -143,6 +142,9 @@ __global__ void __launch_bounds__(256) pad_rows_kernel(const E* __restrict__ src
   }
 }
 
+// A size that the kernels' 32-bit counts hold with room to step past its end
+static bool sized(int n) { return n > 0 && n <= NSA_MAX_SIZE; }
+
 // An operand whose rows start on 16-byte boundaries: the caller's own, or a padded copy.
 struct Mat { const void* p; long long ld; };
 static int operand(Arena& w, const void* p, long long rows, int cols, int dtype, Mat* m) {
@@ -204,7 +206,7 @@ static int zero(void* p, long long bytes, cudaStream_t st) {
 
 // ---------------------------------------------------------------- linear
 static int check_linear(const nsa_linear_args& a) {
-  NSA_REQUIRE(a.M >= 0 && a.N > 0 && a.K > 0, NSA_ERR_ARG, "linear: bad sizes M=%d N=%d K=%d", a.M, a.N, a.K);
+  NSA_REQUIRE((a.M == 0 || sized(a.M)) && sized(a.N) && sized(a.K), NSA_ERR_ARG, "linear: bad sizes M=%d N=%d K=%d", a.M, a.N, a.K);
   NSA_REQUIRE(is16(a.dtype) || is8(a.dtype), NSA_ERR_UNSUPPORTED, "linear: operand dtype %d", a.dtype);
   NSA_REQUIRE(is16(a.y_dtype) && (is8(a.dtype) || a.y_dtype == a.dtype), NSA_ERR_UNSUPPORTED, "linear: result dtype %d of operands %d", a.y_dtype, a.dtype);
   NSA_REQUIRE(a.act >= NSA_ACT_NONE && a.act <= NSA_ACT_RELU, NSA_ERR_ARG, "linear: activation %d", a.act);
@@ -241,7 +243,7 @@ int linear(const nsa_linear_args& a, cudaStream_t st) {
 }
 
 static int check_linear_bwd(const nsa_linear_bwd_args& a) {
-  NSA_REQUIRE(a.M >= 0 && a.N > 0 && a.K > 0, NSA_ERR_ARG, "linear backward: bad sizes M=%d N=%d K=%d", a.M, a.N, a.K);
+  NSA_REQUIRE((a.M == 0 || sized(a.M)) && sized(a.N) && sized(a.K), NSA_ERR_ARG, "linear backward: bad sizes M=%d N=%d K=%d", a.M, a.N, a.K);
   NSA_REQUIRE(is16(a.dtype), NSA_ERR_UNSUPPORTED, "linear backward: dtype %d", a.dtype);
   return NSA_OK;
 }
@@ -285,7 +287,7 @@ int linear_bwd(const nsa_linear_bwd_args& a, cudaStream_t st) {
 
 // ---------------------------------------------------------------- gated feed-forward block
 static int check_mlp(int M, int N, int F, int dtype, int act) {
-  NSA_REQUIRE(M >= 0 && N > 0 && F > 0, NSA_ERR_ARG, "gated_mlp: bad sizes M=%d N=%d F=%d", M, N, F);
+  NSA_REQUIRE((M == 0 || sized(M)) && sized(N) && sized(F), NSA_ERR_ARG, "gated_mlp: bad sizes M=%d N=%d F=%d", M, N, F);
   NSA_REQUIRE(is16(dtype), NSA_ERR_UNSUPPORTED, "gated_mlp: dtype %d", dtype);
   NSA_REQUIRE(act >= NSA_ACT_NONE && act <= NSA_ACT_RELU, NSA_ERR_ARG, "gated_mlp: activation %d", act);
   return NSA_OK;
@@ -393,7 +395,7 @@ extern "C" {
 
 int nsa_rms_norm(const nsa_norm_args* a, nsa_stream_t stream) {
   NSA_REQUIRE(a, NSA_ERR_ARG, "rms_norm: NULL argument block");
-  NSA_REQUIRE(a->rows >= 0 && a->rows < 2147483648LL && a->hidden > 0, NSA_ERR_ARG, "rms_norm: bad sizes rows=%lld hidden=%d", (long long)a->rows, a->hidden);
+  NSA_REQUIRE(a->rows >= 0 && a->rows < 2147483648LL && sized(a->hidden), NSA_ERR_ARG, "rms_norm: bad sizes rows=%lld hidden=%d", (long long)a->rows, a->hidden);
   NSA_REQUIRE(is_real(a->x_dtype), NSA_ERR_UNSUPPORTED, "rms_norm: x dtype %d", a->x_dtype);
   NSA_REQUIRE(a->w_dtype == a->x_dtype || a->w_dtype == NSA_FP32, NSA_ERR_UNSUPPORTED, "rms_norm: weight dtype %d beside x %d", a->w_dtype, a->x_dtype);
   NSA_REQUIRE(a->y_dtype == a->x_dtype || is8(a->y_dtype), NSA_ERR_UNSUPPORTED, "rms_norm: result dtype %d of x %d", a->y_dtype, a->x_dtype);
@@ -410,13 +412,13 @@ int nsa_rms_norm(const nsa_norm_args* a, nsa_stream_t stream) {
 }
 
 int64_t nsa_rms_norm_bwd_ws_bytes(int64_t rows, int hidden) {
-  NSA_REQUIRE(rows >= 0 && hidden > 0, NSA_ERR_ARG, "rms_norm backward: bad sizes rows=%lld hidden=%d", (long long)rows, hidden);
+  NSA_REQUIRE(rows >= 0 && sized(hidden), NSA_ERR_ARG, "rms_norm backward: bad sizes rows=%lld hidden=%d", (long long)rows, hidden);
   return rms_norm_bwd_ws_bytes(rows, hidden);
 }
 
 int nsa_rms_norm_bwd(const nsa_norm_bwd_args* a, nsa_stream_t stream) {
   NSA_REQUIRE(a, NSA_ERR_ARG, "rms_norm backward: NULL argument block");
-  NSA_REQUIRE(a->rows >= 0 && a->hidden > 0, NSA_ERR_ARG, "rms_norm backward: bad sizes rows=%lld hidden=%d", (long long)a->rows, a->hidden);
+  NSA_REQUIRE(a->rows >= 0 && sized(a->hidden), NSA_ERR_ARG, "rms_norm backward: bad sizes rows=%lld hidden=%d", (long long)a->rows, a->hidden);
   NSA_REQUIRE(is_real(a->x_dtype) && (a->w_dtype == a->x_dtype || a->w_dtype == NSA_FP32) && (a->res_dtype == a->x_dtype || a->res_dtype == NSA_FP32),
               NSA_ERR_UNSUPPORTED, "rms_norm backward: dtypes %d/%d/%d", a->x_dtype, a->res_dtype, a->w_dtype);
   if (a->rows == 0) return zero(a->dweight, (long long)a->hidden * (a->w_dtype == NSA_FP32 ? 4 : 2), (cudaStream_t)stream);
@@ -430,7 +432,7 @@ int nsa_rms_norm_bwd(const nsa_norm_bwd_args* a, nsa_stream_t stream) {
 }
 
 int nsa_quantize_rows_fp8(const void* x, void* q, float* scale, int64_t rows, int n, int x_dtype, int fmt, nsa_stream_t stream) {
-  NSA_REQUIRE(rows >= 0 && rows < 2147483648LL && n > 0, NSA_ERR_ARG, "quantize_rows: bad sizes rows=%lld n=%d", (long long)rows, n);
+  NSA_REQUIRE(rows >= 0 && rows < 2147483648LL && sized(n), NSA_ERR_ARG, "quantize_rows: bad sizes rows=%lld n=%d", (long long)rows, n);
   NSA_REQUIRE(is_real(x_dtype), NSA_ERR_UNSUPPORTED, "quantize_rows: dtype %d", x_dtype);
   NSA_REQUIRE(is8(fmt), NSA_ERR_ARG, "quantize_rows: format %d", fmt);
   if (rows == 0) return NSA_OK;
@@ -441,7 +443,7 @@ int nsa_quantize_rows_fp8(const void* x, void* q, float* scale, int64_t rows, in
 
 int nsa_rope_axes(const nsa_rope_axes_args* a, nsa_stream_t stream) {
   NSA_REQUIRE(a, NSA_ERR_ARG, "rope_axes: NULL argument block");
-  NSA_REQUIRE(a->B >= 0 && a->T >= 0 && a->H > 0 && a->Hkv > 0 && a->H + 2LL * a->Hkv < 65536, NSA_ERR_ARG, "rope_axes: bad sizes B=%d T=%d H=%d Hkv=%d", a->B, a->T,
+  NSA_REQUIRE(a->B >= 0 && (a->T == 0 || sized(a->T)) && a->H > 0 && a->Hkv > 0 && a->H + 2LL * a->Hkv < 65536, NSA_ERR_ARG, "rope_axes: bad sizes B=%d T=%d H=%d Hkv=%d", a->B, a->T,
               a->H, a->Hkv);
   NSA_REQUIRE(a->D > 0 && a->D % 2 == 0 && a->D <= 1024, NSA_ERR_UNSUPPORTED, "rope_axes: D=%d must be even and at most 1024", a->D);
   NSA_REQUIRE(a->n_axes >= 1 && a->n_axes <= 8, NSA_ERR_ARG, "rope_axes: %d axes (1 to 8 are taken)", a->n_axes);

@@ -53,9 +53,9 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* ptr(const optional<Tensor>& t) { return t.has_value() && t->defined() ? t->data_ptr() : nullptr; }
 bool given(const optional<Tensor>& t) { return t.has_value() && t->defined(); }
 bool wants(const optional<Tensor>& t) { return given(t) && t->requires_grad(); }
-// a size that the C ABI holds in 32 bits
+// a size that the kernels take
 int32_t size32(int64_t n, const char* what) {
-  TORCH_CHECK_VALUE(n <= 2147483647, what, ": ", n, " is more than the kernels' 32-bit sizes hold");
+  TORCH_CHECK_VALUE(n <= NSA_MAX_SIZE, what, ": ", n, " is more than the kernels' 32-bit sizes hold");
   return (int32_t)n;
 }
 void ok(int rc, const char* what) { TORCH_CHECK(rc == NSA_OK, what, " failed (status ", rc, "): ", nsa_last_error()); }
