@@ -18,7 +18,7 @@ addition, gated feed-forward block with the residual in its epilogue.
 """
 from __future__ import annotations
 
-from typing import Optional, Sequence
+from typing import Dict, Optional, Sequence, Tuple
 
 import torch
 import torch.nn as nn
@@ -149,15 +149,23 @@ class NSABlock(nn.Module):
         self.eps, self.activation = eps, activation
         self.rope_sections = tuple(rope_sections) if rope_sections is not None else (head_dim // 2,)
         self.rope_base = rope_base
-        self._inv_freq: Optional[Tensor] = None              # fp64, and stays that when the module is cast
+        # fp64, and stays that when the module is cast; by device and base, and kept while the module lives, since a captured
+        # step or another stream's may still read an earlier one
+        self._inv_freq: Dict[Tuple, Tensor] = {}
 
     def _frequencies(self, device: torch.device) -> Tensor:
-        if self._inv_freq is not None and self._inv_freq.device == device:
-            return self._inv_freq
+        key = (device, float(self.rope_base), self.attn.head_dim)
+        f = self._inv_freq.get(key)
+        if f is not None:
+            return f
         with torch.inference_mode(False):                    # a later training step saves it for its backward
             f = rope_frequencies(self.attn.head_dim, self.rope_base, device)
-        if not torch.cuda.is_current_stream_capturing():     # in a capture it holds nothing until the replay
-            self._inv_freq = f
+        if device.type == "cuda":
+            with torch.cuda.device(device):
+                if torch.cuda.is_current_stream_capturing():
+                    return f                                 # holds nothing until the replay
+                torch.cuda.current_stream().synchronize()    # whichever stream the next call is on finds it filled
+            self._inv_freq[key] = f
         return f
 
     def new_cache(self, batch: int, max_len: int) -> KVCache:
