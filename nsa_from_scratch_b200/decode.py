@@ -32,6 +32,8 @@ class KVCache:
     def __init__(self, B: int, Hkv: int, D: int, max_len: int, cfg, dtype: torch.dtype = torch.bfloat16, device="cuda"):
         if not cfg.causal:
             raise ValueError("KVCache: decoding needs causal=True")
+        if getattr(cfg, "pool", "mean") == "learned":
+            raise NotImplementedError("KVCache: the cache keeps window means; pool='learned' has no decoding")
         self.cfg = cfg
         self.bc = int(cfg.block_size_c)
         self.stride = self.bc if getattr(cfg, "stride_c", None) is None else int(cfg.stride_c)

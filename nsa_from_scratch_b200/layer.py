@@ -109,10 +109,13 @@ class NSAAttention(nn.Module):
         """The module in bf16 or fp16 on the layer's own operators: x [B,T,hidden] -> [B,T,hidden] (+ residual, in the output
         projection's epilogue).  positions [axes,B,T], inv_freq and sections as for `rope_axes_to_heads`.  With `cache`
         (decoding, no gradients) the T positions are appended to it and attend everything it holds; else they attend each
-        other.  Differentiable without a cache; pool="learned" takes the inference routes only."""
+        other.  Differentiable without a cache; pool="learned" takes the inference route without a cache only (a KVCache keeps
+        window means)."""
         B, T, _ = x.shape
         H, Hkv, D = self.n_heads, self.n_kv_heads, self.head_dim
         cfg = self.nsa_cfg
+        if cache is not None and getattr(cfg, "pool", "mean") == "learned":
+            raise NotImplementedError("NSAAttention.attend: the cache keeps window means; pool='learned' has no decoding")
         q = linear(x, self.q_proj.weight).view(B, T, H, D)
         k = linear(x, self.k_proj.weight).view(B, T, Hkv, D)
         v = linear(x, self.v_proj.weight).view(B, T, Hkv, D)
