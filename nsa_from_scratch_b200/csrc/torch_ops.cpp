@@ -53,6 +53,13 @@ void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
 void* ptr(const optional<Tensor>& t) { return t.has_value() && t->defined() ? t->data_ptr() : nullptr; }
 bool given(const optional<Tensor>& t) { return t.has_value() && t->defined(); }
 bool wants(const optional<Tensor>& t) { return given(t) && t->requires_grad(); }
+// Forward-mode differentiation has no rules here: a tangent is refused, not dropped
+bool tangent(const Tensor& t) { return t.defined() && t._fw_grad(/*level=*/0).defined(); }
+bool tangent(const optional<Tensor>& t) { return t.has_value() && tangent(*t); }
+template <typename... T> void no_tangents(const char* what, const T&... t) {
+  if (C10_UNLIKELY((tangent(t) || ...)) && c10::AutogradState::get_tls_state().get_fw_grad_mode())
+    TORCH_CHECK(false, what, ": forward-mode differentiation is not provided; gradients are those of backward()");
+}
 // a size that the kernels take
 int32_t size32(int64_t n, const char* what) {
   TORCH_CHECK_VALUE(n <= NSA_MAX_SIZE, what, ": ", n, " is more than the kernels' 32-bit sizes hold");
@@ -170,6 +177,7 @@ struct RmsNorm : Function<RmsNorm> {
 };
 
 variable_list rms_norm(const Tensor& x, const Tensor& w, const optional<Tensor>& res, double eps) {
+  no_tangents("rms_norm", x, w, res);
   if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || wants(res))) return RmsNorm::apply(x, w, res, eps);
   const nsa_norm_args a = check_norm(x, w, res, eps, "rms_norm");
   const Tensor y = fresh(x);
@@ -178,6 +186,7 @@ variable_list rms_norm(const Tensor& x, const Tensor& w, const optional<Tensor>&
 }
 
 variable_list rms_norm_fp8(const Tensor& x, const Tensor& w, const optional<Tensor>& res, double eps, int64_t fmt) {
+  no_tangents("rms_norm_fp8", x, w, res);
   at::NoGradGuard off;
   nsa_norm_args a = check_norm(x, w, res, eps, "rms_norm_fp8");
   a.y_dtype = (int32_t)fmt;
@@ -188,6 +197,7 @@ variable_list rms_norm_fp8(const Tensor& x, const Tensor& w, const optional<Tens
 }
 
 variable_list quantize_rows(const Tensor& x, int64_t fmt) {
+  no_tangents("quantize_rows_to_fp8", x);
   at::NoGradGuard off;
   first(x, "x");
   TORCH_CHECK_TYPE(is_real(x) && x.dim() >= 1, "quantize_rows_to_fp8: x must be a bf16, fp16 or fp32 tensor of rows, got ", x.scalar_type());
@@ -284,6 +294,7 @@ struct RopeAxes : Function<RopeAxes> {
 };
 
 variable_list rope_axes(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& pos, const Tensor& inv, const std::vector<int64_t>& sections, int64_t dtype) {
+  no_tangents("rope_axes_to_heads", q, k, v, inv);
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) return RopeAxes::apply(q, k, v, pos, inv, at::IntArrayRef(sections), dtype);
   return launch_rope(check_rope(q, k, v, pos, inv, sections, dtype), q, type_of(dtype));
 }
@@ -376,11 +387,13 @@ struct Linear : Function<Linear> {
 };
 
 Tensor linear(const Tensor& x, const Tensor& w, const optional<Tensor>& bias, const optional<Tensor>& res, int64_t act) {
+  no_tangents("linear", x, w, bias, res);
   if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || wants(bias) || wants(res))) return Linear::apply(x, w, bias, res, act);
   need_cuda(x);
   return launch_linear(check_linear(x, w, bias, res, {}, {}, act, is16(x) ? code(x.scalar_type()) : NSA_BF16, "linear"), x, nullptr);
 }
 Tensor linear_fp8(const Tensor& x, const Tensor& w, const Tensor& xs, const Tensor& ws, const optional<Tensor>& bias, const optional<Tensor>& res, int64_t act, int64_t dtype) {
+  no_tangents("linear_fp8", xs, ws, bias, res);
   at::NoGradGuard off;
   return launch_linear(check_linear(x, w, bias, res, xs, ws, act, dtype, "linear_fp8"), x, nullptr);
 }
@@ -451,6 +464,7 @@ struct GatedMlp : Function<GatedMlp> {
 };
 
 Tensor gated_mlp(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, const optional<Tensor>& res, int64_t act) {
+  no_tangents("gated_mlp", x, wg, wu, wd, res);
   if (at::GradMode::is_enabled() && (x.requires_grad() || wg.requires_grad() || wu.requires_grad() || wd.requires_grad() || wants(res)))
     return GatedMlp::apply(x, wg, wu, wd, res, act);
   return launch_mlp(check_mlp(x, wg, wu, wd, res, act), x, nullptr);
