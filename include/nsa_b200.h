@@ -54,6 +54,8 @@ typedef void* nsa_stream_t; /* a cudaStream_t; NULL is the default stream */
 #define NSA_ENGINE_TCGEN05 2
 
 const char* nsa_last_error(void);
+/* Raised when a struct or a prototype of this file changes; nsa_abi_version() is the library's. */
+#define NSA_ABI_VERSION 7
 int nsa_abi_version(void);
 
 /* Mean over windows of `block` rows every `stride` rows:  x [B,H,T,D] -> out [B,H,n_out,D].

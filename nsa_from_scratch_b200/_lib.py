@@ -258,14 +258,19 @@ def torch_ops():
         load()                       # checks the ABI version of the library that the module links to
         try:
             path = _build.build_torch()
-        except RuntimeError:
+        except _build.NoCompiler:    # a source that does not compile is an error, whatever was built before it
             path = _build.TORCH_LIB
             if not os.path.exists(path):
-                raise                # with a module present (no compiler on this machine) its import decides
+                raise                # with a module present the checks below decide
         import importlib.util
         spec = importlib.util.spec_from_file_location("_nsa_torch", path)
-        _torch_ops = importlib.util.module_from_spec(spec)
-        spec.loader.exec_module(_torch_ops)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        built = getattr(module, "abi_version", None)
+        if built != ABI_VERSION:
+            raise RuntimeError(f"{path} was built for ABI version {built}, this package expects {ABI_VERSION}: "
+                               "rebuild with `python -m nsa_from_scratch_b200.build --force`")
+        _torch_ops = module
     return _torch_ops
 
 

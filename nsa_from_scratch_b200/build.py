@@ -30,11 +30,15 @@ NVCC_FLAGS = [
 ]
 
 
+class NoCompiler(RuntimeError):
+    """This machine has no nvcc: what was built elsewhere may be used as it is."""
+
+
 def _nvcc() -> str:
     for cand in (os.environ.get("NVCC"), shutil.which("nvcc"), "/usr/local/cuda/bin/nvcc"):
         if cand and os.path.exists(cand):
             return cand
-    raise RuntimeError("nvcc not found; set NVCC")
+    raise NoCompiler("nvcc not found; set NVCC")
 
 
 def _sources():

@@ -474,6 +474,7 @@ Tensor gated_mlp(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tens
 
 PYBIND11_MODULE(_nsa_torch, m) {
   m.doc() = "The layer's operators on torch tensors (norm.py, rotary.py and projections.py are their public side)";
+  m.attr("abi_version") = NSA_ABI_VERSION;       // of the structs that this module fills
   // torch's wrapper: its exception types, and the interpreter's lock is released meanwhile
   using torch::wrap_pybind_function_no_gil;
   m.def("rms_norm", wrap_pybind_function_no_gil(rms_norm));
