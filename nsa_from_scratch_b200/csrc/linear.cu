@@ -17,7 +17,7 @@ int sm_count() {
 // ---------------------------------------------------------------- gradient through the activation, bias gradient
 // dz = dy * act' (slope: coded by the forward; NULL: no activation, nothing is written) and the column sums of dz
 // (part: a row of partial sums per block row; NULL: not wanted).  A thread owns 8 columns and walks the rows of its
-// block row, four under way at a time; bound by HBM: 20 us at 4001 x 4096 = 4.9 TB/s.
+// block row, four under way at a time; bound by HBM: 22 us at 4001 x 4096 = 4.5 TB/s.
 template <typename T>
 __global__ void __launch_bounds__(128) act_bwd_kernel(const void* __restrict__ dy, const uint16_t* __restrict__ slope, void* __restrict__ dz,
                                                       float* __restrict__ part, int M, int N, long long lddz, int rows, int vec, int vecz) {

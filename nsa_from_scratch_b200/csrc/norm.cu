@@ -7,7 +7,7 @@
 //
 // Bound by HBM.  A block owns a row: every element is read once, 16 bytes a load, and stays in registers (fp32) between
 // the sum and the result.  V = vectors of 8 elements per thread.  Sums are fp32, formed in a fixed order.
-// 16384 x 8192 bf16 with the residual and an fp8 result: 171 us = 5.5 TB/s (a plain copy reaches 6.5); 250 with one vector
+// 16384 x 8192 bf16 with the residual and an fp8 result: 172 us = 5.5 TB/s (a plain copy reaches 6.5); 250 with one vector
 // a thread, 173 with four, 178 with streaming loads and stores.  8189 x 4096 fp16: 46 us = 5.8 TB/s.
 #include "gemm.cuh"
 #include "tc5_ptx.cuh"

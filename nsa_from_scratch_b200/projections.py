@@ -21,7 +21,8 @@ def linear(x: Tensor, weight: Tensor, bias: Optional[Tensor] = None, *, activati
            residual: Optional[Tensor] = None) -> Tensor:
     """act(x weight^T + bias) + residual.  x [..., K], weight [N, K], bias [N], residual [..., N], all bf16 or all fp16;
     activation None, "silu", "gelu_tanh" or "relu".  Returns [..., N] in x's dtype: fp32 sums and epilogue, one rounding.
-    Differentiable wrt x, weight, bias and residual (act' is kept in 16 bits of its own for the backward)."""
+    Differentiable wrt x, weight, bias and residual (act' is kept in 16 bits of its own for the backward, whose dy act' is
+    rounded to x's dtype before the gradients' products)."""
     if not (x.is_contiguous() and weight.is_contiguous()):
         x, weight = ops._dense(x, "x"), ops._dense(weight, "weight")
     if bias is not None and not bias.is_contiguous():
@@ -50,7 +51,8 @@ def gated_mlp(x: Tensor, w_gate: Tensor, w_up: Tensor, w_down: Tensor, *, activa
               residual: Optional[Tensor] = None) -> Tensor:
     """(act(x w_gate^T) * (x w_up^T)) w_down^T + residual.  x and residual [..., N], w_gate and w_up [F, N], w_down [N, F], all bf16 or all
     fp16; activation as for `linear` (None: the plain product of the two).  fp32 sums; the gated product is rounded to x's
-    dtype between the two matrix products, the result once.  Differentiable wrt every tensor."""
+    dtype between the two matrix products, the result once.  Differentiable wrt every tensor (the gradients of the two inner
+    products are rounded to x's dtype before the gradients' products, their factors kept in 24 bits)."""
     if not (x.is_contiguous() and w_gate.is_contiguous() and w_up.is_contiguous() and w_down.is_contiguous()):
         x, w_gate, w_up, w_down = ops._dense(x, "x"), ops._dense(w_gate, "w_gate"), ops._dense(w_up, "w_up"), ops._dense(w_down, "w_down")
     if residual is not None and not residual.is_contiguous():
