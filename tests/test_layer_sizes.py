@@ -15,11 +15,11 @@ FP32 = 4
 def scratch(fn, args, without):
     """Bytes of workspace that the products of `without` take."""
     lib = L.load()
-    with_, rest = getattr(lib, fn)(C.byref(args)), None
+    with_ = getattr(lib, fn)(C.byref(args))
     for name in without:
         setattr(args, name, None)
     rest = getattr(lib, fn)(C.byref(args))
-    assert with_ >= 0 and rest >= 0, L.load().nsa_last_error()
+    assert with_ >= 0 and rest >= 0, lib.nsa_last_error()
     return with_ - rest
 
 
